@@ -282,6 +282,68 @@ int loom_hip_ssd_prologue_f16(const void* x, const void* dt, const void* A, cons
                               int64_t chunk_size, int64_t headdim, int64_t dstate, void* stream,
                               char* err, size_t errlen);
 
+/* ---- caches of different lengths -------------------------------------------
+ * What a serving loop does around a decoding step; the reference, whose
+ * @flash_decode reads caches of one length, has no counterpart.  Sequence b of
+ * B holds n = clamp(lens[b], 0, S) keys for each of its G KV heads: k [B,G,D,S]
+ * (keys transposed), v [B,G,S,D], in slots 0 .. n-1 of S; lens [B] int32 on the
+ * device.  What the slots behind a length hold (leftovers, NaN) is never used
+ * and, except where tokens are appended, left as it is.  All extents must be
+ * positive unless said otherwise, D a multiple of 8 up to 256 (else
+ * LOOM_HIP_EUNSUP), B*G <= 65535, S, P and T at most 2^30. */
+
+/* Appends new_k, new_v [B,T,G,D] (as a projection of B x T tokens gives them)
+ * behind every sequence's n keys: the first c = clamp(counts[b], 0, T) of its T
+ * tokens (all T with counts null); tokens past slot S-1 are dropped.  With
+ * weights [B,G,S] fp32 (null: none) the new keys' weights become zero.
+ * lens_out[b] = min(n + c, S); lens_out must not overlap lens or counts.  Moves
+ * 16-bit elements of either type. */
+int loom_hip_cache_append(void* k, void* v, void* weights, const void* lens, const void* new_k,
+                          const void* new_v, const void* counts, void* lens_out, int64_t B,
+                          int64_t G, int64_t D, int64_t S, int64_t T, void* stream, char* err,
+                          size_t errlen);
+
+/* Bytes of loom_hip_cache_decode's workspace (weights != 0: of a call that
+ * gathers weights).  It holds nothing between calls; calls that overlap in
+ * time need one each. */
+size_t loom_hip_cache_decode_workspace_bytes(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P,
+                                             int64_t S, int weights);
+
+/* One decoding step: row (b, g, h) of q, out [B,G,H,D] attends over the P keys
+ * of the prefix that every sequence shares (prefix_k [G,D,P], prefix_v [G,P,D];
+ * both null with P = 0) and the n keys of (b, g) together.  `scale` (finite and
+ * positive) multiplies q.k.  A row without keys, or whose scores are all -inf,
+ * gives zeros.  With weights and weights_out [B,G,S] fp32 (both or neither;
+ * they may be the same tensor, else must not overlap):
+ *   weights_out[b,g,j] = weights[b,g,j] + sum over h of row (b,g,h)'s softmax
+ * weight of own key j, for j < n; other elements are left as they are.
+ * S (P) not a multiple of 8 needs D*S (D*P) < 2^30. */
+int loom_hip_cache_decode(const void* prefix_k, const void* prefix_v, const void* k, const void* v,
+                          const void* q, const void* lens, const void* weights, void* weights_out,
+                          void* out, void* workspace, size_t workspace_bytes, int64_t B, int64_t G,
+                          int64_t H, int64_t D, int64_t P, int64_t S, float scale, void* stream,
+                          char* err, size_t errlen);
+int loom_hip_cache_decode_f16(const void* prefix_k, const void* prefix_v, const void* k,
+                              const void* v, const void* q, const void* lens, const void* weights,
+                              void* weights_out, void* out, void* workspace,
+                              size_t workspace_bytes, int64_t B, int64_t G, int64_t H, int64_t D,
+                              int64_t P, int64_t S, float scale, void* stream, char* err,
+                              size_t errlen);
+
+/* Cuts every (b, g) of more than `keep` keys to `keep` of them: its first
+ * `sinks`, its last `recent` and, of the others, those of the largest weights
+ * [B,G,S] (fp32; ties: the lowest slot; NaN below everything; only the order of
+ * the values counts).  Needs 1 <= keep <= S_out and recent + sinks <= keep.
+ * The kept keys' K, V and weights move, in the order of their slots, to the
+ * front of k_out [B,G,D,S_out], v_out [B,G,S_out,D], weights_out [B,G,S_out]
+ * (the rest of these is left as it is; no output overlaps an input);
+ * lens_out[b] = min(n, keep); index [B,G,keep] int32 receives the kept slots, -1
+ * behind them.  Moves 16-bit elements of either type. */
+int loom_hip_cache_evict(const void* k, const void* v, const void* weights, const void* lens,
+                         void* k_out, void* v_out, void* weights_out, void* lens_out, void* index,
+                         int64_t B, int64_t G, int64_t D, int64_t S, int64_t S_out, int64_t keep,
+                         int64_t recent, int64_t sinks, void* stream, char* err, size_t errlen);
+
 /* ---- MLIR memref descriptors ---------------------------------------------
  * A materialized variant is an MLIR function over memrefs; a caller lowered
  * through MLIR's C interface (`_mlir_ciface_<func>`, whose arguments are

@@ -53,12 +53,15 @@ _SIGS = {
     "loom_hip_ssd_bmm_chunk": [_vp] * 3 + [_i64] * 5 + [_vp, *_ERR],
     "loom_hip_ssd_chunk_state_passing": [_vp] * 5 + [_i64] * 7 + [_vp, *_ERR],
     "loom_hip_ssd_prologue": [_vp] * 8 + [_i64] * 7 + [_vp, *_ERR],
+    "loom_hip_cache_append": [_vp] * 8 + [_i64] * 5 + [_vp, *_ERR],
+    "loom_hip_cache_decode": [_vp] * 10 + [_sz] + [_i64] * 6 + [_f32, _vp, *_ERR],
+    "loom_hip_cache_evict": [_vp] * 9 + [_i64] * 8 + [_vp, *_ERR],
 }
 # f16 twins: same arguments, 16-bit tensors in IEEE binary16
 for _name in ("loom_hip_matmul", "loom_hip_batch_matmul", "loom_hip_split_k_matmul_gather",
               "loom_hip_attention", "loom_hip_flash_decode",
               "loom_hip_helion_mamba2_chunk_scan_kernel", "loom_hip_ssd_bmm_chunk",
-              "loom_hip_ssd_chunk_state_passing", "loom_hip_ssd_prologue"):
+              "loom_hip_ssd_chunk_state_passing", "loom_hip_ssd_prologue", "loom_hip_cache_decode"):
     _SIGS[_name + "_f16"] = _SIGS[_name]
 for _name, _args in _SIGS.items():
     _fn = getattr(_lib, _name)
@@ -68,6 +71,8 @@ _lib.loom_hip_split_k_workspace_bytes.argtypes = [_i64] * 4
 _lib.loom_hip_split_k_workspace_bytes.restype = _sz
 _lib.loom_hip_flash_decode_workspace_bytes.argtypes = [_i64] * 5
 _lib.loom_hip_flash_decode_workspace_bytes.restype = _sz
+_lib.loom_hip_cache_decode_workspace_bytes.argtypes = [_i64] * 6 + [ctypes.c_int]
+_lib.loom_hip_cache_decode_workspace_bytes.restype = _sz
 _lib.loom_hip_version.restype = ctypes.c_char_p
 _lib.loom_hip_materialize_variants.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p),
                                                ctypes.c_int, ctypes.c_char_p, _sz, *_ERR]
@@ -136,7 +141,8 @@ _lib.loom_hip_hw_spec.restype = ctypes.c_int
 EXPORTED = tuple(_SIGS) + tuple(_CIFACE) + ("loom_hip_peak_hbm_read", "loom_hip_peak_mfma_bf16", "loom_hip_synth") + ("loom_hip_dispatch_memref",
                                             "loom_hip_dispatch_memref_f16",
                                             "loom_hip_check_memref") + ("loom_hip_split_k_workspace_bytes",
-                           "loom_hip_flash_decode_workspace_bytes", "loom_hip_version",
+                           "loom_hip_flash_decode_workspace_bytes",
+                           "loom_hip_cache_decode_workspace_bytes", "loom_hip_version",
                            "loom_hip_materialize_variants", "loom_hip_parse_variant",
                            "loom_hip_dispatch", "loom_hip_dispatch_f16", "loom_hip_check_variant",
                            "loom_hip_workspace_bytes",
@@ -747,6 +753,217 @@ def ssd_prologue(x, dt, A, B, C, chunk_size, *, dA_cumsum=None, cb=None, prev_st
     args = [_check_device(a[0], a[1], dev) for a in spec]
     _call("loom_hip_ssd_prologue" + sfx, *args, b, nc, H, G, Q, P, N, _stream(x))
     return dt.view(b, H, nc, Q), dA_cumsum, cb, prev_states_T
+
+# ---------------------------------------------------------------------------
+# caches of different lengths: append, decode (shared prefix, weights), evict
+# ---------------------------------------------------------------------------
+
+_i32 = torch.int32
+
+# Tensor arguments in the entry points' order: (name, kind, shape from the
+# extents); kind "e" is the call's 16-bit type.  A trailing "?" marks those a
+# call may leave out (None).
+_CACHE_SPECS = {
+    "cache_append": lambda B, G, D, S, T: (
+        ("k", "e", (B, G, D, S)), ("v", "e", (B, G, S, D)), ("weights?", _fp32, (B, G, S)),
+        ("lens", _i32, (B,)), ("new_k", "e", (B, T, G, D)), ("new_v", "e", (B, T, G, D)),
+        ("counts?", _i32, (B,)), ("lens_out?", _i32, (B,))),
+    "cache_decode": lambda B, G, H, D, P, S: (
+        ("prefix_k?", "e", (G, D, P)), ("prefix_v?", "e", (G, P, D)), ("k", "e", (B, G, D, S)),
+        ("v", "e", (B, G, S, D)), ("q", "e", (B, G, H, D)), ("lens", _i32, (B,)),
+        ("weights?", _fp32, (B, G, S)), ("weights_out?", _fp32, (B, G, S)),
+        ("out?", "e", (B, G, H, D))),
+    "cache_evict": lambda B, G, D, S, So, keep: (
+        ("k", "e", (B, G, D, S)), ("v", "e", (B, G, S, D)), ("weights", _fp32, (B, G, S)),
+        ("lens", _i32, (B,)), ("k_out?", "e", (B, G, D, So)), ("v_out?", "e", (B, G, So, D)),
+        ("weights_out?", _fp32, (B, G, So)), ("lens_out?", _i32, (B,)),
+        ("index?", _i32, (B, G, keep))),
+}
+
+
+@functools.lru_cache(maxsize=1024)
+def _cache_plan(func: str, sig: tuple, extra: tuple):
+    """(entry point, its name, extents, 16-bit type) of a call's signature, which
+    holds (dtype, shape) of every tensor argument (None where it is left out);
+    kept by value for the last 1024 signatures.  Raises what is wrong with it."""
+    at = {"cache_append": (0, 4), "cache_decode": (2, 4), "cache_evict": (0, 0)}[func]
+    names = [a[0].rstrip("?") for a in _CACHE_SPECS[func](*(0,) * (5 if func == "cache_append"
+                                                                    else 6))]
+    for i in at:
+        if sig[i] is None or len(sig[i][1]) != 4:
+            raise ValueError(f"{func}: {names[i]} must have 4 dims, got "
+                             f"{'None' if sig[i] is None else f'shape {tuple(sig[i][1])}'}")
+    B, G, D, S = sig[at[0]][1]
+    if func == "cache_append":
+        dims = (B, G, D, S, sig[4][1][1])
+    elif func == "cache_decode":
+        if (sig[0] is None) != (sig[1] is None):
+            raise ValueError("cache_decode: prefix_k and prefix_v are given together or not at all")
+        if sig[6] is None and sig[7] is not None:
+            raise ValueError("cache_decode: weights_out needs weights")
+        if sig[0] is not None and len(sig[0][1]) != 3:
+            raise ValueError(f"cache_decode: prefix_k must have 3 dims, got shape "
+                             f"{tuple(sig[0][1])}")
+        dims = (B, G, sig[4][1][2], D, 0 if sig[0] is None else sig[0][1][2], S)
+    else:
+        keep, So = extra
+        for i, axis in ((4, 3), (5, 2), (6, 2)):    # the capacity of the caches moved to
+            if So is None and sig[i] is not None and len(sig[i][1]) > axis:
+                So = sig[i][1][axis]
+        dims = (B, G, D, S, S if So is None else So, keep)
+    e = sig[at[0]][0]
+    if e not in (_bf16, _f16):
+        raise TypeError(f"{names[at[0]]}: expected torch.bfloat16 or torch.float16, got {e}")
+    for s, (name, kind, shape) in zip(sig, _CACHE_SPECS[func](*dims)):
+        if s is None:
+            if not name.endswith("?"):
+                raise TypeError(f"{name}: expected a torch.Tensor, got NoneType")
+            continue
+        want = e if kind == "e" else kind
+        if s[0] != want:
+            raise TypeError(f"{name.rstrip('?')}: expected {want}, got {s[0]}")
+        if tuple(s[1]) != shape:
+            raise ValueError(f"{name.rstrip('?')}: expected shape {shape}, got {tuple(s[1])}")
+    name = "loom_hip_" + func + ("_f16" if e == _f16 and func == "cache_decode" else "")
+    return getattr(_lib, name), name, dims, e, names
+
+
+def _cache_enter(func: str, tensors, extra=()):
+    """(plan, device index) of a call; raises what is wrong with a tensor."""
+    sig = []
+    for t in tensors:
+        if t is None:
+            sig.append(None)
+        elif isinstance(t, torch.Tensor):
+            sig.append((t.dtype, t.shape))
+        else:
+            raise TypeError(f"{func}: expected torch.Tensors, got {type(t).__name__}")
+    plan = _cache_plan(func, tuple(sig), extra)
+    dev = None
+    for t, name in zip(tensors, plan[4]):
+        if t is None:
+            continue
+        i = t.get_device()
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: must be contiguous")
+        if i < 0:
+            raise ValueError(f"{name}: must be on a ROCm device, got {t.device}")
+        if dev is None:
+            dev = i
+        elif i != dev:
+            raise ValueError(f"{name}: on {t.device}, the call's tensors are on cuda:{dev}")
+    return plan, dev
+
+
+def _cache_run(plan, dev, *args):
+    """The entry point on the current stream of the tensors' device, which
+    becomes the current one for the call where it is not."""
+    if dev == torch.cuda.current_device():
+        _run(plan, *args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _run(plan, *args, _raw_stream(dev))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def cache_append(k, v, lens, new_k, new_v, lens_out=None, *, counts=None, weights=None):
+    """Appends new tokens to caches of different lengths, in place.
+
+    k [B,G,D,S] (keys transposed), v [B,G,S,D], lens [B] int32 (the lengths
+    before), new_k, new_v [B,T,G,D] -> lens_out [B], the lengths after.  Sequence
+    b takes its first ``counts[b]`` tokens (int32; all T by default); tokens past
+    the capacity S are dropped.  With ``weights`` [B,G,S] (see cache_decode) the
+    new keys' become zero.  ``lens_out`` must not be ``lens``."""
+    plan, dev = _cache_enter("cache_append", (k, v, weights, lens, new_k, new_v, counts, lens_out))
+    if lens_out is None:
+        lens_out = torch.empty_like(lens)
+    _cache_run(plan, dev, k.data_ptr(), v.data_ptr(), _ptr(weights), lens.data_ptr(),
+               new_k.data_ptr(), new_v.data_ptr(), _ptr(counts), lens_out.data_ptr(), *plan[2])
+    return lens_out
+
+
+@functools.lru_cache(maxsize=1024)
+def cache_decode_workspace_bytes(B, G, H, D, P, S, weights=False) -> int:
+    return int(_lib.loom_hip_cache_decode_workspace_bytes(B, G, H, D, P, S, int(bool(weights))))
+
+
+def cache_decode_workspace(B, G, H, D, P, S, weights, device):
+    """A cache_decode workspace (uint8 tensor) for these extents."""
+    return torch.empty(max(cache_decode_workspace_bytes(B, G, H, D, P, S, weights), 4),
+                       dtype=torch.uint8, device=device)
+
+
+def cache_decode(k, v, q, lens, out=None, workspace=None, *, prefix_k=None, prefix_v=None,
+                 weights=None, weights_out=None, scale=None):
+    """One decoding step over caches of different lengths.
+
+    k [B,G,D,S] (keys transposed), v [B,G,S,D], q [B,G,H,D] (H query heads to
+    each of G KV heads), lens [B] int32 -> out [B,G,H,D].  Every sequence also
+    attends to the prefix that all share, prefix_k [G,D,P] and prefix_v [G,P,D],
+    whose scores are computed for the whole batch at once.  With ``weights``
+    [B,G,S] fp32 each own key's softmax weight, summed over the H heads, is
+    added to it (into ``weights_out`` where given).  ``scale`` defaults to
+    1/sqrt(D)."""
+    if weights_out is None:
+        weights_out = weights
+    plan, dev = _cache_enter("cache_decode", (prefix_k, prefix_v, k, v, q, lens, weights,
+                                              weights_out, out))
+    dims = plan[2]
+    if scale is None:
+        scale = 1.0 / math.sqrt(dims[3]) if dims[3] > 0 else 1.0
+    if out is None:
+        out = torch.empty_like(q)
+    need = cache_decode_workspace_bytes(*dims, weights is not None)
+    if workspace is None:
+        workspace = torch.empty(max(need, 4), dtype=torch.uint8, device=q.device)
+        wp = workspace.data_ptr()
+    else:
+        wp = _check_workspace(workspace, need, q.device, "cache_decode")
+    # P == 0: an empty prefix is no prefix
+    pk, pv = (prefix_k.data_ptr(), prefix_v.data_ptr()) if dims[4] else (None, None)
+    _cache_run(plan, dev, pk, pv, k.data_ptr(), v.data_ptr(), q.data_ptr(), lens.data_ptr(),
+               _ptr(weights), _ptr(weights_out), out.data_ptr(), wp, workspace.numel(), *dims,
+               float(scale))
+    return out
+
+
+def cache_evict(k, v, weights, lens, keep, *, recent=0, sinks=0, capacity=None, k_out=None,
+                v_out=None, weights_out=None, lens_out=None, index=None):
+    """Cuts caches of more than ``keep`` keys to their first ``sinks``, their
+    last ``recent`` and, of the others, the keys of the largest ``weights``
+    [B,G,S] (as cache_decode gathers them; ties: the lowest slot).
+
+    k [B,G,D,S], v [B,G,S,D], lens [B] -> (k_out [B,G,D,capacity], v_out
+    [B,G,capacity,D], weights_out [B,G,capacity], lens_out [B], index
+    [B,G,keep]): the kept keys in the order of their slots at the front (what
+    lies behind them is left as it is), the lengths min(lens, keep), and the
+    slots they came from, -1 behind them.  ``capacity`` defaults to that of the
+    outputs given, else S."""
+    keep, recent, sinks = int(keep), int(recent), int(sinks)
+    plan, dev = _cache_enter("cache_evict", (k, v, weights, lens, k_out, v_out, weights_out,
+                                             lens_out, index),
+                             (keep, None if capacity is None else int(capacity)))
+    B, G, D, S, So = plan[2][:5]
+    if min(B, G, D, So, keep) <= 0:
+        raise ValueError("cache_evict: extents and keep must be positive")
+    if k_out is None:
+        k_out = torch.empty((B, G, D, So), dtype=plan[3], device=k.device)
+    if v_out is None:
+        v_out = torch.empty((B, G, So, D), dtype=plan[3], device=k.device)
+    if weights_out is None:
+        weights_out = torch.empty((B, G, So), dtype=_fp32, device=k.device)
+    if lens_out is None:
+        lens_out = torch.empty_like(lens)
+    if index is None:
+        index = torch.empty((B, G, keep), dtype=_i32, device=k.device)
+    _cache_run(plan, dev, k.data_ptr(), v.data_ptr(), weights.data_ptr(), lens.data_ptr(),
+               k_out.data_ptr(), v_out.data_ptr(), weights_out.data_ptr(), lens_out.data_ptr(),
+               index.data_ptr(), B, G, D, S, So, keep, recent, sinks)
+    return k_out, v_out, weights_out, lens_out, index
+
 
 # ---------------------------------------------------------------------------
 # materialization contract and by-name dispatch
