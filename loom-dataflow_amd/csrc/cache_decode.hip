@@ -17,6 +17,9 @@
 
 namespace {
 
+constexpr int kThreads = 256;     // four waves
+constexpr int kKeys = 64;         // keys per stage
+
 struct StepParams {
   const uint16_t* pk;
   const uint16_t* pv;
@@ -27,89 +30,656 @@ struct StepParams {
   const float* w;
   float* w_out;
   uint16_t* out;
-  float* score;   // [B G H, P + S], log2 domain
-  float* ml;      // [B G H, 2]: maximum and sum of a row
-  int B, G, H, D, P, S;
-  float c2;       // scale * log2(e)
+  int2* plan;       // [B]: a sequence's first chunk, and the chunks' keys
+  f32x4_t* ml;      // per partial row: base, sum of the rounded p, sum of p
+  float* o;         // per partial row: sum of p v, D values
+  float* score;     // [B G, H, Sp] scores of the own keys, log2 domain
+  int B, G, H, D, P, S, Sp;
+  int nht;          // row tiles of a (b, g)'s H heads
+  int chunks;       // chunks that the whole batch aims at
+  int ntp, nsp, tile_p;   // the prefix: row tiles per head, splits, keys of one
+  int nprefix;      // workgroups of the prefix
+  float c2;         // scale * log2(e)
 };
 
-constexpr int kThreads = 256;
+LOOM_DEV int seq_len(const StepParams& p, int b) { return min(max(p.lens[b], 0), p.S); }
 
-// One workgroup per row (b, g, h): the scores (a thread per key), their
-// maximum and sum, then the values' weighted sum (a thread per d).
-template <bool F16>
-__global__ void __launch_bounds__(kThreads) cache_row_kernel(StepParams p) {
-  __shared__ float s_q[256], s_red[kThreads / 64], s_o[kThreads];
-  const int64_t row = blockIdx.x;
-  const int64_t bg = row / p.H;
-  const int b = (int)(bg / p.G), g = (int)(bg % p.G);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int D = p.D, P = p.P, n = min(max(p.lens[b], 0), p.S), N = P + n;
-  const uint16_t* const pk = p.pk + (int64_t)g * D * P;
-  const uint16_t* const pv = p.pv + (int64_t)g * P * D;
-  const uint16_t* const k = p.k + bg * D * p.S;
-  const uint16_t* const v = p.v + bg * p.S * D;
-  float* const sc = p.score + row * (P + p.S);
-  if (tid < D) s_q[tid] = lo16<F16>(p.q[row * D + tid]);
-  __syncthreads();
-  float m = -INFINITY;
-  for (int j = tid; j < N; j += kThreads) {
-    float s = 0.f;
-    if (j < P)
-      for (int d = 0; d < D; ++d) s += s_q[d] * lo16<F16>(pk[(int64_t)d * P + j]);
-    else
-      for (int d = 0; d < D; ++d) s += s_q[d] * lo16<F16>(k[(int64_t)d * p.S + j - P]);
-    s *= p.c2;
-    sc[j] = s;
-    m = fmaxf(m, s);
-  }
-  m = wave_max(m);
-  if (lane == 0) s_red[wave] = m;
-  __syncthreads();
-  for (int x = 0; x < kThreads / 64; ++x) m = fmaxf(m, s_red[x]);
-  const float base = m == -INFINITY ? 0.f : m;
-  __syncthreads();
-  float l = 0.f;
-  for (int j = tid; j < N; j += kThreads) l += exp2f(sc[j] - base);
-  l = wave_sum(l);
-  if (lane == 0) s_red[wave] = l;
-  __syncthreads();
-  l = 0.f;
-  for (int x = 0; x < kThreads / 64; ++x) l += s_red[x];
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  if (tid == 0) {
-    p.ml[2 * row] = base;
-    p.ml[2 * row + 1] = inv;
-  }
-  for (int d0 = 0; d0 < D; d0 += 64) {
-    const int d = d0 + lane;
-    float o = 0.f;
-    if (d < D)
-      for (int j = wave; j < N; j += kThreads / 64) {
-        const float e = exp2f(sc[j] - base);
-        const uint32_t x = j < P ? pv[(int64_t)j * D + d] : v[(int64_t)(j - P) * D + d];
-        o += e * lo16<F16>(x);
+// ---------------------------------------------------------------------------
+// One part: up to RT query rows against the keys [s0, s1) of one K, V.
+// ---------------------------------------------------------------------------
+LOOM_DEV int ck_swz(int d) { return (2 * (d & 3)) ^ (2 * ((d >> 3) & 1)); }
+template <int D>
+LOOM_DEV int cv_swz(int k) { return D >= 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3); }
+
+struct Part {
+  const uint16_t* k;    // [D][ld]
+  const uint16_t* v;    // [ld][D]
+  int ld;               // keys of a K row
+  int s0, s1;           // this part's keys, s0 a multiple of 64
+  int rows;             // query rows
+  int i0;               // first row: of the (b, g)'s heads, or of head g's B H rows
+  int g;                // the KV head of a prefix part, -1: rows are consecutive
+  int64_t out0;         // partial row of row 0 (own part)
+  float* score;         // scores of row 0, Sp apart, or null
+};
+
+// Row lr of a part in q's [B G H] rows.  A prefix's rows are all sequences'
+// heads of its g.
+LOOM_DEV int64_t part_row(const StepParams& p, const Part& a, int lr) {
+  const int i = a.i0 + lr;
+  if (a.g < 0 || p.G == 1) return i;
+  const int b = i / p.H;
+  return ((int64_t)b * p.G + a.g) * p.H + (i - b * p.H);
+}
+
+template <int D, bool F16, bool WT, int QT, int KG, bool KREG>
+LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
+  constexpr int W = kThreads / 64;
+  constexpr int RT = 16 * QT * W / KG;          // rows of a workgroup
+  constexpr int K_BYTES = D * kKeys * 2, V_BYTES = kKeys * D * 2;
+  constexpr int STAGE = K_BYTES + V_BYTES;
+  constexpr int K_INSTR = K_BYTES / 1024 / W, V_INSTR = V_BYTES / 1024 / W;
+  constexpr int VROW = D * 2, V_ROWS_PER_I = 1024 / VROW;
+  constexpr int DSTEPS = D / 32, DT = D / 16;
+  constexpr int Q_INSTR = RT * D * 2 / 1024 / W;
+  static_assert(RT * D * 2 <= STAGE, "the queries arrive in the second stage");
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int a4 = r >> 2, c4 = r & 3;            // transposed-read lane roles
+  const int qw = wave / KG, kh = wave % KG;     // query rows and key half of this wave
+  const int Dr = p.D, ld = a.ld, s0 = a.s0, s1 = a.s1;
+  const uint16_t* __restrict__ kg = a.k;
+  const uint16_t* __restrict__ vg = a.v;
+  const int nblk = (s1 - s0 + kKeys - 1) / kKeys;
+  const bool active = 16 * QT * qw < a.rows;    // this wave has rows
+
+  auto stK = [&](int s) { return (lds_char_t*)(smem + s * STAGE); };
+  auto stV = [&](int s) { return (lds_char_t*)(smem + s * STAGE + K_BYTES); };
+  // ---- DMA of block `blk` into stage s: K pieces past the row's end are
+  // clamped (their keys are masked), rows d >= Dr come from zeros; V rows past
+  // s1 repeat the last one, whose weight there is zero (slots behind a length
+  // may hold NaN, and 0 NaN is NaN)
+  auto issue = [&](int s, int blk) {
+    const int kv0 = s0 + blk * kKeys;
+    const uint32_t lk = lds_addr(stK(s)), lv = lds_addr(stV(s));
+    if constexpr (!KREG) {
+#pragma unroll
+      for (int i = 0; i < K_INSTR; ++i) {
+        const int j = wave * K_INSTR + i;
+        const int d = j * 8 + lane / 8;
+        const int key = min(kv0 + ((lane % 8) ^ ck_swz(d)) * 8, ld - 8);
+        if (j * 8 < Dr)                                 // wave-uniform
+          dma_load16(kg + (int64_t)d * ld + key, lk + j * 1024);
+        else
+          dma_load16(loom_zero_kb + lane * 4, lk + j * 1024);
       }
-    s_o[tid] = o;
-    __syncthreads();
-    if (wave == 0 && d < D) {
-      for (int x = 1; x < kThreads / 64; ++x) o += s_o[x * 64 + lane];
-      p.out[row * D + d] = (uint16_t)cvt16<F16>(o * inv);
     }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V_INSTR; ++i) {
+      const int j = wave * V_INSTR + i;
+      const int kr = j * V_ROWS_PER_I + lane / (D / 8);
+      const int c = min((lane % (D / 8)) ^ cv_swz<D>(kr), Dr / 8 - 1);
+      const int key = min(kv0 + kr, s1 - 1);
+      dma_load16(vg + (int64_t)key * Dr + c * 8, lv + j * 1024);
+    }
+  };
+  // ---- KREG (ld not a multiple of 8): K pieces through registers
+  const rsrc_t krs = make_rsrc(kg, KREG ? (uint32_t)(Dr * ld * 2) : 0u);
+  u32x4_t kr[KREG ? K_INSTR : 1];
+  auto kload = [&](int blk) {
+    const int kv0 = s0 + blk * kKeys;
+#pragma unroll
+    for (int i = 0; i < K_INSTR; ++i) {
+      const int j = wave * K_INSTR + i;
+      const int d = j * 8 + lane / 8;
+      kr[i] = j * 8 < Dr ? row_piece8(krs, ld, d, kv0 + ((lane % 8) ^ ck_swz(d)) * 8)
+                         : u32x4_t{0u, 0u, 0u, 0u};
+    }
+  };
+  auto kstore = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < K_INSTR; ++i)
+      *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(
+          stK(s) + (wave * K_INSTR + i) * 1024 + lane * 16) = kr[i];
+  };
+
+  // ---- the queries into the second stage (rows past the part's repeat its
+  // last, elements past Dr are zeroed when read), then the first block
+  lds_char_t* const sq = stK(1);
+#pragma unroll
+  for (int i = 0; i < Q_INSTR; ++i) {
+    const int j = wave * Q_INSTR + i;
+    const int e = j * 512 + lane * 8;
+    const int64_t row = part_row(p, a, min(e / D, a.rows - 1));
+    dma_load16(p.q + row * Dr + min(e % D, Dr - 8), lds_addr(sq) + j * 1024);
+  }
+  if constexpr (KREG) {
+    kload(0);
+    kstore(0);
+  }
+  issue(0, 0);
+
+  u32x4_t qf[DSTEPS][QT];
+  const float c2 = p.c2;
+  float m_run[QT], lx[QT];
+  f32x4_t ot[DT][QT], lacc[QT];
+  const u32x4_t ones = u32x4_t{kOnePair<F16>, kOnePair<F16>, kOnePair<F16>, kOnePair<F16>};
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m_run[qt] = lx[qt] = 0.f;
+    lacc[qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) ot[dt][qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  bool first = true;
+
+  // ---- 32 keys (half h of block blk in stage s) against this wave's rows
+  auto half = [&](int s, int blk, int h) {
+    const int kv0 = s0 + blk * kKeys + 32 * h;
+    const lds_char_t* ks = stK(s);
+    const lds_char_t* vs = stV(s);
+    // st[j][qt][i]: key kv0 + 16 j + 4 g + i, row 16 qt + r of this wave
+    f32x4_t st[2][QT];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) st[j][qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ds = 0; ds < DSTEPS; ++ds) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int d = ds * 32 + g * 8 + a4;
+        const int ch = (2 * (2 * h + j) + (c4 >> 1)) ^ ck_swz(d);
+        const lds_char_t* q = ks + d * (kKeys * 2) + ch * 16 + (c4 & 1) * 8;
+        const u32x2_t lo = lds_read_tr16(q);
+        const u32x2_t hi = lds_read_tr16(q + 4 * (kKeys * 2));
+        const u32x4_t kf = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) st[j][qt] = mfma16t<F16>(kf, qf[ds][qt], st[j][qt]);
+      }
+    }
+    const bool edge = kv0 + 32 > s1;
+    if constexpr (WT) {
+      if (a.score) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          const int lr = 16 * (QT * qw + qt) + r;
+          if (lr < a.rows) {
+            float* to = a.score + (int64_t)lr * p.Sp + kv0 + 4 * g;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              *reinterpret_cast<f32x4_t*>(to + 16 * j) = st[j][qt] * c2;
+          }
+        }
+      }
+    }
+    // log2-domain scores relative to the base; keys past s1 are -inf
+    float lmax[QT];
+    bool big = false;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = __builtin_fmaf(st[j][qt][i], c2, -m_run[qt]);
+          if (edge && kv0 + 16 * j + 4 * g + i >= s1) v = -INFINITY;
+          st[j][qt][i] = v;
+          mx = fmaxf(mx, v);
+        }
+      lmax[qt] = mx;
+      big |= mx > 8.f;
+    }
+    // lazy online softmax: a row's base is set by its first block with a
+    // finite score and moves (O and the sums rescale) when one rises 2^8 above
+    if (first || __builtin_amdgcn_ballot_w64(big) != 0) {
+      bool unset_left = false;
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        float mx = lmax[qt];
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const bool unset = first && lacc[qt][0] == 0.f;
+        const float shift = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
+        const float alpha = unset ? 1.f : fast_exp2(-shift);
+        lacc[qt] *= alpha;
+        lx[qt] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) ot[dt][qt] *= alpha;
+        m_run[qt] += shift;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) st[j][qt] -= shift;
+        unset_left |= unset && mx == -INFINITY;
+      }
+      first = __builtin_amdgcn_ballot_w64(unset_left) != 0;
+    }
+    u32x4_t pf[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      f32x4_t e0, e1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e0[i] = fast_exp2(st[0][qt][i]);
+        e1[i] = fast_exp2(st[1][qt][i]);
+      }
+      if constexpr (WT)
+        lx[qt] += ((e0[0] + e0[1]) + (e0[2] + e0[3])) + ((e1[0] + e1[1]) + (e1[2] + e1[3]));
+      pf[qt] = u32x4_t{pack2<F16>(e0[0], e0[1]), pack2<F16>(e0[2], e0[3]),
+                       pack2<F16>(e1[0], e1[1]), pack2<F16>(e1[2], e1[3])};
+      lacc[qt] = mfma16t<F16>(ones, pf[qt], lacc[qt]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int k0r = 32 * h + 4 * g + a4;
+      const int ch = (2 * dt + (c4 >> 1)) ^ cv_swz<D>(k0r);
+      const lds_char_t* q = vs + k0r * VROW + ch * 16 + (c4 & 1) * 8;
+      const u32x2_t lo = lds_read_tr16(q);
+      const u32x2_t hi = lds_read_tr16(q + 16 * VROW);
+      const u32x4_t vf = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) ot[dt][qt] = mfma16t<F16>(vf, pf[qt], ot[dt][qt]);
+    }
+  };
+
+  for (int it = 0; it < nblk; ++it) {
+    const int s = it & 1;
+    lds_order();
+    LOOM_WAIT_VMCNT(0);
+    LOOM_WAIT_LGKM0();
+    barrier_nofence();
+    if (it == 0) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int ds = 0; ds < DSTEPS; ++ds) {
+          const int lr = 16 * (QT * qw + qt) + r;
+          const u32x4_t raw = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
+              sq + (lr * D + ds * 32 + g * 8) * 2);
+          qf[ds][qt] = ds * 32 + g * 8 < Dr ? raw : u32x4_t{0u, 0u, 0u, 0u};
+        }
+      LOOM_WAIT_LGKM0();      // the second stage is overwritten next
+      barrier_nofence();
+    }
+    const bool ahead = it + 1 < nblk;
+    if constexpr (KREG) {
+      if (ahead) kload(it + 1);
+    }
+    if (ahead) issue(s ^ 1, it + 1);
+    if (active) {
+      if constexpr (KG == 2) {
+        half(s, it, kh);
+      } else {
+        half(s, it, 0);
+        half(s, it, 1);
+      }
+    }
+    if constexpr (KREG) {
+      if (ahead) kstore(s ^ 1);
+    }
+  }
+
+  // ---- the sums of the four lane groups, each of which held other keys
+  if constexpr (WT) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      lx[qt] += __shfl_xor(lx[qt], 16);
+      lx[qt] += __shfl_xor(lx[qt], 32);
+    }
+  }
+  // ---- KG 2: the pair's second wave hands its state over through the idle
+  // stages, lane by lane (both hold the same rows and columns); a half without
+  // a key of finite score (l = 0) takes no part
+  if constexpr (KG == 2) {
+    constexpr int SLOT = QT * (DT + 1) * 64;
+    static_assert(W / 2 * SLOT * 16 <= 2 * STAGE, "merge area");
+    LOOM_WAIT_LGKM0();
+    barrier_nofence();
+    f32x4_t* const mg = reinterpret_cast<f32x4_t*>(smem) + qw * SLOT + lane;
+    if (kh == 1) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) mg[(qt * (DT + 1) + dt) * 64] = ot[dt][qt];
+        mg[(qt * (DT + 1) + DT) * 64] = f32x4_t{lacc[qt][0], m_run[qt], lx[qt], 0.f};
+      }
+    }
+    LOOM_WAIT_LGKM0();
+    barrier_nofence();
+    if (kh == 1) return;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const f32x4_t lm = mg[(qt * (DT + 1) + DT) * 64];
+      const float l0 = lacc[qt][0], l1 = lm[0], m0 = m_run[qt], m1 = lm[1];
+      const float M = l0 != 0.f ? (l1 != 0.f ? fmaxf(m0, m1) : m0) : m1;
+      const float f0 = l0 != 0.f ? fast_exp2(m0 - M) : 0.f;
+      const float f1 = l1 != 0.f ? fast_exp2(m1 - M) : 0.f;
+      lacc[qt][0] = l0 * f0 + l1 * f1;
+      lx[qt] = lx[qt] * f0 + lm[2] * f1;
+      m_run[qt] = M;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        ot[dt][qt] = ot[dt][qt] * f0 + mg[(qt * (DT + 1) + dt) * 64] * f1;
+    }
+  }
+  // ---- (base, sums, O) of every row: ot[dt][qt][i] is d = 16 dt + 4 g + i
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int lr = 16 * (QT * qw + qt) + r;
+    if (lr < a.rows) {
+      const int64_t row = a.out0 + (a.g < 0 ? lr : part_row(p, a, lr));
+      if (g == 0) p.ml[row] = f32x4_t{m_run[qt], lacc[qt][0], lx[qt], 0.f};
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        if (dt * 16 + 4 * g < Dr)
+          *reinterpret_cast<f32x4_t*>(p.o + row * Dr + dt * 16 + 4 * g) = ot[dt][qt];
+    }
   }
 }
 
-__global__ void __launch_bounds__(256) cache_weight_kernel(StepParams p) {
-  const int64_t bg = blockIdx.y;
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= min(max(p.lens[bg / p.G], 0), p.S)) return;
-  float a = 0.f;
-  for (int h = 0; h < p.H; ++h) {
-    const int64_t row = bg * p.H + h;
-    a += exp2f(p.score[row * (p.P + p.S) + p.P + j] - p.ml[2 * row]) * p.ml[2 * row + 1];
+LOOM_DEV int64_t wave_sum64(int64_t v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+// Where chunk c of the batch's own keys lies: sequences in order, each cut into
+// chunks of t keys, t the multiple of 64 that gives about p.chunks of them over
+// all sequences whatever their lengths.  Every workgroup works it out from the
+// lengths (one load per 256 sequences), so nothing is planned on the host and a
+// replayed graph follows them.
+struct Chunk {
+  int b, i, n, t;   // sequence (-1: none), its chunk, its length, keys of a chunk
+};
+LOOM_DEV Chunk find_chunk(const StepParams& p, int c) {
+  __shared__ int64_t s_sum[kThreads / 64];
+  __shared__ int s_cnt[kThreads / 64], s_b, s_i, s_n;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t total = 0;
+  for (int b = tid; b < p.B; b += kThreads) total += seq_len(p, b);
+  total = wave_sum64(total);
+  if (lane == 0) s_sum[wave] = total;
+  if (tid == 0) s_b = -1;
+  __syncthreads();
+  total = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  const int t = (int)min((int64_t)1 << 30,
+                         max((int64_t)1, ((total + p.chunks - 1) / p.chunks + kKeys - 1) / kKeys) *
+                             kKeys);
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    const int b = b0 + tid;
+    const int n = b < p.B ? seq_len(p, b) : 0;
+    const int cnt = (n + t - 1) / t;
+    int inc = cnt;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int o = __shfl_up(inc, m);
+      if (lane >= m) inc += o;
+    }
+    if (lane == 63) s_cnt[wave] = inc;
+    __syncthreads();
+    int before = base;
+    for (int x = 0; x < wave; ++x) before += s_cnt[x];
+    const int at = before + inc - cnt;
+    if (c >= at && c < at + cnt) {
+      s_b = b;
+      s_i = c - at;
+      s_n = n;
+    }
+    base += s_cnt[0] + s_cnt[1] + s_cnt[2] + s_cnt[3];
+    __syncthreads();
+    if (c < base) break;
   }
-  p.w_out[bg * p.S + j] = p.w[bg * p.S + j] + a;
+  return Chunk{__builtin_amdgcn_readfirstlane(s_b), __builtin_amdgcn_readfirstlane(s_i),
+               __builtin_amdgcn_readfirstlane(s_n), __builtin_amdgcn_readfirstlane(t)};
+}
+
+// ids received round-robin by the eight XCDs -> contiguous ranges for each
+LOOM_DEV int xcd_range(int id, int n) {
+  const int x = id & 7, q = n >> 3, r = n & 7;
+  return x * q + min(x, r) + (id >> 3);
+}
+
+template <int D, bool F16, bool WT>
+__global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(StepParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[2 * 4 * kKeys * D];
+  Part a;
+  int tile;                 // rows of the tile this part runs on
+  const int id = blockIdx.x;
+  if (id < p.nprefix) {     // a prefix part: row tiles of the same keys side by side
+    const int x = xcd_range(id, p.nprefix);
+    const int rt = x % p.ntp, s = x / p.ntp % p.nsp, g = x / (p.ntp * p.nsp);
+    const int rows = p.B * p.H;
+    tile = rows <= 32 ? 32 : 128;
+    a.k = p.pk + (int64_t)g * p.D * p.P;
+    a.v = p.pv + (int64_t)g * p.P * p.D;
+    a.ld = p.P;
+    a.s0 = s * p.tile_p;
+    a.s1 = min(p.P, a.s0 + p.tile_p);
+    a.i0 = rt * 128;
+    a.rows = min(128, rows - a.i0);
+    a.g = g;
+    a.out0 = (int64_t)s * p.B * p.G * p.H;
+    a.score = nullptr;
+  } else {                  // a chunk of a sequence's own keys
+    const int x = id - p.nprefix, per = p.G * p.nht;
+    const Chunk c = find_chunk(p, x / per);
+    if (c.b < 0) return;
+    const int g = x % per / p.nht, ht = x % p.nht;
+    const int64_t bg = (int64_t)c.b * p.G + g;
+    if (c.i == 0 && x % per == 0 && threadIdx.x == 0) p.plan[c.b] = int2{x / per, c.t};
+    tile = p.H <= 32 ? 32 : 128;
+    a.k = p.k + bg * p.D * p.S;
+    a.v = p.v + bg * p.S * p.D;
+    a.ld = p.S;
+    a.s0 = c.i * c.t;
+    a.s1 = min(c.n, a.s0 + c.t);
+    a.g = -1;
+    a.rows = min(128, p.H - ht * 128);
+    a.i0 = (int)(bg * p.H) + ht * 128;
+    a.out0 = (int64_t)p.nsp * p.B * p.G * p.H + ((int64_t)(x / per) * p.G + g) * p.H + ht * 128;
+    a.score = WT ? p.score + (bg * p.H + ht * 128) * p.Sp : nullptr;
+  }
+  const bool kreg = a.ld % 8 != 0;
+  if (tile == 32) {
+    if (kreg) run_part<D, F16, WT, 1, 2, true>(p, a, smem);
+    else run_part<D, F16, WT, 1, 2, false>(p, a, smem);
+  } else {
+    if (kreg) run_part<D, F16, WT, 2, 1, true>(p, a, smem);
+    else run_part<D, F16, WT, 2, 1, false>(p, a, smem);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The parts of a row joined, and the weights
+// ---------------------------------------------------------------------------
+struct Splits {             // a row's partial rows: the prefix's, then its own
+  int64_t R, row, own0;     // own0 + s G H: its own part s
+  int nsp, n, GH;
+};
+LOOM_DEV Splits row_splits(const StepParams& p, int b, int g, int h) {
+  Splits s;
+  s.R = (int64_t)p.B * p.G * p.H;
+  s.row = ((int64_t)b * p.G + g) * p.H + h;
+  const int len = seq_len(p, b);
+  const int2 pl = len > 0 ? p.plan[b] : int2{0, 1};
+  s.nsp = p.nsp;
+  s.GH = p.G * p.H;
+  s.own0 = s.nsp * s.R + ((int64_t)pl.x * p.G + g) * p.H + h;
+  s.n = s.nsp + (len + pl.y - 1) / pl.y;
+  return s;
+}
+LOOM_DEV int64_t split_at(const Splits& s, int u) {
+  return u < s.nsp ? u * s.R + s.row : s.own0 + (int64_t)(u - s.nsp) * s.GH;
+}
+
+constexpr int kJoinMax = 64;
+
+template <bool F16>
+LOOM_DEV void join_row(const StepParams& p) {
+  constexpr int CH = 8;
+  __shared__ f32x4_t s_acc[256];
+  __shared__ float s_m[kJoinMax], s_den[kJoinMax];
+  const int D = p.D, row = blockIdx.x;
+  const int bg = row / p.H, h = row - bg * p.H, b = bg / p.G, g = bg - b * p.G;
+  const Splits sp = row_splits(p, b, g, h);
+  const int ns = sp.n;
+  const int TPR = D / 4, NG = min(256 / TPR, kJoinMax);
+  const int grp = (int)threadIdx.x / TPR, d = ((int)threadIdx.x % TPR) * 4;
+  float M = -INFINITY, den = 0.f;
+  f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if (grp < NG) {
+    for (int u0 = grp; u0 < ns; u0 += CH * NG) {
+      f32x4_t l[CH], o[CH];
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        const int64_t at = split_at(sp, min(u0 + u * NG, ns - 1));   // clamped: weight 0
+        l[u] = p.ml[at];
+        o[u] = *reinterpret_cast<const f32x4_t*>(p.o + at * D + d);
+      }
+      float mc = M;
+#pragma unroll
+      for (int u = 0; u < CH; ++u)
+        if (u0 + u * NG < ns && l[u][1] != 0.f) mc = fmaxf(mc, l[u][0]);
+      const float r = M == -INFINITY ? 0.f : fast_exp2(M - mc);
+      den *= r;
+      acc *= r;
+      M = mc;
+#pragma unroll
+      for (int u = 0; u < CH; ++u)
+        if (u0 + u * NG < ns && l[u][1] != 0.f) {
+          const float w = fast_exp2(l[u][0] - M);
+          den += w * l[u][1];
+          acc += o[u] * w;
+        }
+    }
+    s_acc[threadIdx.x] = acc;
+    if (d == 0) {
+      s_m[grp] = M;
+      s_den[grp] = den;
+    }
+  }
+  __syncthreads();
+  if (grp != 0) return;
+  const int ng = min(NG, ns);
+  float Mt = -INFINITY;
+  for (int y = 0; y < ng; ++y)
+    if (s_den[y] != 0.f) Mt = fmaxf(Mt, s_m[y]);
+  float dt = 0.f;
+  f32x4_t at = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int y = 0; y < ng; ++y)
+    if (s_den[y] != 0.f) {
+      const float w = fast_exp2(s_m[y] - Mt);
+      dt += s_den[y] * w;
+      at += s_acc[y * TPR + (int)threadIdx.x] * w;
+    }
+  const float inv = dt != 0.f ? 1.f / dt : 0.f;
+  *reinterpret_cast<u32x2_t*>(p.out + (int64_t)row * D + d) =
+      u32x2_t{pack2<F16>(at[0] * inv, at[1] * inv), pack2<F16>(at[2] * inv, at[3] * inv)};
+}
+
+// 256 keys of one (b, g): weights_out = weights + sum over its heads of
+// 2^(score - M) / l, M and l the row's base and sum over all its parts.  A wave
+// takes every fourth head, a lane four keys.
+constexpr int kWeightKeys = 256;
+LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
+  __shared__ float s_M[32], s_inv[32];
+  __shared__ f32x4_t s_w[4][64];
+  const int b = bg / p.G, g = bg - b * p.G;
+  const int len = seq_len(p, b);
+  if (j0 >= len) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  f32x4_t sum = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int j = j0 + 4 * lane;
+  for (int h0 = 0; h0 < p.H; h0 += 32) {
+    const int hn = min(32, p.H - h0);
+    // eight threads to a head, each every eighth part
+    {
+      const int h = tid >> 3, y = tid & 7;
+      float M = -INFINITY, L = 0.f;
+      if (h < hn) {
+        const Splits sp = row_splits(p, b, g, h0 + h);
+        for (int u = y; u < sp.n; u += 8) {
+          const f32x4_t l = p.ml[split_at(sp, u)];
+          if (l[1] != 0.f) {
+            const float m = fmaxf(M, l[0]);
+            L = (M == -INFINITY ? 0.f : L * fast_exp2(M - m)) + l[2] * fast_exp2(l[0] - m);
+            M = m;
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) {
+        const float M2 = __shfl_xor(M, x), L2 = __shfl_xor(L, x);
+        const float m = fmaxf(M, M2);
+        L = (L != 0.f ? L * fast_exp2(M - m) : 0.f) + (L2 != 0.f ? L2 * fast_exp2(M2 - m) : 0.f);
+        M = m;
+      }
+      if (y == 0) {
+        s_M[h] = M == -INFINITY ? 0.f : M;
+        s_inv[h] = L != 0.f ? 1.f / L : 0.f;
+      }
+    }
+    __syncthreads();
+    if (j < len)      // Sp is a multiple of 64: a whole piece
+      for (int h = wave; h < hn; h += 4) {
+        const f32x4_t sc = *reinterpret_cast<const f32x4_t*>(
+            p.score + ((int64_t)bg * p.H + h0 + h) * p.Sp + j);
+        const float M = s_M[h], inv = s_inv[h];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(sc[i] - M) * inv;
+      }
+    __syncthreads();
+  }
+  s_w[wave][lane] = sum;
+  __syncthreads();
+  const float* f = reinterpret_cast<const float*>(s_w);
+  const int at = j0 + tid;
+  if (at < len)
+    p.w_out[(int64_t)bg * p.S + at] =
+        p.w[(int64_t)bg * p.S + at] + ((f[tid] + f[256 + tid]) + (f[512 + tid] + f[768 + tid]));
+}
+
+template <bool F16, bool WT>
+__global__ void __launch_bounds__(256) cache_join_kernel(StepParams p) {
+  const int R = p.B * p.G * p.H;
+  if constexpr (WT) {
+    if ((int)blockIdx.x >= R) {
+      const int nw = (p.S + kWeightKeys - 1) / kWeightKeys;
+      const int x = blockIdx.x - R;
+      add_weights(p, x / nw, x % nw * kWeightKeys);
+      return;
+    }
+  }
+  join_row<F16>(p);
+}
+
+// The launch's shape, from the extents alone.
+struct Shape {
+  int nht, chunks, ntp, nsp, tile_p, nprefix;
+  int64_t max_chunks, Sp, rows;
+};
+
+Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P, int64_t S) {
+  Shape s{};
+  const int64_t slots = D > 128 ? 256 : 512;   // workgroups that run at once
+  s.nht = H <= 32 ? 1 : (int)cdiv64(H, 128);
+  s.chunks = (int)std::max<int64_t>(1, slots / (G * s.nht));
+  s.max_chunks = s.chunks + B;
+  s.Sp = cdiv64(S, kKeys) * kKeys;
+  if (P > 0) {
+    const int64_t rows = B * H;
+    s.ntp = rows <= 32 ? 1 : (int)cdiv64(rows, 128);
+    const int64_t least = rows <= 32 ? 64 : 256;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / (G * s.ntp), 32));
+    s.tile_p = (int)(cdiv64(std::max(cdiv64(P, want), least), kKeys) * kKeys);
+    s.nsp = (int)cdiv64(P, s.tile_p);
+    s.nprefix = (int)(G * s.ntp * s.nsp);
+  }
+  s.rows = s.nsp * B * G * H + s.max_chunks * G * H;
+  return s;
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -140,7 +710,7 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
                      "cache_decode: head_dim %lld not built (a multiple of 8 up to 256)",
                      (long long)D);
   if (S > (1 << 30) || P > (1 << 30) || !loom_prod_le({B, G}, 65535) ||
-      !loom_prod_le({B, G, H}, 1 << 24) || !loom_prod_le({B, G, S, D}, (int64_t)1 << 50) ||
+      !loom_prod_le({B, G, H}, 1 << 24) || !loom_prod_le({B, G, cdiv64(S, 256)}, 1 << 24) || !loom_prod_le({B, G, S, D}, (int64_t)1 << 50) ||
       !loom_prod_le({G, P, D}, (int64_t)1 << 50))
     return loom_fail(err, errlen, LOOM_EINVAL, "cache_decode: problem too large");
   // a capacity or prefix that is not a multiple of 8 takes buffer descriptors,
@@ -175,24 +745,52 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   p.w = static_cast<const float*>(weights);
   p.w_out = static_cast<float*>(weights_out);
   p.out = static_cast<uint16_t*>(out);
-  p.ml = static_cast<float*>(workspace);
-  p.score = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                     align256((size_t)B * G * H * 8));
+  const Shape s = shape_of(B, G, H, D, P, S);
+  char* ws = static_cast<char*>(workspace);
+  p.plan = reinterpret_cast<int2*>(ws);
+  ws += align256((size_t)B * 8);
+  p.ml = reinterpret_cast<f32x4_t*>(ws);
+  ws += align256((size_t)s.rows * 16);
+  p.o = reinterpret_cast<float*>(ws);
+  ws += align256((size_t)s.rows * D * 4);
+  p.score = reinterpret_cast<float*>(ws);
   p.B = (int)B;
   p.G = (int)G;
   p.H = (int)H;
   p.D = (int)D;
   p.P = (int)P;
   p.S = (int)S;
+  p.Sp = (int)s.Sp;
+  p.nht = s.nht;
+  p.chunks = s.chunks;
+  p.ntp = s.ntp;
+  p.nsp = s.nsp;
+  p.tile_p = s.tile_p;
+  p.nprefix = s.nprefix;
   p.c2 = scale * 1.4426950408889634f;
   if (loom_validate_only()) return loom_ok(err, errlen);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(cache_row_kernel<F16>, dim3((unsigned)(B * G * H)), dim3(kThreads), 0, st, p);
-  int rc = loom_check_launch(err, errlen, "cache_decode");
-  if (rc || !weights) return rc;
-  hipLaunchKernelGGL(cache_weight_kernel, dim3((unsigned)cdiv64(S, 256), (unsigned)(B * G)),
-                     dim3(256), 0, st, p);
-  return loom_check_launch(err, errlen, "cache_decode (weights)");
+  const dim3 grid((unsigned)(s.nprefix + s.max_chunks * G * s.nht)), block(kThreads);
+  // the kernel built for 64, 128 or 256 (the next one up) runs any narrower D
+  auto split = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, st, p); };
+  if (weights) {
+    if (D > 128) split(cache_split_kernel<256, F16, true>);
+    else if (D > 64) split(cache_split_kernel<128, F16, true>);
+    else split(cache_split_kernel<64, F16, true>);
+  } else {
+    if (D > 128) split(cache_split_kernel<256, F16, false>);
+    else if (D > 64) split(cache_split_kernel<128, F16, false>);
+    else split(cache_split_kernel<64, F16, false>);
+  }
+  int rc = loom_check_launch(err, errlen, "cache_decode (split)");
+  if (rc) return rc;
+  const int64_t R = B * G * H;
+  if (weights)
+    hipLaunchKernelGGL((cache_join_kernel<F16, true>),
+                       dim3((unsigned)(R + B * G * cdiv64(S, kWeightKeys))), block, 0, st, p);
+  else
+    hipLaunchKernelGGL((cache_join_kernel<F16, false>), dim3((unsigned)R), block, 0, st, p);
+  return loom_check_launch(err, errlen, "cache_decode (join)");
 }
 
 }  // namespace
@@ -202,9 +800,13 @@ extern "C" {
 size_t loom_hip_cache_decode_workspace_bytes(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P,
                                              int64_t S, int weights) {
   if (B <= 0 || G <= 0 || H <= 0 || D <= 0 || P < 0 || S <= 0) return 0;
-  if (P > (1 << 30) || S > (1 << 30) || !loom_prod_le({B, G, H, P + S, 4}, (int64_t)1 << 60))
+  // what does not fit is reported as no size at all fits
+  if (P > (1 << 30) || S > (1 << 30) || D > (1 << 20) || !loom_prod_le({B, G}, 65535) ||
+      !loom_prod_le({B, G, H}, 1 << 24))
     return SIZE_MAX;
-  return align256((size_t)B * G * H * 8) + (size_t)B * G * H * (P + S) * 4;
+  const Shape s = shape_of(B, G, H, D, P, S);
+  return align256((size_t)B * 8) + align256((size_t)s.rows * 16) +
+         align256((size_t)s.rows * D * 4) + (weights ? (size_t)(B * G * H * s.Sp) * 4 : 0);
 }
 
 int loom_hip_cache_decode(const void* prefix_k, const void* prefix_v, const void* k, const void* v,
