@@ -290,7 +290,7 @@ int loom_hip_ssd_prologue_f16(const void* x, const void* dt, const void* A, cons
  * device.  What the slots behind a length hold (leftovers, NaN) is never used
  * and, except where tokens are appended, left as it is.  All extents must be
  * positive unless said otherwise, D a multiple of 8 up to 256 (else
- * LOOM_HIP_EUNSUP), B*G <= 65535, S, P and T at most 2^30. */
+ * LOOM_HIP_EUNSUP), B*G <= 65535, S, P and T at most 2^29. */
 
 /* Appends new_k, new_v [B,T,G,D] (as a projection of B x T tokens gives them)
  * behind every sequence's n keys: the first c = clamp(counts[b], 0, T) of its T

@@ -31,7 +31,7 @@ struct AppendParams {
   int B, G, D, S, T;
 };
 
-// One workgroup per (new token, sequence): a thread per (g, d) element.
+// Few tokens: a thread per element of one (token, sequence).
 __global__ void __launch_bounds__(256) cache_append_kernel(AppendParams p) {
   const int t = blockIdx.x, b = blockIdx.y;
   const int n = cache_len(p.lens, b, p.S);
@@ -49,6 +49,67 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendParams p) {
   }
 }
 
+// Many tokens: a workgroup per 64 slots (a multiple of 64 first, so that whole
+// 16-byte pieces of a K row are written) of one (b, g).  The tokens' K rows go
+// to LDS as they are, DP elements apart, and come back transposed: a lane of
+// ds_read_b64_tr_b16 gets four tokens of one d.  Each 32-lane pass reads 32
+// bytes of rows k..k+3 and k+8..k+11; rows are whole 256-byte bank windows, so
+// the XOR gives the eight rows distinct pairs of 16-byte chunks.
+constexpr int kTok = 64;
+LOOM_DEV int tok_swz(int k) { return 2 * ((k & 3) | ((k >> 1) & 4)); }
+
+template <int DP>
+__global__ void __launch_bounds__(256) cache_append_tile_kernel(AppendParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[kTok * DP * 2];
+  const int bg = blockIdx.y, b = bg / p.G, g = bg - b * p.G;
+  const int n = cache_len(p.lens, b, p.S);
+  const int c = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+  const int tid = threadIdx.x;
+  if (blockIdx.x == 0 && g == 0 && tid == 0) p.lens_out[b] = min(n + c, p.S);
+  const int end = min(n + c, p.S);                     // slots n .. end-1 are written
+  const int k0 = (n / kTok + (int)blockIdx.x) * kTok;  // this workgroup's slots
+  if (k0 >= end) return;
+  const int D = p.D, cpr = D / 8, S = p.S;             // 16-byte chunks of a row
+  const int64_t row = (int64_t)p.G * D;                // elements from token to token
+  // element 0 of slot k0's token (before the tensor for slots < n: not read)
+  const int64_t src0 = ((int64_t)b * p.T + (k0 - n)) * row + (int64_t)g * D;
+  uint16_t* const vo = p.v + ((int64_t)bg * S + k0) * D;
+  for (int e = tid; e < kTok * cpr; e += 256) {
+    const int k = e / cpr, ch = e - k * cpr;
+    if (k0 + k < n || k0 + k >= end) continue;
+    const int64_t src = src0 + k * row + ch * 8;
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p.nk + src);
+    const u32x4_t y = *reinterpret_cast<const u32x4_t*>(p.nv + src);
+    *reinterpret_cast<u32x4_t*>(smem + k * (DP * 2) + ((ch ^ tok_swz(k)) * 16)) = x;
+    *reinterpret_cast<u32x4_t*>(vo + (int64_t)k * D + ch * 8) = y;
+  }
+  if (p.w && tid < kTok && k0 + tid >= n && k0 + tid < end) p.w[(int64_t)bg * S + k0 + tid] = 0.f;
+  __syncthreads();
+  // wave w: 16 rows d at a time; lane group q tokens 8 q .. 8 q + 7 of 32
+  const int lane = tid & 63, wave = tid >> 6;
+  const int r = lane & 15, q = lane >> 4, a4 = r >> 2, c4 = r & 3;
+  const int64_t ko = (int64_t)bg * D * S;
+  for (int x = wave; x < (D + 15) / 16 * 2; x += 4) {
+    const int dt = x >> 1, kk = 32 * (x & 1) + 8 * q;  // first of this lane's eight slots
+    const int ch = 2 * dt + (c4 >> 1);
+    const lds_char_t* const base = (lds_char_t*)smem + (c4 & 1) * 8;
+    const u32x2_t lo = lds_read_tr16(base + (kk + a4) * (DP * 2) + ((ch ^ tok_swz(kk + a4)) * 16));
+    const u32x2_t hi =
+        lds_read_tr16(base + (kk + 4 + a4) * (DP * 2) + ((ch ^ tok_swz(kk + 4 + a4)) * 16));
+    const int d = 16 * dt + r, at = k0 + kk;
+    if (d >= D) continue;
+    uint16_t* const to = p.k + ko + (int64_t)d * S + at;
+    const u32x4_t v = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    if (at >= n && at + 8 <= end) {
+      __builtin_memcpy(to, &v, 16);     // 16-byte aligned when S is a multiple of 8
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (at + i >= n && at + i < end) to[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+
 struct EvictParams {
   const uint16_t* k;
   const uint16_t* v;
@@ -60,6 +121,7 @@ struct EvictParams {
   int* lens_out;
   int* index;          // [B, G, keep]
   int B, G, D, S, So, keep, recent, sinks;
+  int nk, njk, rows_k;  // K parts of a (b, g): njk stretches of slots x rows_k rows each
 };
 
 // A weight as a whole number of the same order: NaN below -inf, -0 as +0.
@@ -69,67 +131,107 @@ LOOM_DEV uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelWaves = 16;
+constexpr int kSelWaves = 16, kSel = 64 * kSelWaves;
+constexpr int kBins = 2048;     // 11 bits a digit: three digits of a 32-bit key
 
 // The kept slots of one (sequence, KV head), ascending, by one workgroup: a
-// radix selection of the weights' keys (four digits of 8 bits, highest first)
-// finds the smallest key that stays and how many of its equals do; each wave
-// then counts what stays of its stretch of slots and writes it behind the
-// waves before it.
-__global__ void __launch_bounds__(64 * kSelWaves) cache_select_kernel(EvictParams p) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t s_digit, s_left;
+// radix selection of the weights' keys (11, 11 and 10 bits, highest first) finds
+// the smallest key that stays and how many of its equals do; each wave then
+// counts what stays of its stretch of slots and writes it behind the waves
+// before it.  A wave owns a contiguous stretch; with KPT > 0 its keys stay in
+// registers (KPT a lane, slots 64 apart), else (KPT 0, longer caches) every pass
+// reads the weights again.
+template <int KPT>
+__global__ void __launch_bounds__(kSel) cache_select_kernel(EvictParams p) {
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t s_part[kSelWaves], s_digit, s_left;
   __shared__ int s_sel[kSelWaves], s_eq[kSelWaves];
   const int bg = blockIdx.x, b = bg / p.G;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = cache_len(p.lens, b, p.S);
   int* const idx = p.index + (int64_t)bg * p.keep;
-  if (bg % p.G == 0 && tid == 0) p.lens_out[b] = min(n, p.keep);
+  if (bg - b * p.G == 0 && tid == 0) p.lens_out[b] = min(n, p.keep);
   if (n <= p.keep) {
-    for (int j = tid; j < p.keep; j += 64 * kSelWaves) idx[j] = j < n ? j : -1;
+    for (int j = tid; j < p.keep; j += kSel) idx[j] = j < n ? j : -1;
     return;
   }
   const float* const w = p.w + (int64_t)bg * p.S;
   const int lo = p.sinks, hi = n - p.recent;   // the slots that are weighed
-  uint32_t left = (uint32_t)(p.keep - p.sinks - p.recent);   // how many of them stay
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
-    for (int i = tid; i < 256; i += 64 * kSelWaves) hist[i] = 0;
-    __syncthreads();
-    for (int i = lo + tid; i < hi; i += 64 * kSelWaves) {
-      const uint32_t key = weight_key(w[i]);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[(key >> shift) & 255u], 1u);
+  const int per = KPT > 0 ? KPT : (n + kSel - 1) / kSel;   // keys of a lane
+  const int i0 = wave * per * 64;              // this wave's slots: i0 + 64 u + lane
+  uint32_t reg[KPT > 0 ? KPT : 1];
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) {
+      const int i = i0 + u * 64 + lane;
+      reg[u] = weight_key(w[min(i, n - 1)]);
     }
+  }
+  auto each = [&](auto f) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int u = 0; u < KPT; ++u) f(i0 + u * 64 + lane, reg[u]);
+    } else {
+      for (int u = 0; u < per && i0 + u * 64 < n; ++u) {
+        const int i = i0 + u * 64 + lane;
+        f(i, weight_key(w[min(i, n - 1)]));
+      }
+    }
+  };
+  uint32_t left = (uint32_t)(p.keep - p.sinks - p.recent);   // how many weighed ones stay
+  const bool none = left == 0;
+  uint32_t prefix = 0;
+  for (int pass = 0; pass < 3 && !none; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t above = pass == 0 ? 0u : ~0u << (pass == 1 ? 21 : 10);   // digits found
+    const uint32_t mask = pass == 2 ? 1023u : 2047u;
+    for (int i = tid; i < kBins; i += kSel) hist[i] = 0;
     __syncthreads();
-    if (tid == 0) {
-      uint32_t above = 0;
-      int d = 255;
-      while (d > 0 && above + hist[d] < left) above += hist[d--];
-      s_digit = (uint32_t)d;
-      s_left = left - above;
+    each([&](int i, uint32_t key) {
+      const bool in = i >= lo && i < hi && (key & above) == prefix;
+      const uint32_t dig = (key >> shift) & mask;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+      if (m == 0) return;
+      // lanes of one digit (a stretch of equal weights) count as one
+      const uint32_t d0 = __builtin_amdgcn_readlane(dig, __builtin_ctzll(m));
+      const uint64_t same = __builtin_amdgcn_ballot_w64(in && dig == d0);
+      if (in && dig != d0) atomicAdd(&hist[dig], 1u);
+      if (lane == 0) atomicAdd(&hist[d0], (uint32_t)__popcll(same));
+    });
+    __syncthreads();
+    // the digit at which the count from the top reaches `left`: two bins a
+    // thread, highest first
+    const int bin = kBins - 1 - 2 * tid;
+    const uint32_t h0 = hist[bin], h1 = hist[bin - 1];
+    uint32_t inc = h0 + h1;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const uint32_t o = __shfl_up(inc, m);
+      if (lane >= m) inc += o;
+    }
+    if (lane == 63) s_part[wave] = inc;
+    __syncthreads();
+    uint32_t before = inc - h0 - h1;            // keys of higher digits
+    for (int x = 0; x < wave; ++x) before += s_part[x];
+    if (before < left && before + h0 >= left) {
+      s_digit = bin;
+      s_left = left - before;
+    } else if (before + h0 < left && before + h0 + h1 >= left) {
+      s_digit = bin - 1;
+      s_left = left - before - h0;
     }
     __syncthreads();
     prefix |= s_digit << shift;
     left = s_left;
-    __syncthreads();
   }
   // stays: above the threshold, and the first `left` equal to it
-  const bool none = p.keep == p.sinks + p.recent;
-  const int seg = (n + 64 * kSelWaves - 1) / (64 * kSelWaves) * 64;
-  const int i0 = min(wave * seg, n), i1 = min(i0 + seg, n);
   int sel = 0, eq = 0;
-  for (int i = i0 + lane; i < i1; i += 64) {
-    const bool must = i < lo || i >= hi;
-    const uint32_t key = must || none ? 0u : weight_key(w[i]);
-    sel += must || (!none && key > prefix);
-    eq += !must && !none && key == prefix;
-  }
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    sel += __shfl_xor(sel, m);
-    eq += __shfl_xor(eq, m);
-  }
+  each([&](int i, uint32_t key) {
+    const bool in = i < n, must = in && (i < lo || i >= hi), free = in && !must && !none;
+    sel += __popcll(__builtin_amdgcn_ballot_w64(must || (free && key > prefix)));
+    eq += __popcll(__builtin_amdgcn_ballot_w64(free && key == prefix));
+  });
   if (lane == 0) {
     s_sel[wave] = sel;
     s_eq[wave] = eq;
@@ -141,34 +243,67 @@ __global__ void __launch_bounds__(64 * kSelWaves) cache_select_kernel(EvictParam
     eqs += s_eq[x];
   }
   at += min(eqs, (int)left);
-  for (int base = i0; base < i1; base += 64) {
-    const int i = base + lane;
-    const bool in = i < i1, must = in && (i < lo || i >= hi);
-    const uint32_t key = !in || must || none ? 0u : weight_key(w[i]);
-    const bool same = in && !must && !none && key == prefix;
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  each([&](int i, uint32_t key) {
+    const bool in = i < n, must = in && (i < lo || i >= hi), free = in && !must && !none;
+    const bool same = free && key == prefix;
     const uint64_t eqm = __builtin_amdgcn_ballot_w64(same);
-    const bool stays = must || (in && !none && key > prefix) ||
+    const bool stays = must || (free && key > prefix) ||
                        (same && eqs + __popcll(eqm & below) < (int)left);
     const uint64_t m = __builtin_amdgcn_ballot_w64(stays);
     if (stays) idx[at + __popcll(m & below)] = i;
     at += __popcll(m);
     eqs += __popcll(eqm);
-  }
+  });
 }
 
-// Rows of the kept slots: K elements of row d (blockIdx.y < D), V and weights.
-__global__ void __launch_bounds__(256) cache_gather_kernel(EvictParams p) {
-  const int bg = blockIdx.z, y = blockIdx.y;
-  const int n = min(cache_len(p.lens, bg / p.G, p.S), p.keep);
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
-  const int i = p.index[(int64_t)bg * p.keep + j];
-  if (y < p.D) {
-    p.k_out[((int64_t)bg * p.D + y) * p.So + j] = p.k[((int64_t)bg * p.D + y) * p.S + i];
-    p.v_out[((int64_t)bg * p.So + j) * p.D + y] = p.v[((int64_t)bg * p.S + i) * p.D + y];
-  } else {
-    p.w_out[(int64_t)bg * p.So + j] = p.w[(int64_t)bg * p.S + i];
+// The kept keys moved.  K parts take rows_k rows d of one (b, g) and 1024 kept
+// slots: a lane an element, so a load touches the few lines that 64 kept slots
+// span (eight elements a lane, for 16-byte stores, touched 64 of them); the
+// slots stay in registers over the rows.  V parts take rows of D elements, 16
+// bytes a lane, and the weights.
+constexpr int kMoveK = 4;           // slots of a thread
+constexpr int kMoveV = 64;          // slots of a V part
+__global__ void __launch_bounds__(256) cache_move_kernel(EvictParams p) {
+  const int bg = blockIdx.y, b = bg / p.G, tid = threadIdx.x;
+  const int n = min(cache_len(p.lens, b, p.S), p.keep);
+  const int* const idx = p.index + (int64_t)bg * p.keep;
+  const int D = p.D;
+  int x = blockIdx.x;
+  if (x < p.nk) {
+    const int j0 = x % p.njk * (256 * kMoveK) + tid, d0 = x / p.njk * p.rows_k;
+    if (j0 - tid >= n) return;
+    int at[kMoveK];
+#pragma unroll
+    for (int u = 0; u < kMoveK; ++u) at[u] = idx[min(j0 + 256 * u, n - 1)];
+    const int d1 = min(D, d0 + p.rows_k);
+    const uint16_t* src = p.k + ((int64_t)bg * D + d0) * p.S;
+    uint16_t* dst = p.k_out + ((int64_t)bg * D + d0) * p.So;
+#pragma unroll 4
+    for (int d = d0; d < d1; ++d) {
+      uint16_t e[kMoveK];
+#pragma unroll
+      for (int u = 0; u < kMoveK; ++u) e[u] = src[at[u]];
+#pragma unroll
+      for (int u = 0; u < kMoveK; ++u)
+        if (j0 + 256 * u < n) dst[j0 + 256 * u] = e[u];
+      src += p.S;
+      dst += p.So;
+    }
+    return;
+  }
+  x -= p.nk;
+  const int j0 = x * kMoveV, jn = min(kMoveV, n - j0);
+  if (jn <= 0) return;
+  if (tid < jn) p.w_out[(int64_t)bg * p.So + j0 + tid] = p.w[(int64_t)bg * p.S + idx[j0 + tid]];
+  const int cpr = D / 8;
+  const uint16_t* const src = p.v + (int64_t)bg * p.S * D;
+  uint16_t* const dst = p.v_out + ((int64_t)bg * p.So + j0) * D;
+#pragma unroll 4
+  for (int e = tid; e < jn * cpr; e += 256) {
+    const int j = e / cpr, c = e - j * cpr;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(src + (int64_t)idx[j0 + j] * D + c * 8);
+    *reinterpret_cast<u32x4_t*>(dst + (int64_t)j * D + c * 8) = v;
   }
 }
 
@@ -196,7 +331,7 @@ int loom_hip_cache_append(void* k, void* v, void* weights, const void* lens, con
     return loom_fail(err, errlen, LOOM_EUNSUP,
                      "cache_append: head_dim %lld not built (a multiple of 8 up to 256)",
                      (long long)D);
-  if (S > (1 << 30) || T > (1 << 30) || !loom_prod_le({B, G}, 65535) ||
+  if (S > (1 << 29) || T > (1 << 29) || !loom_prod_le({B, G}, 65535) ||
       !loom_prod_le({B, G, S, D}, (int64_t)1 << 50) ||
       !loom_prod_le({B, G, T, D}, (int64_t)1 << 50))
     return loom_fail(err, errlen, LOOM_EINVAL, "cache_append: problem too large");
@@ -224,8 +359,18 @@ int loom_hip_cache_append(void* k, void* v, void* weights, const void* lens, con
   p.S = (int)S;
   p.T = (int)T;
   if (loom_validate_only()) return loom_ok(err, errlen);
-  hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)T, (unsigned)B), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), p);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (T < 16) {
+    hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)T, (unsigned)B), dim3(256), 0, st, p);
+  } else {
+    // slots that a sequence's tokens reach from any length: T and the part of a
+    // tile before them
+    const dim3 grid((unsigned)(cdiv64(std::min(T, S), kTok) + 1), (unsigned)(B * G));
+    if (D <= 128)
+      hipLaunchKernelGGL(cache_append_tile_kernel<128>, grid, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL(cache_append_tile_kernel<256>, grid, dim3(256), 0, st, p);
+  }
   return loom_check_launch(err, errlen, "cache_append");
 }
 
@@ -246,7 +391,7 @@ int loom_hip_cache_evict(const void* k, const void* v, const void* weights, cons
     return loom_fail(err, errlen, LOOM_EUNSUP,
                      "cache_evict: head_dim %lld not built (a multiple of 8 up to 256)",
                      (long long)D);
-  if (S > (1 << 30) || S_out > (1 << 30) || !loom_prod_le({B, G}, 65535) ||
+  if (S > (1 << 29) || S_out > (1 << 29) || !loom_prod_le({B, G}, 65535) ||
       !loom_prod_le({B, G, S, D}, (int64_t)1 << 50) ||
       !loom_prod_le({B, G, S_out, D}, (int64_t)1 << 50))
     return loom_fail(err, errlen, LOOM_EINVAL, "cache_evict: problem too large");
@@ -289,12 +434,19 @@ int loom_hip_cache_evict(const void* k, const void* v, const void* weights, cons
   p.sinks = (int)sinks;
   if (loom_validate_only()) return loom_ok(err, errlen);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(cache_select_kernel, dim3((unsigned)(B * G)), dim3(64 * kSelWaves), 0, st, p);
+  const dim3 sel((unsigned)(B * G)), selb(kSel);
+  if (S <= 4 * kSel) hipLaunchKernelGGL(cache_select_kernel<4>, sel, selb, 0, st, p);
+  else if (S <= 16 * kSel) hipLaunchKernelGGL(cache_select_kernel<16>, sel, selb, 0, st, p);
+  else hipLaunchKernelGGL(cache_select_kernel<0>, sel, selb, 0, st, p);
   int rc = loom_check_launch(err, errlen, "cache_evict (select)");
   if (rc) return rc;
-  const dim3 grid((unsigned)cdiv64(keep, 256), (unsigned)D + 1, (unsigned)(B * G));
-  hipLaunchKernelGGL(cache_gather_kernel, grid, dim3(256), 0, st, p);
-  return loom_check_launch(err, errlen, "cache_evict (gather)");
+  // rows of a K part: as many (up to 16) as leave about 1024 parts
+  p.njk = (int)cdiv64(keep, 256 * kMoveK);
+  p.rows_k = (int)std::max<int64_t>(2, std::min<int64_t>(16, B * G * p.njk * D / 1024));
+  p.nk = (int)(p.njk * cdiv64(D, p.rows_k));
+  const dim3 grid((unsigned)(p.nk + cdiv64(keep, kMoveV)), (unsigned)(B * G));
+  hipLaunchKernelGGL(cache_move_kernel, grid, dim3(256), 0, st, p);
+  return loom_check_launch(err, errlen, "cache_evict (move)");
 }
 
 }  // extern "C"

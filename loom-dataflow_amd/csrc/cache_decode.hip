@@ -709,7 +709,7 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
     return loom_fail(err, errlen, LOOM_EUNSUP,
                      "cache_decode: head_dim %lld not built (a multiple of 8 up to 256)",
                      (long long)D);
-  if (S > (1 << 30) || P > (1 << 30) || !loom_prod_le({B, G}, 65535) ||
+  if (S > (1 << 29) || P > (1 << 29) || !loom_prod_le({B, G}, 65535) ||
       !loom_prod_le({B, G, H}, 1 << 24) || !loom_prod_le({B, G, cdiv64(S, 256)}, 1 << 24) || !loom_prod_le({B, G, S, D}, (int64_t)1 << 50) ||
       !loom_prod_le({G, P, D}, (int64_t)1 << 50))
     return loom_fail(err, errlen, LOOM_EINVAL, "cache_decode: problem too large");
@@ -801,7 +801,7 @@ size_t loom_hip_cache_decode_workspace_bytes(int64_t B, int64_t G, int64_t H, in
                                              int64_t S, int weights) {
   if (B <= 0 || G <= 0 || H <= 0 || D <= 0 || P < 0 || S <= 0) return 0;
   // what does not fit is reported as no size at all fits
-  if (P > (1 << 30) || S > (1 << 30) || D > (1 << 20) || !loom_prod_le({B, G}, 65535) ||
+  if (P > (1 << 29) || S > (1 << 29) || D > (1 << 20) || !loom_prod_le({B, G}, 65535) ||
       !loom_prod_le({B, G, H}, 1 << 24))
     return SIZE_MAX;
   const Shape s = shape_of(B, G, H, D, P, S);
