@@ -30,7 +30,7 @@ struct StepParams {
   const float* w;
   float* w_out;
   uint16_t* out;
-  int2* plan;       // [B]: a sequence's first chunk, and the chunks' keys
+  int2* plan;       // [B]: a sequence's first chunk and their number
   f32x4_t* ml;      // per partial row: base, sum of the rounded p, sum of p
   float* o;         // per partial row: sum of p v, D values
   float* score;     // [B G, H, Sp] scores of the own keys, log2 domain
@@ -59,7 +59,7 @@ struct Part {
   int rows;             // query rows
   int i0;               // first row: of the (b, g)'s heads, or of head g's B H rows
   int g;                // the KV head of a prefix part, -1: rows are consecutive
-  int64_t out0;         // partial row of row 0 (own part)
+  int64_t out0;         // partial row of row 0; the others follow
   float* score;         // scores of row 0, Sp apart, or null
 };
 
@@ -94,6 +94,11 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
   const uint16_t* __restrict__ vg = a.v;
   const int nblk = (s1 - s0 + kKeys - 1) / kKeys;
   const bool active = 16 * QT * qw < a.rows;    // this wave has rows
+  // score stores of a block that every active wave issues at least (those of
+  // its first row tile): younger than the next block's copies, so the wait for
+  // the copies need not wait for them
+  const bool stores = WT && active && a.score;
+  constexpr int STORES = KG == 2 ? 2 : 4;
 
   auto stK = [&](int s) { return (lds_char_t*)(smem + s * STAGE); };
   auto stV = [&](int s) { return (lds_char_t*)(smem + s * STAGE + K_BYTES); };
@@ -148,7 +153,8 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
   // ---- the queries into the second stage (rows past the part's repeat its
   // last, elements past Dr are zeroed when read), then the first block
   lds_char_t* const sq = stK(1);
-#pragma unroll
+  // (a rolled loop: code that a workgroup runs once is fetched as it runs)
+#pragma unroll 1
   for (int i = 0; i < Q_INSTR; ++i) {
     const int j = wave * Q_INSTR + i;
     const int e = j * 512 + lane * 8;
@@ -175,23 +181,25 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
   }
   bool first = true;
 
-  // ---- 32 keys (half h of block blk in stage s) against this wave's rows
-  auto half = [&](int s, int blk, int h) {
-    const int kv0 = s0 + blk * kKeys + 32 * h;
+  // ---- this wave's keys of block blk in stage s (one 32-key half with two key
+  // groups, else both) against its rows
+  constexpr int NH = 2 / KG;
+  auto compute = [&](int s, int blk) {
+    const int kv0 = s0 + blk * kKeys + 32 * (KG == 2 ? kh : 0);
     const lds_char_t* ks = stK(s);
     const lds_char_t* vs = stV(s);
     // st[j][qt][i]: key kv0 + 16 j + 4 g + i, row 16 qt + r of this wave
-    f32x4_t st[2][QT];
+    f32x4_t st[2 * NH][QT];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2 * NH; ++j)
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) st[j][qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ds = 0; ds < DSTEPS; ++ds) {
+    for (int j = 0; j < 2 * NH; ++j) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int ds = 0; ds < DSTEPS; ++ds) {
         const int d = ds * 32 + g * 8 + a4;
-        const int ch = (2 * (2 * h + j) + (c4 >> 1)) ^ ck_swz(d);
+        const int ch = (2 * ((KG == 2 ? 2 * kh : 0) + j) + (c4 >> 1)) ^ ck_swz(d);
         const lds_char_t* q = ks + d * (kKeys * 2) + ch * 16 + (c4 & 1) * 8;
         const u32x2_t lo = lds_read_tr16(q);
         const u32x2_t hi = lds_read_tr16(q + 4 * (kKeys * 2));
@@ -200,18 +208,17 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
         for (int qt = 0; qt < QT; ++qt) st[j][qt] = mfma16t<F16>(kf, qf[ds][qt], st[j][qt]);
       }
     }
-    const bool edge = kv0 + 32 > s1;
+    const bool edge = kv0 + 32 * NH > s1;
     if constexpr (WT) {
       if (a.score) {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
           const int lr = 16 * (QT * qw + qt) + r;
-          if (lr < a.rows) {
-            float* to = a.score + (int64_t)lr * p.Sp + kv0 + 4 * g;
+          float* to = a.score + (int64_t)lr * p.Sp + kv0 + 4 * g;
+          if (lr < a.rows)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2 * NH; ++j)
               *reinterpret_cast<f32x4_t*>(to + 16 * j) = st[j][qt] * c2;
-          }
         }
       }
     }
@@ -222,7 +229,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
     for (int qt = 0; qt < QT; ++qt) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2 * NH; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v = __builtin_fmaf(st[j][qt][i], c2, -m_run[qt]);
@@ -251,43 +258,47 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
         for (int dt = 0; dt < DT; ++dt) ot[dt][qt] *= alpha;
         m_run[qt] += shift;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) st[j][qt] -= shift;
+        for (int j = 0; j < 2 * NH; ++j) st[j][qt] -= shift;
         unset_left |= unset && mx == -INFINITY;
       }
       first = __builtin_amdgcn_ballot_w64(unset_left) != 0;
     }
-    u32x4_t pf[QT];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      f32x4_t e0, e1;
+    for (int h = 0; h < NH; ++h) {
+      u32x4_t pf[QT];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e0[i] = fast_exp2(st[0][qt][i]);
-        e1[i] = fast_exp2(st[1][qt][i]);
+      for (int qt = 0; qt < QT; ++qt) {
+        f32x4_t e0, e1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e0[i] = fast_exp2(st[2 * h][qt][i]);
+          e1[i] = fast_exp2(st[2 * h + 1][qt][i]);
+        }
+        if constexpr (WT)
+          lx[qt] += ((e0[0] + e0[1]) + (e0[2] + e0[3])) + ((e1[0] + e1[1]) + (e1[2] + e1[3]));
+        pf[qt] = u32x4_t{pack2<F16>(e0[0], e0[1]), pack2<F16>(e0[2], e0[3]),
+                         pack2<F16>(e1[0], e1[1]), pack2<F16>(e1[2], e1[3])};
+        lacc[qt] = mfma16t<F16>(ones, pf[qt], lacc[qt]);
       }
-      if constexpr (WT)
-        lx[qt] += ((e0[0] + e0[1]) + (e0[2] + e0[3])) + ((e1[0] + e1[1]) + (e1[2] + e1[3]));
-      pf[qt] = u32x4_t{pack2<F16>(e0[0], e0[1]), pack2<F16>(e0[2], e0[3]),
-                       pack2<F16>(e1[0], e1[1]), pack2<F16>(e1[2], e1[3])};
-      lacc[qt] = mfma16t<F16>(ones, pf[qt], lacc[qt]);
-    }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const int k0r = 32 * h + 4 * g + a4;
-      const int ch = (2 * dt + (c4 >> 1)) ^ cv_swz<D>(k0r);
-      const lds_char_t* q = vs + k0r * VROW + ch * 16 + (c4 & 1) * 8;
-      const u32x2_t lo = lds_read_tr16(q);
-      const u32x2_t hi = lds_read_tr16(q + 16 * VROW);
-      const u32x4_t vf = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+      for (int dt = 0; dt < DT; ++dt) {
+        const int k0r = 32 * (KG == 2 ? kh : h) + 4 * g + a4;
+        const int ch = (2 * dt + (c4 >> 1)) ^ cv_swz<D>(k0r);
+        const lds_char_t* q = vs + k0r * VROW + ch * 16 + (c4 & 1) * 8;
+        const u32x2_t lo = lds_read_tr16(q);
+        const u32x2_t hi = lds_read_tr16(q + 16 * VROW);
+        const u32x4_t vf = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) ot[dt][qt] = mfma16t<F16>(vf, pf[qt], ot[dt][qt]);
+        for (int qt = 0; qt < QT; ++qt) ot[dt][qt] = mfma16t<F16>(vf, pf[qt], ot[dt][qt]);
+      }
     }
   };
 
   for (int it = 0; it < nblk; ++it) {
     const int s = it & 1;
     lds_order();
-    LOOM_WAIT_VMCNT(0);
+    if (it > 0 && stores) LOOM_WAIT_VMCNT(STORES);
+    else LOOM_WAIT_VMCNT(0);
     LOOM_WAIT_LGKM0();
     barrier_nofence();
     if (it == 0) {
@@ -308,14 +319,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
       if (ahead) kload(it + 1);
     }
     if (ahead) issue(s ^ 1, it + 1);
-    if (active) {
-      if constexpr (KG == 2) {
-        half(s, it, kh);
-      } else {
-        half(s, it, 0);
-        half(s, it, 1);
-      }
-    }
+    if (active) compute(s, it);
     if constexpr (KREG) {
       if (ahead) kstore(s ^ 1);
     }
@@ -364,76 +368,123 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
         ot[dt][qt] = ot[dt][qt] * f0 + mg[(qt * (DT + 1) + dt) * 64] * f1;
     }
   }
-  // ---- (base, sums, O) of every row: ot[dt][qt][i] is d = 16 dt + 4 g + i
+  // ---- (base, sums, O) of every row.  ot[dt][qt][i] is d = 16 dt + 4 g + i of
+  // row 16 qt + r: turned through this wave's stretch of the idle stages (16 rows
+  // of D + 4 floats, free of conflicts) into whole rows, 16 bytes a lane.  Rolled
+  // loops: a workgroup runs this once, and fetching unrolled code took longer
+  // than the stores
+  constexpr int OROW = D + 4, PPR = D / 4;      // floats and 16-byte pieces of a row
+  constexpr int OFF = KG == 2 ? W / 2 * QT * (DT + 1) * 64 * 4 : 0;   // past the handed-over state
+  static_assert(OFF * 4 + W / KG * 16 * OROW * 4 <= 2 * STAGE, "O rows fit the stages");
+  if (KG == 1) {
+    LOOM_WAIT_LGKM0();
+    barrier_nofence();
+  }
+  float* const mo = reinterpret_cast<float*>(smem) + OFF + qw * 16 * OROW;
+  const int lr0 = lane / PPR, c = (lane % PPR) * 4;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    const int lr = 16 * (QT * qw + qt) + r;
-    if (lr < a.rows) {
-      const int64_t row = a.out0 + (a.g < 0 ? lr : part_row(p, a, lr));
-      if (g == 0) p.ml[row] = f32x4_t{m_run[qt], lacc[qt][0], lx[qt], 0.f};
+    const int t0 = 16 * (QT * qw + qt);         // first row of the tile
+    const int n = min(16, a.rows - t0);
+    const int64_t row0 = a.out0 + t0;
+    if (r < n && g == 0) p.ml[row0 + r] = f32x4_t{m_run[qt], lacc[qt][0], lx[qt], 0.f};
+    lds_order();
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        if (dt * 16 + 4 * g < Dr)
-          *reinterpret_cast<f32x4_t*>(p.o + row * Dr + dt * 16 + 4 * g) = ot[dt][qt];
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<f32x4_t*>(mo + r * OROW + dt * 16 + 4 * g) = ot[dt][qt];
+    lds_order();
+    if (c < Dr) {
+      float* to = p.o + (row0 + lr0) * Dr + c;
+#pragma unroll 1
+      for (int lr = lr0; lr < n; lr += 64 / PPR, to += 64 / PPR * Dr)
+        *reinterpret_cast<f32x4_t*>(to) =
+            *reinterpret_cast<const f32x4_t*>(mo + lr * OROW + c);
     }
+    lds_order();
   }
 }
 
+// Where chunk c of the batch's own keys lies.  t, a multiple of 64, is the chunk
+// that gives about p.chunks of them over all sequences whatever their lengths;
+// a sequence takes as many as t asks for, of equal size, sequences in order.
+// Every workgroup works it out from the lengths, so nothing is planned on the
+// host and a replayed graph follows them.
+struct Chunk {
+  int b, i, n;    // sequence (-1: none), its chunk, its length
+  int cnt, size;  // the sequence's chunks, the keys of one
+  int c0;         // the sequence's first chunk
+};
+LOOM_DEV int chunk_keys(const StepParams& p, int64_t total) {
+  const int64_t per = (total + p.chunks - 1) / p.chunks;
+  return (int)min((int64_t)1 << 30, max((int64_t)1, (per + kKeys - 1) / kKeys) * kKeys);
+}
+LOOM_DEV int wave_scan(int v, int lane) {   // inclusive
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int o = __shfl_up(v, m);
+    if (lane >= m) v += o;
+  }
+  return v;
+}
 LOOM_DEV int64_t wave_sum64(int64_t v) {
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
   return v;
 }
-
-// Where chunk c of the batch's own keys lies: sequences in order, each cut into
-// chunks of t keys, t the multiple of 64 that gives about p.chunks of them over
-// all sequences whatever their lengths.  Every workgroup works it out from the
-// lengths (one load per 256 sequences), so nothing is planned on the host and a
-// replayed graph follows them.
-struct Chunk {
-  int b, i, n, t;   // sequence (-1: none), its chunk, its length, keys of a chunk
-};
 LOOM_DEV Chunk find_chunk(const StepParams& p, int c) {
-  __shared__ int64_t s_sum[kThreads / 64];
-  __shared__ int s_cnt[kThreads / 64], s_b, s_i, s_n;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int64_t total = 0;
-  for (int b = tid; b < p.B; b += kThreads) total += seq_len(p, b);
-  total = wave_sum64(total);
-  if (lane == 0) s_sum[wave] = total;
-  if (tid == 0) s_b = -1;
-  __syncthreads();
-  total = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-  const int t = (int)min((int64_t)1 << 30,
-                         max((int64_t)1, ((total + p.chunks - 1) / p.chunks + kKeys - 1) / kKeys) *
-                             kKeys);
-  int base = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const int b = b0 + tid;
-    const int n = b < p.B ? seq_len(p, b) : 0;
+  Chunk r{-1, 0, 0, 1, 0, 0};
+  if (p.B <= 64) {          // each wave by itself: one load, no barrier
+    const int n = lane < p.B ? seq_len(p, lane) : 0;
+    const int t = chunk_keys(p, wave_sum64(n));
     const int cnt = (n + t - 1) / t;
-    int inc = cnt;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int o = __shfl_up(inc, m);
-      if (lane >= m) inc += o;
-    }
-    if (lane == 63) s_cnt[wave] = inc;
+    const int inc = wave_scan(cnt, lane);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(c < inc);
+    if (m == 0) return r;
+    r.b = __builtin_ctzll(m);
+    r.n = __builtin_amdgcn_readlane(n, r.b);
+    r.cnt = __builtin_amdgcn_readlane(cnt, r.b);
+    r.c0 = __builtin_amdgcn_readlane(inc, r.b) - r.cnt;
+  } else {
+    __shared__ int64_t s_sum[kThreads / 64];
+    __shared__ int s_cnt[kThreads / 64], s_r[4];
+    int64_t total = 0;
+    for (int b = tid; b < p.B; b += kThreads) total += seq_len(p, b);
+    total = wave_sum64(total);
+    if (lane == 0) s_sum[wave] = total;
+    if (tid == 0) s_r[0] = -1;
     __syncthreads();
-    int before = base;
-    for (int x = 0; x < wave; ++x) before += s_cnt[x];
-    const int at = before + inc - cnt;
-    if (c >= at && c < at + cnt) {
-      s_b = b;
-      s_i = c - at;
-      s_n = n;
+    const int t = chunk_keys(p, s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+      const int b = b0 + tid;
+      const int n = b < p.B ? seq_len(p, b) : 0;
+      const int cnt = (n + t - 1) / t;
+      const int inc = wave_scan(cnt, lane);
+      if (lane == 63) s_cnt[wave] = inc;
+      __syncthreads();
+      int at = base + inc - cnt;
+      for (int x = 0; x < wave; ++x) at += s_cnt[x];
+      if (c >= at && c < at + cnt) {
+        s_r[0] = b;
+        s_r[1] = n;
+        s_r[2] = cnt;
+        s_r[3] = at;
+      }
+      base += s_cnt[0] + s_cnt[1] + s_cnt[2] + s_cnt[3];
+      __syncthreads();
+      if (c < base) break;
     }
-    base += s_cnt[0] + s_cnt[1] + s_cnt[2] + s_cnt[3];
-    __syncthreads();
-    if (c < base) break;
+    r.b = __builtin_amdgcn_readfirstlane(s_r[0]);
+    if (r.b < 0) return r;
+    r.n = __builtin_amdgcn_readfirstlane(s_r[1]);
+    r.cnt = __builtin_amdgcn_readfirstlane(s_r[2]);
+    r.c0 = __builtin_amdgcn_readfirstlane(s_r[3]);
   }
-  return Chunk{__builtin_amdgcn_readfirstlane(s_b), __builtin_amdgcn_readfirstlane(s_i),
-               __builtin_amdgcn_readfirstlane(s_n), __builtin_amdgcn_readfirstlane(t)};
+  r.i = c - r.c0;
+  // no more than t (a multiple of 64 that gives cnt of them), so none is empty
+  r.size = ((r.n + r.cnt - 1) / r.cnt + kKeys - 1) / kKeys * kKeys;
+  return r;
 }
 
 // ids received round-robin by the eight XCDs -> contiguous ranges for each
@@ -461,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(
     a.i0 = rt * 128;
     a.rows = min(128, rows - a.i0);
     a.g = g;
-    a.out0 = (int64_t)s * p.B * p.G * p.H;
+    a.out0 = ((int64_t)s * p.G + g) * rows + a.i0;
     a.score = nullptr;
   } else {                  // a chunk of a sequence's own keys
     const int x = id - p.nprefix, per = p.G * p.nht;
@@ -469,13 +520,13 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(
     if (c.b < 0) return;
     const int g = x % per / p.nht, ht = x % p.nht;
     const int64_t bg = (int64_t)c.b * p.G + g;
-    if (c.i == 0 && x % per == 0 && threadIdx.x == 0) p.plan[c.b] = int2{x / per, c.t};
+    if (c.i == 0 && x % per == 0 && threadIdx.x == 0) p.plan[c.b] = int2{c.c0, c.cnt};
     tile = p.H <= 32 ? 32 : 128;
     a.k = p.k + bg * p.D * p.S;
     a.v = p.v + bg * p.S * p.D;
     a.ld = p.S;
-    a.s0 = c.i * c.t;
-    a.s1 = min(c.n, a.s0 + c.t);
+    a.s0 = c.i * c.size;
+    a.s1 = min(c.n, a.s0 + c.size);
     a.g = -1;
     a.rows = min(128, p.H - ht * 128);
     a.i0 = (int)(bg * p.H) + ht * 128;
@@ -496,64 +547,82 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(
 // The parts of a row joined, and the weights
 // ---------------------------------------------------------------------------
 struct Splits {             // a row's partial rows: the prefix's, then its own
-  int64_t R, row, own0;     // own0 + s G H: its own part s
+  int64_t R, pre0, own0;    // pre0 + s R: prefix part s; own0 + s G H: its own part s
   int nsp, n, GH;
 };
 LOOM_DEV Splits row_splits(const StepParams& p, int b, int g, int h) {
   Splits s;
   s.R = (int64_t)p.B * p.G * p.H;
-  s.row = ((int64_t)b * p.G + g) * p.H + h;
+  s.pre0 = ((int64_t)g * p.B + b) * p.H + h;
+  // (both loaded at once: of a sequence without keys the plan is not written)
   const int len = seq_len(p, b);
-  const int2 pl = len > 0 ? p.plan[b] : int2{0, 1};
+  const int2 pl = p.plan[b];
   s.nsp = p.nsp;
   s.GH = p.G * p.H;
   s.own0 = s.nsp * s.R + ((int64_t)pl.x * p.G + g) * p.H + h;
-  s.n = s.nsp + (len + pl.y - 1) / pl.y;
+  s.n = s.nsp + (len > 0 ? pl.y : 0);
   return s;
 }
 LOOM_DEV int64_t split_at(const Splits& s, int u) {
-  return u < s.nsp ? u * s.R + s.row : s.own0 + (int64_t)(u - s.nsp) * s.GH;
+  return u < s.nsp ? u * s.R + s.pre0 : s.own0 + (int64_t)(u - s.nsp) * s.GH;
 }
 
 constexpr int kJoinMax = 64;
 
+// CH parts of a thread, u0, u0 + NG, ...: every load at once, then (max, sum, row)
+template <int CH>
+LOOM_DEV void join_parts(const StepParams& p, const Splits& sp, int u0, int NG, int d, float& M,
+                         float& den, f32x4_t& acc) {
+  f32x4_t l[CH], o[CH];
+#pragma unroll
+  for (int u = 0; u < CH; ++u) {
+    const int64_t at = split_at(sp, min(u0 + u * NG, sp.n - 1));   // clamped: weight 0
+    l[u] = p.ml[at];
+    o[u] = *reinterpret_cast<const f32x4_t*>(p.o + at * p.D + d);
+  }
+  float mc = M;
+#pragma unroll
+  for (int u = 0; u < CH; ++u) {
+    // a part without a key of finite score takes no part (its l is 0, not NaN)
+    if (u0 + u * NG >= sp.n || l[u][1] == 0.f) l[u][0] = -INFINITY;
+    mc = fmaxf(mc, l[u][0]);
+  }
+  const float base = mc == -INFINITY ? 0.f : mc;
+  const float r = fast_exp2(M - base);
+  den *= r;
+  acc *= r;
+  M = mc;
+#pragma unroll
+  for (int u = 0; u < CH; ++u) {
+    const float w = fast_exp2(l[u][0] - base);
+    den += w != 0.f ? w * l[u][1] : 0.f;
+    acc += w != 0.f ? o[u] * w : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// One workgroup per row, its threads in groups of D / 4 (four d each), group y
+// taking parts y, y + NG, ...; the groups' (max, sum, row) meet in LDS.
 template <bool F16>
-LOOM_DEV void join_row(const StepParams& p) {
-  constexpr int CH = 8;
+LOOM_DEV void join_row(const StepParams& p, int bg, int h) {
   __shared__ f32x4_t s_acc[256];
   __shared__ float s_m[kJoinMax], s_den[kJoinMax];
-  const int D = p.D, row = blockIdx.x;
-  const int bg = row / p.H, h = row - bg * p.H, b = bg / p.G, g = bg - b * p.G;
+  const int D = p.D;
+  const int b = p.G == 1 ? bg : bg / p.G, g = bg - b * p.G;
   const Splits sp = row_splits(p, b, g, h);
   const int ns = sp.n;
   const int TPR = D / 4, NG = min(256 / TPR, kJoinMax);
-  const int grp = (int)threadIdx.x / TPR, d = ((int)threadIdx.x % TPR) * 4;
+  const int grp = (int)threadIdx.x / TPR, d = ((int)threadIdx.x - grp * TPR) * 4;
   float M = -INFINITY, den = 0.f;
   f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if (grp < NG) {
-    for (int u0 = grp; u0 < ns; u0 += CH * NG) {
-      f32x4_t l[CH], o[CH];
-#pragma unroll
-      for (int u = 0; u < CH; ++u) {
-        const int64_t at = split_at(sp, min(u0 + u * NG, ns - 1));   // clamped: weight 0
-        l[u] = p.ml[at];
-        o[u] = *reinterpret_cast<const f32x4_t*>(p.o + at * D + d);
-      }
-      float mc = M;
-#pragma unroll
-      for (int u = 0; u < CH; ++u)
-        if (u0 + u * NG < ns && l[u][1] != 0.f) mc = fmaxf(mc, l[u][0]);
-      const float r = M == -INFINITY ? 0.f : fast_exp2(M - mc);
-      den *= r;
-      acc *= r;
-      M = mc;
-#pragma unroll
-      for (int u = 0; u < CH; ++u)
-        if (u0 + u * NG < ns && l[u][1] != 0.f) {
-          const float w = fast_exp2(l[u][0] - M);
-          den += w * l[u][1];
-          acc += o[u] * w;
-        }
+  if (grp < NG && grp < ns) {
+    if (ns <= NG) {
+      join_parts<1>(p, sp, grp, NG, d, M, den, acc);
+    } else if (ns <= 2 * NG) {
+      join_parts<2>(p, sp, grp, NG, d, M, den, acc);
+    } else if (ns <= 4 * NG) {
+      join_parts<4>(p, sp, grp, NG, d, M, den, acc);
+    } else {
+      for (int u0 = grp; u0 < ns; u0 += 8 * NG) join_parts<8>(p, sp, u0, NG, d, M, den, acc);
     }
     s_acc[threadIdx.x] = acc;
     if (d == 0) {
@@ -565,53 +634,66 @@ LOOM_DEV void join_row(const StepParams& p) {
   if (grp != 0) return;
   const int ng = min(NG, ns);
   float Mt = -INFINITY;
-  for (int y = 0; y < ng; ++y)
-    if (s_den[y] != 0.f) Mt = fmaxf(Mt, s_m[y]);
+  for (int y = 0; y < ng; ++y) Mt = fmaxf(Mt, s_m[y]);
+  const float base = Mt == -INFINITY ? 0.f : Mt;
   float dt = 0.f;
   f32x4_t at = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int y = 0; y < ng; ++y)
-    if (s_den[y] != 0.f) {
-      const float w = fast_exp2(s_m[y] - Mt);
-      dt += s_den[y] * w;
-      at += s_acc[y * TPR + (int)threadIdx.x] * w;
-    }
+  for (int y = 0; y < ng; ++y) {
+    const float w = fast_exp2(s_m[y] - base);
+    dt += s_den[y] * w;
+    at += s_acc[y * TPR + (int)threadIdx.x] * w;
+  }
   const float inv = dt != 0.f ? 1.f / dt : 0.f;
-  *reinterpret_cast<u32x2_t*>(p.out + (int64_t)row * D + d) =
+  *reinterpret_cast<u32x2_t*>(p.out + ((int64_t)bg * p.H + h) * D + d) =
       u32x2_t{pack2<F16>(at[0] * inv, at[1] * inv), pack2<F16>(at[2] * inv, at[3] * inv)};
 }
 
-// 256 keys of one (b, g): weights_out = weights + sum over its heads of
-// 2^(score - M) / l, M and l the row's base and sum over all its parts.  A wave
-// takes every fourth head, a lane four keys.
-constexpr int kWeightKeys = 256;
+// 128 keys of one (b, g): weights_out = weights + sum over its heads of
+// 2^(score - M) / l, M and l the row's base and sum over all its parts.  A half
+// wave takes every eighth head, a lane four keys; the scores are on their way
+// while M and l of up to 64 heads are found, four threads to a head.
+constexpr int kWeightKeys = 128;
 LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
-  __shared__ float s_M[32], s_inv[32];
-  __shared__ f32x4_t s_w[4][64];
+  constexpr int HG = 64, HN = HG / 8;
+  __shared__ float s_M[HG], s_inv[HG];
+  __shared__ f32x4_t s_w[8][32];
   const int b = bg / p.G, g = bg - b * p.G;
+  const Splits sp0 = row_splits(p, b, g, 0);
   const int len = seq_len(p, b);
   if (j0 >= len) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, hw = tid >> 5, l32 = tid & 31;
   f32x4_t sum = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int j = j0 + 4 * lane;
-  for (int h0 = 0; h0 < p.H; h0 += 32) {
-    const int hn = min(32, p.H - h0);
-    // eight threads to a head, each every eighth part
+  const int j = min(j0 + 4 * l32, p.Sp - 4);   // Sp is a multiple of 64: whole pieces
+  const float* const score = p.score + (int64_t)bg * p.H * p.Sp + j;
+  for (int h0 = 0; h0 < p.H; h0 += HG) {
+    const int hn = min(HG, p.H - h0);
+    f32x4_t sc[HN];
+#pragma unroll
+    for (int x = 0; x < HN; ++x)
+      sc[x] = *reinterpret_cast<const f32x4_t*>(
+          score + (int64_t)(h0 + min(hw + 8 * x, hn - 1)) * p.Sp);
     {
-      const int h = tid >> 3, y = tid & 7;
+      const int h = tid >> 2, y = tid & 3;
       float M = -INFINITY, L = 0.f;
       if (h < hn) {
-        const Splits sp = row_splits(p, b, g, h0 + h);
-        for (int u = y; u < sp.n; u += 8) {
-          const f32x4_t l = p.ml[split_at(sp, u)];
-          if (l[1] != 0.f) {
-            const float m = fmaxf(M, l[0]);
-            L = (M == -INFINITY ? 0.f : L * fast_exp2(M - m)) + l[2] * fast_exp2(l[0] - m);
-            M = m;
-          }
+        Splits sp = sp0;
+        sp.pre0 += h0 + h;
+        sp.own0 += h0 + h;
+        for (int u0 = y; u0 < sp.n; u0 += 16) {
+          f32x4_t l[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) l[x] = p.ml[split_at(sp, min(u0 + 4 * x, sp.n - 1))];
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (u0 + 4 * x < sp.n && l[x][1] != 0.f) {
+              const float m = fmaxf(M, l[x][0]);
+              L = (M == -INFINITY ? 0.f : L * fast_exp2(M - m)) + l[x][2] * fast_exp2(l[x][0] - m);
+              M = m;
+            }
         }
       }
 #pragma unroll
-      for (int x = 1; x < 8; x <<= 1) {
+      for (int x = 1; x < 4; x <<= 1) {
         const float M2 = __shfl_xor(M, x), L2 = __shfl_xor(L, x);
         const float m = fmaxf(M, M2);
         L = (L != 0.f ? L * fast_exp2(M - m) : 0.f) + (L2 != 0.f ? L2 * fast_exp2(M2 - m) : 0.f);
@@ -623,37 +705,40 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
       }
     }
     __syncthreads();
-    if (j < len)      // Sp is a multiple of 64: a whole piece
-      for (int h = wave; h < hn; h += 4) {
-        const f32x4_t sc = *reinterpret_cast<const f32x4_t*>(
-            p.score + ((int64_t)bg * p.H + h0 + h) * p.Sp + j);
+#pragma unroll
+    for (int x = 0; x < HN; ++x) {
+      const int h = hw + 8 * x;
+      if (h < hn) {
         const float M = s_M[h], inv = s_inv[h];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(sc[i] - M) * inv;
+        for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(sc[x][i] - M) * inv;
       }
+    }
     __syncthreads();
   }
-  s_w[wave][lane] = sum;
+  s_w[hw][l32] = sum;
   __syncthreads();
-  const float* f = reinterpret_cast<const float*>(s_w);
   const int at = j0 + tid;
-  if (at < len)
-    p.w_out[(int64_t)bg * p.S + at] =
-        p.w[(int64_t)bg * p.S + at] + ((f[tid] + f[256 + tid]) + (f[512 + tid] + f[768 + tid]));
+  if (tid < kWeightKeys && at < len) {
+    const float* f = reinterpret_cast<const float*>(s_w) + tid;
+    float w = 0.f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) w += f[x * kWeightKeys];
+    p.w_out[(int64_t)bg * p.S + at] = p.w[(int64_t)bg * p.S + at] + w;
+  }
 }
 
+// A row per workgroup (blockIdx.x < H), then the weights' parts of the (b, g).
 template <bool F16, bool WT>
 __global__ void __launch_bounds__(256) cache_join_kernel(StepParams p) {
-  const int R = p.B * p.G * p.H;
+  const int x = blockIdx.x, bg = blockIdx.y;
   if constexpr (WT) {
-    if ((int)blockIdx.x >= R) {
-      const int nw = (p.S + kWeightKeys - 1) / kWeightKeys;
-      const int x = blockIdx.x - R;
-      add_weights(p, x / nw, x % nw * kWeightKeys);
+    if (x >= p.H) {
+      add_weights(p, bg, (x - p.H) * kWeightKeys);
       return;
     }
   }
-  join_row<F16>(p);
+  join_row<F16>(p, bg, x);
 }
 
 // The launch's shape, from the extents alone.
@@ -664,7 +749,13 @@ struct Shape {
 
 Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P, int64_t S) {
   Shape s{};
-  const int64_t slots = D > 128 ? 256 : 512;   // workgroups that run at once
+#ifndef PW
+#define PW 256
+#endif
+#ifndef CF
+#define CF 1
+#endif
+  const int64_t slots = (D > 128 ? 256 : 512) * CF;   // workgroups that run at once
   s.nht = H <= 32 ? 1 : (int)cdiv64(H, 128);
   s.chunks = (int)std::max<int64_t>(1, slots / (G * s.nht));
   s.max_chunks = s.chunks + B;
@@ -672,8 +763,8 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P, int64_t S)
   if (P > 0) {
     const int64_t rows = B * H;
     s.ntp = rows <= 32 ? 1 : (int)cdiv64(rows, 128);
-    const int64_t least = rows <= 32 ? 64 : 256;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / (G * s.ntp), 32));
+    const int64_t least = rows <= 32 ? 64 : 128;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(PW / (G * s.ntp), 64));
     s.tile_p = (int)(cdiv64(std::max(cdiv64(P, want), least), kKeys) * kKeys);
     s.nsp = (int)cdiv64(P, s.tile_p);
     s.nprefix = (int)(G * s.ntp * s.nsp);
@@ -784,12 +875,12 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   }
   int rc = loom_check_launch(err, errlen, "cache_decode (split)");
   if (rc) return rc;
-  const int64_t R = B * G * H;
+  const unsigned rows = (unsigned)H, bgs = (unsigned)(B * G);
   if (weights)
     hipLaunchKernelGGL((cache_join_kernel<F16, true>),
-                       dim3((unsigned)(R + B * G * cdiv64(S, kWeightKeys))), block, 0, st, p);
+                       dim3(rows + (unsigned)cdiv64(S, kWeightKeys), bgs), block, 0, st, p);
   else
-    hipLaunchKernelGGL((cache_join_kernel<F16, false>), dim3((unsigned)R), block, 0, st, p);
+    hipLaunchKernelGGL((cache_join_kernel<F16, false>), dim3(rows, bgs), block, 0, st, p);
   return loom_check_launch(err, errlen, "cache_decode (join)");
 }
 
