@@ -37,8 +37,9 @@ struct StepParams {
   int B, G, H, D, P, S, Sp;
   int nht;          // row tiles of a (b, g)'s H heads
   int chunks;       // chunks that the whole batch aims at
-  int ntp, nsp, tile_p;   // the prefix: row tiles per head, splits, keys of one
+  int rtp, ntp, nsp, tile_p;   // the prefix: rows of a tile, tiles per head, splits, keys of one
   int nprefix;      // workgroups of the prefix
+  int wkeys;        // keys of a workgroup that gathers weights: 128 or 256
   float c2;         // scale * log2(e)
 };
 
@@ -188,26 +189,53 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
     const int kv0 = s0 + blk * kKeys + 32 * (KG == 2 ? kh : 0);
     const lds_char_t* ks = stK(s);
     const lds_char_t* vs = stV(s);
+    // K^T operand of 16 keys jt, 32 d; V^T operand of 16 d, 32 keys hv.  A half's
+    // are read well before the MFMAs that use them, V's before the softmax:
+    // left to itself the compiler keeps two in flight, and every MFMA waits
+    // for the LDS
+    auto k_op = [&](int jt, int ds) {
+      const int d = ds * 32 + g * 8 + a4;
+      const int ch = (2 * jt + (c4 >> 1)) ^ ck_swz(d);
+      const lds_char_t* q = ks + d * (kKeys * 2) + ch * 16 + (c4 & 1) * 8;
+      const u32x2_t lo = lds_read_tr16(q);
+      const u32x2_t hi = lds_read_tr16(q + 4 * (kKeys * 2));
+      return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    };
+    auto v_op = [&](int hv, int dt) {
+      const int k0r = 32 * hv + 4 * g + a4;
+      const int ch = (2 * dt + (c4 >> 1)) ^ cv_swz<D>(k0r);
+      const lds_char_t* q = vs + k0r * VROW + ch * 16 + (c4 & 1) * 8;
+      const u32x2_t lo = lds_read_tr16(q);
+      const u32x2_t hi = lds_read_tr16(q + 16 * VROW);
+      return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    };
+    constexpr int kFence = 0x0006;              // VALU and SALU may cross
+    const int h0 = KG == 2 ? kh : 0;
     // st[j][qt][i]: key kv0 + 16 j + 4 g + i, row 16 qt + r of this wave
     f32x4_t st[2 * NH][QT];
 #pragma unroll
     for (int j = 0; j < 2 * NH; ++j)
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) st[j][qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    u32x4_t kf[2][DSTEPS], vf[DT];
 #pragma unroll
-    for (int j = 0; j < 2 * NH; ++j) {
+    for (int h = 0; h < NH; ++h) {
 #pragma unroll
-      for (int ds = 0; ds < DSTEPS; ++ds) {
-        const int d = ds * 32 + g * 8 + a4;
-        const int ch = (2 * ((KG == 2 ? 2 * kh : 0) + j) + (c4 >> 1)) ^ ck_swz(d);
-        const lds_char_t* q = ks + d * (kKeys * 2) + ch * 16 + (c4 & 1) * 8;
-        const u32x2_t lo = lds_read_tr16(q);
-        const u32x2_t hi = lds_read_tr16(q + 4 * (kKeys * 2));
-        const u32x4_t kf = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+      for (int ds = 0; ds < DSTEPS; ++ds)
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) st[j][qt] = mfma16t<F16>(kf, qf[ds][qt], st[j][qt]);
-      }
+        for (int j = 0; j < 2; ++j) kf[j][ds] = k_op(2 * (h0 + h) + j, ds);
+      __builtin_amdgcn_sched_barrier(kFence);
+#pragma unroll
+      for (int ds = 0; ds < DSTEPS; ++ds)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+            st[2 * h + j][qt] = mfma16t<F16>(kf[j][ds], qf[ds][qt], st[2 * h + j][qt]);
     }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) vf[dt] = v_op(h0, dt);
+    __builtin_amdgcn_sched_barrier(kFence);
     const bool edge = kv0 + 32 * NH > s1;
     if constexpr (WT) {
       if (a.score) {
@@ -282,14 +310,9 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const int k0r = 32 * (KG == 2 ? kh : h) + 4 * g + a4;
-        const int ch = (2 * dt + (c4 >> 1)) ^ cv_swz<D>(k0r);
-        const lds_char_t* q = vs + k0r * VROW + ch * 16 + (c4 & 1) * 8;
-        const u32x2_t lo = lds_read_tr16(q);
-        const u32x2_t hi = lds_read_tr16(q + 16 * VROW);
-        const u32x4_t vf = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) ot[dt][qt] = mfma16t<F16>(vf, pf[qt], ot[dt][qt]);
+        for (int qt = 0; qt < QT; ++qt) ot[dt][qt] = mfma16t<F16>(vf[dt], pf[qt], ot[dt][qt]);
+        if (h + 1 < NH) vf[dt] = v_op(h + 1, dt);
       }
     }
   };
@@ -503,14 +526,14 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(
     const int x = xcd_range(id, p.nprefix);
     const int rt = x % p.ntp, s = x / p.ntp % p.nsp, g = x / (p.ntp * p.nsp);
     const int rows = p.B * p.H;
-    tile = rows <= 32 ? 32 : 128;
+    tile = p.rtp;
     a.k = p.pk + (int64_t)g * p.D * p.P;
     a.v = p.pv + (int64_t)g * p.P * p.D;
     a.ld = p.P;
     a.s0 = s * p.tile_p;
     a.s1 = min(p.P, a.s0 + p.tile_p);
-    a.i0 = rt * 128;
-    a.rows = min(128, rows - a.i0);
+    a.i0 = rt * tile;
+    a.rows = min(tile, rows - a.i0);
     a.g = g;
     a.out0 = ((int64_t)s * p.G + g) * rows + a.i0;
     a.score = nullptr;
@@ -521,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(
     const int g = x % per / p.nht, ht = x % p.nht;
     const int64_t bg = (int64_t)c.b * p.G + g;
     if (c.i == 0 && x % per == 0 && threadIdx.x == 0) p.plan[c.b] = int2{c.c0, c.cnt};
-    tile = p.H <= 32 ? 32 : 128;
+    tile = p.H <= 32 ? 32 : p.H <= 64 ? 64 : 128;
     a.k = p.k + bg * p.D * p.S;
     a.v = p.v + bg * p.S * p.D;
     a.ld = p.S;
@@ -537,6 +560,9 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(
   if (tile == 32) {
     if (kreg) run_part<D, F16, WT, 1, 2, true>(p, a, smem);
     else run_part<D, F16, WT, 1, 2, false>(p, a, smem);
+  } else if (tile == 64) {
+    if (kreg) run_part<D, F16, WT, 1, 1, true>(p, a, smem);
+    else run_part<D, F16, WT, 1, 1, false>(p, a, smem);
   } else {
     if (kreg) run_part<D, F16, WT, 2, 1, true>(p, a, smem);
     else run_part<D, F16, WT, 2, 1, false>(p, a, smem);
@@ -648,37 +674,41 @@ LOOM_DEV void join_row(const StepParams& p, int bg, int h) {
       u32x2_t{pack2<F16>(at[0] * inv, at[1] * inv), pack2<F16>(at[2] * inv, at[3] * inv)};
 }
 
-// 128 keys of one (b, g): weights_out = weights + sum over its heads of
-// 2^(score - M) / l, M and l the row's base and sum over all its parts.  A half
-// wave takes every eighth head, a lane four keys; the scores are on their way
-// while M and l of up to 64 heads are found, four threads to a head.
-constexpr int kWeightKeys = 128;
+// The keys j0 .. j0 + p.wkeys - 1 of one (b, g): weights_out = weights + sum over its heads of
+// 2^(score - M) / l, M and l the row's base and sum over all its parts.  A lane
+// takes four keys, the workgroup's 1024 / wkeys groups of lanes every so many
+// heads; a group's first scores are on their way while M and l are found, four
+// threads to a head.
 LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
-  constexpr int HG = 64, HN = HG / 8;
-  __shared__ float s_M[HG], s_inv[HG];
-  __shared__ f32x4_t s_w[8][32];
-  const int b = bg / p.G, g = bg - b * p.G;
+  constexpr int HB = 256, HN = 8;
+  __shared__ float s_M[HB], s_inv[HB];
+  __shared__ f32x4_t s_w[kThreads];
+  const int wkeys = p.wkeys, NG = 1024 / wkeys, LPG = wkeys / 4;
+  const int b = p.G == 1 ? bg : bg / p.G, g = bg - b * p.G;
   const Splits sp0 = row_splits(p, b, g, 0);
   const int len = seq_len(p, b);
   if (j0 >= len) return;
-  const int tid = threadIdx.x, hw = tid >> 5, l32 = tid & 31;
+  const int tid = threadIdx.x, grp = tid / LPG, lg = tid - grp * LPG;
   f32x4_t sum = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int j = min(j0 + 4 * l32, p.Sp - 4);   // Sp is a multiple of 64: whole pieces
+  const int j = min(j0 + 4 * lg, p.Sp - 4);    // Sp is a multiple of 64: whole pieces
   const float* const score = p.score + (int64_t)bg * p.H * p.Sp + j;
-  for (int h0 = 0; h0 < p.H; h0 += HG) {
-    const int hn = min(HG, p.H - h0);
-    f32x4_t sc[HN];
+  f32x4_t sc[HN];
+  auto load = [&](int h0, int hn) {            // heads h0 + grp + NG x below hn
 #pragma unroll
     for (int x = 0; x < HN; ++x)
       sc[x] = *reinterpret_cast<const f32x4_t*>(
-          score + (int64_t)(h0 + min(hw + 8 * x, hn - 1)) * p.Sp);
-    {
-      const int h = tid >> 2, y = tid & 3;
+          score + (int64_t)min(h0 + grp + NG * x, hn - 1) * p.Sp);
+  };
+  for (int hb = 0; hb < p.H; hb += HB) {
+    const int hn = min(p.H, hb + HB);
+    load(hb, hn);
+    for (int h0 = hb; h0 < hn; h0 += 64) {
+      const int h = h0 + (tid >> 2), y = tid & 3;
       float M = -INFINITY, L = 0.f;
       if (h < hn) {
         Splits sp = sp0;
-        sp.pre0 += h0 + h;
-        sp.own0 += h0 + h;
+        sp.pre0 += h;
+        sp.own0 += h;
         for (int u0 = y; u0 < sp.n; u0 += 16) {
           f32x4_t l[4];
 #pragma unroll
@@ -699,32 +729,34 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
         L = (L != 0.f ? L * fast_exp2(M - m) : 0.f) + (L2 != 0.f ? L2 * fast_exp2(M2 - m) : 0.f);
         M = m;
       }
-      if (y == 0) {
-        s_M[h] = M == -INFINITY ? 0.f : M;
-        s_inv[h] = L != 0.f ? 1.f / L : 0.f;
+      if (y == 0 && h < hn) {
+        s_M[h - hb] = M == -INFINITY ? 0.f : M;
+        s_inv[h - hb] = L != 0.f ? 1.f / L : 0.f;
       }
     }
     __syncthreads();
+    for (int h0 = hb; h0 < hn; h0 += NG * HN) {
+      if (h0 > hb) load(h0, hn);
 #pragma unroll
-    for (int x = 0; x < HN; ++x) {
-      const int h = hw + 8 * x;
-      if (h < hn) {
-        const float M = s_M[h], inv = s_inv[h];
+      for (int x = 0; x < HN; ++x) {
+        const int h = h0 + grp + NG * x;
+        if (h < hn) {
+          const float M = s_M[h - hb], inv = s_inv[h - hb];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(sc[x][i] - M) * inv;
+          for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(sc[x][i] - M) * inv;
+        }
       }
     }
     __syncthreads();
   }
-  s_w[hw][l32] = sum;
+  s_w[tid] = sum;
   __syncthreads();
-  const int at = j0 + tid;
-  if (tid < kWeightKeys && at < len) {
+  if (tid < wkeys && j0 + tid < len) {
     const float* f = reinterpret_cast<const float*>(s_w) + tid;
     float w = 0.f;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) w += f[x * kWeightKeys];
-    p.w_out[(int64_t)bg * p.S + at] = p.w[(int64_t)bg * p.S + at] + w;
+    for (int x = 0; x < NG; ++x) w += f[x * wkeys];
+    const int64_t at = (int64_t)bg * p.S + j0 + tid;
+    p.w_out[at] = p.w[at] + w;
   }
 }
 
@@ -734,7 +766,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(StepParams p) {
   const int x = blockIdx.x, bg = blockIdx.y;
   if constexpr (WT) {
     if (x >= p.H) {
-      add_weights(p, bg, (x - p.H) * kWeightKeys);
+      add_weights(p, bg, (x - p.H) * p.wkeys);
       return;
     }
   }
@@ -743,28 +775,27 @@ __global__ void __launch_bounds__(256) cache_join_kernel(StepParams p) {
 
 // The launch's shape, from the extents alone.
 struct Shape {
-  int nht, chunks, ntp, nsp, tile_p, nprefix;
+  int nht, chunks, rtp, ntp, nsp, tile_p, nprefix;
   int64_t max_chunks, Sp, rows;
 };
 
 Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P, int64_t S) {
   Shape s{};
-#ifndef PW
-#define PW 256
-#endif
-#ifndef CF
-#define CF 1
-#endif
-  const int64_t slots = (D > 128 ? 256 : 512) * CF;   // workgroups that run at once
+  const int64_t slots = D > 128 ? 256 : 512;   // workgroups that run at once
   s.nht = H <= 32 ? 1 : (int)cdiv64(H, 128);
   s.chunks = (int)std::max<int64_t>(1, slots / (G * s.nht));
   s.max_chunks = s.chunks + B;
   s.Sp = cdiv64(S, kKeys) * kKeys;
   if (P > 0) {
     const int64_t rows = B * H;
-    s.ntp = rows <= 32 ? 1 : (int)cdiv64(rows, 128);
+    // 128 rows share a stage once there are eight stages of them for every CU
+    // (G8 B48 H8 P16384: 50 us of split kernel against 68 with 64); below, twice
+    // as many tiles over half as many splits, whose sums cost more than the
+    // stages (B32 H32 P8192 21.8 us against 25.0, P2048 14.4 against 15.8)
+    s.rtp = rows <= 32 ? 32 : G * cdiv64(rows, 128) * cdiv64(P, kKeys) < 8 * 256 ? 64 : 128;
+    s.ntp = (int)cdiv64(rows, s.rtp);
     const int64_t least = rows <= 32 ? 64 : 128;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(PW / (G * s.ntp), 64));
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / (G * s.ntp), 64));
     s.tile_p = (int)(cdiv64(std::max(cdiv64(P, want), least), kKeys) * kKeys);
     s.nsp = (int)cdiv64(P, s.tile_p);
     s.nprefix = (int)(G * s.ntp * s.nsp);
@@ -854,10 +885,15 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   p.Sp = (int)s.Sp;
   p.nht = s.nht;
   p.chunks = s.chunks;
+  p.rtp = s.rtp;
   p.ntp = s.ntp;
   p.nsp = s.nsp;
   p.tile_p = s.tile_p;
   p.nprefix = s.nprefix;
+  // 256 keys spread the heads' statistics over more of them (B32 H32 n6144 33.6
+  // against 35.3 us for the step); 128 give few workgroups more of the CUs (B1
+  // S4096 12.9 against 13.3, B16 H71 n1024 17.9 against 18.9)
+  p.wkeys = B * G * cdiv64(S, 256) < 256 ? 128 : 256;
   p.c2 = scale * 1.4426950408889634f;
   if (loom_validate_only()) return loom_ok(err, errlen);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -878,7 +914,7 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   const unsigned rows = (unsigned)H, bgs = (unsigned)(B * G);
   if (weights)
     hipLaunchKernelGGL((cache_join_kernel<F16, true>),
-                       dim3(rows + (unsigned)cdiv64(S, kWeightKeys), bgs), block, 0, st, p);
+                       dim3(rows + (unsigned)cdiv64(S, p.wkeys), bgs), block, 0, st, p);
   else
     hipLaunchKernelGGL((cache_join_kernel<F16, false>), dim3(rows, bgs), block, 0, st, p);
   return loom_check_launch(err, errlen, "cache_decode (join)");
