@@ -15,6 +15,8 @@
 //           slots.
 #include "common.h"
 
+#include <type_traits>
+
 namespace {
 
 LOOM_DEV int cache_len(const int* lens, int b, int S) { return min(max(lens[b], 0), S); }
@@ -122,188 +124,363 @@ struct EvictParams {
   int* index;          // [B, G, keep]
   int B, G, D, S, So, keep, recent, sinks;
   int nk, njk, rows_k;  // K parts of a (b, g): njk stretches of slots x rows_k rows each
+  int slots_v;          // slots of a V part, at most 256
 };
 
-// A weight as a whole number of the same order: NaN below -inf, -0 as +0.
+// A weight as a whole number of the same order, above 0: NaN below -inf (1), -0
+// as +0 (what the addition gives).
 LOOM_DEV uint32_t weight_key(float w) {
-  const uint32_t u = w == 0.f ? 0u : __float_as_uint(w);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return w == w ? k : 1u;
 }
 
 constexpr int kSelWaves = 16, kSel = 64 * kSelWaves;
-constexpr int kBins = 2048;     // 11 bits a digit: three digits of a 32-bit key
+constexpr int kBins = 4096;     // 12 bits of the first digit, 10 of the others
+// copies of the histogram (lane l counts in copy l % 4: fewer lanes of one
+// instruction meet in a bin), 16 banks apart
+constexpr int kCopies = 4, kCopyStep = kBins + 16;
+constexpr int kList = 256;
+
+LOOM_DEV int lanes_below(uint64_t m) {   // set lanes below this one
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
+                                        __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+}
+// Inclusive sum over the lanes below: DPP adds (a shuffle goes through the LDS
+// unit, which sixteen waves share here).
+template <int CTRL, int ROWS>
+LOOM_DEV uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+LOOM_DEV uint32_t row_scan(uint32_t v) {   // within 16 lanes
+  v = dpp_add<0x111, 0xf>(v);              // row_shr:1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  return dpp_add<0x118, 0xf>(v);
+}
+LOOM_DEV uint32_t lane_scan(uint32_t v) {
+  v = row_scan(v);
+  v = dpp_add<0x142, 0xa>(v);              // row_bcast:15 into rows 1 and 3
+  return dpp_add<0x143, 0xc>(v);           // row_bcast:31 into rows 2 and 3
+}
+// Sum of the 16 waves' values below `wave`.
+LOOM_DEV uint32_t waves_before(const uint32_t* v, int lane, int wave) {
+  const uint32_t x = row_scan(lane < wave ? v[lane & (kSelWaves - 1)] : 0u);
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 15);
+}
 
 // The kept slots of one (sequence, KV head), ascending, by one workgroup: a
-// radix selection of the weights' keys (11, 11 and 10 bits, highest first) finds
-// the smallest key that stays and how many of its equals do; each wave then
-// counts what stays of its stretch of slots and writes it behind the waves
-// before it.  A wave owns a contiguous stretch; with KPT > 0 its keys stay in
-// registers (KPT a lane, slots 64 apart), else (KPT 0, longer caches) every pass
-// reads the weights again.
+// histogram of the weights' keys by their first 12 bits (sign, exponent, 3 bits)
+// finds the bin with the smallest key that stays; if it holds at most 256 keys,
+// one wave finds that key among them bit by bit, else two more digits of 10 bits
+// are counted.  Each wave then counts what stays of its stretch of slots and
+// writes it behind the waves before it.  Sinks and recent slots take the highest
+// key and slots behind the length 0, below every weight's, so no pass looks at
+// slot numbers: the instructions per key bound this kernel (a CU's four SIMDs
+// each run four of its waves).  With KPT > 0 the keys stay in registers (KPT a
+// lane, slots 64 apart; in LDS, with rolled loops, 23 us against 15 at 16 a
+// lane), else (KPT 0, longer caches) every pass reads the weights again.
 template <int KPT>
 __global__ void __launch_bounds__(kSel) cache_select_kernel(EvictParams p) {
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t s_part[kSelWaves], s_digit, s_left;
-  __shared__ int s_sel[kSelWaves], s_eq[kSelWaves];
+  __shared__ __attribute__((aligned(16))) uint32_t hist[kCopyStep * kCopies], s_list[kList];
+  __shared__ uint32_t s_part[kSelWaves], s_digit, s_left, s_count, s_n;
+  __shared__ uint32_t s_sel[kSelWaves], s_eq[kSelWaves];
   const int bg = blockIdx.x, b = bg / p.G;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // the weights are on their way with the length
+  const rsrc_t w = make_rsrc(p.w + (int64_t)bg * p.S, (uint32_t)p.S * 4u);
+  auto load = [&](int i) { return __uint_as_float(buf_load4(w, (uint32_t)i * 4u)); };
+  float x[KPT > 0 ? KPT : 1];
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) x[u] = load((wave * KPT + u) * 64 + lane);
+  }
   const int n = cache_len(p.lens, b, p.S);
+  auto clear = [&]() {
+    for (int i = tid; i < kCopyStep * kCopies / 4; i += kSel)
+      *reinterpret_cast<u32x4_t*>(hist + 4 * i) = u32x4_t{0u, 0u, 0u, 0u};
+  };
+  clear();
+  if (tid == 0) s_n = 0;
   int* const idx = p.index + (int64_t)bg * p.keep;
   if (bg - b * p.G == 0 && tid == 0) p.lens_out[b] = min(n, p.keep);
   if (n <= p.keep) {
     for (int j = tid; j < p.keep; j += kSel) idx[j] = j < n ? j : -1;
     return;
   }
-  const float* const w = p.w + (int64_t)bg * p.S;
   const int lo = p.sinks, hi = n - p.recent;   // the slots that are weighed
   const int per = KPT > 0 ? KPT : (n + kSel - 1) / kSel;   // keys of a lane
   const int i0 = wave * per * 64;              // this wave's slots: i0 + 64 u + lane
+  auto key_of = [&](int base, float v) {       // of slot base + lane
+    uint32_t k = weight_key(v);
+    if (base < lo || base + 64 > hi) {         // wave-uniform
+      const int i = base + lane;
+      k = i < lo || i >= hi ? (i < n ? ~0u : 0u) : k;
+    }
+    return k;
+  };
   uint32_t reg[KPT > 0 ? KPT : 1];
   if constexpr (KPT > 0) {
 #pragma unroll
-    for (int u = 0; u < KPT; ++u) {
-      const int i = i0 + u * 64 + lane;
-      reg[u] = weight_key(w[min(i, n - 1)]);
-    }
+    for (int u = 0; u < KPT; ++u) reg[u] = key_of(i0 + u * 64, x[u]);
   }
-  auto each = [&](auto f) {
+  auto each = [&](auto f) {                    // f(first slot of the wave's 64, key)
     if constexpr (KPT > 0) {
 #pragma unroll
-      for (int u = 0; u < KPT; ++u) f(i0 + u * 64 + lane, reg[u]);
+      for (int u = 0; u < KPT; ++u) f(i0 + u * 64, reg[u]);
     } else {
-      for (int u = 0; u < per && i0 + u * 64 < n; ++u) {
-        const int i = i0 + u * 64 + lane;
-        f(i, weight_key(w[min(i, n - 1)]));
-      }
+      for (int u = 0; u < per && i0 + u * 64 < n; ++u)
+        f(i0 + u * 64, key_of(i0 + u * 64, load(i0 + u * 64 + lane)));
     }
   };
-  uint32_t left = (uint32_t)(p.keep - p.sinks - p.recent);   // how many weighed ones stay
-  const bool none = left == 0;
-  uint32_t prefix = 0;
-  for (int pass = 0; pass < 3 && !none; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const uint32_t above = pass == 0 ? 0u : ~0u << (pass == 1 ? 21 : 10);   // digits found
-    const uint32_t mask = pass == 2 ? 1023u : 2047u;
-    for (int i = tid; i < kBins; i += kSel) hist[i] = 0;
+  uint32_t left = (uint32_t)p.keep;            // how many stay; n > keep keys are above 0
+  uint32_t prefix = 0, found = 0;              // the threshold's digits and their mask
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = 20 - 10 * pass;
+    const uint32_t mask = pass == 0 ? kBins - 1 : 1023u;
+    if (pass > 0) clear();
     __syncthreads();
-    each([&](int i, uint32_t key) {
-      const bool in = i >= lo && i < hi && (key & above) == prefix;
-      const uint32_t dig = (key >> shift) & mask;
-      const uint64_t m = __builtin_amdgcn_ballot_w64(in);
-      if (m == 0) return;
-      // lanes of one digit (a stretch of equal weights) count as one
-      const uint32_t d0 = __builtin_amdgcn_readlane(dig, __builtin_ctzll(m));
-      const uint64_t same = __builtin_amdgcn_ballot_w64(in && dig == d0);
-      if (in && dig != d0) atomicAdd(&hist[dig], 1u);
-      if (lane == 0) atomicAdd(&hist[d0], (uint32_t)__popcll(same));
-    });
+    uint32_t* const mine = hist + lane % kCopies * kCopyStep;
+    if (pass == 0)
+      each([&](int, uint32_t key) {
+        if (key != 0u) atomicAdd(&mine[key >> 20], 1u);
+      });
+    else
+      each([&](int, uint32_t key) {
+        if (key != 0u && (key & found) == prefix) atomicAdd(&mine[(key >> shift) & mask], 1u);
+      });
     __syncthreads();
-    // the digit at which the count from the top reaches `left`: two bins a
+    // the digit at which the count from the top reaches `left`: four bins a
     // thread, highest first
-    const int bin = kBins - 1 - 2 * tid;
-    const uint32_t h0 = hist[bin], h1 = hist[bin - 1];
-    uint32_t inc = h0 + h1;
+    const int bin = kBins - 4 - 4 * tid;
+    u32x4_t h = u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const uint32_t o = __shfl_up(inc, m);
-      if (lane >= m) inc += o;
-    }
+    for (int c = 0; c < kCopies; ++c)
+      h += *reinterpret_cast<const u32x4_t*>(hist + c * kCopyStep + bin);
+    const uint32_t sum = h[0] + h[1] + h[2] + h[3];
+    const uint32_t inc = lane_scan(sum);
     if (lane == 63) s_part[wave] = inc;
     __syncthreads();
-    uint32_t before = inc - h0 - h1;            // keys of higher digits
-    for (int x = 0; x < wave; ++x) before += s_part[x];
-    if (before < left && before + h0 >= left) {
-      s_digit = bin;
+    uint32_t before = inc - sum + waves_before(s_part, lane, wave);   // keys of higher digits
+    if (before < left && before + sum >= left) {
+      int d = 3;
+#pragma unroll
+      for (int c = 3; c > 0; --c)
+        if (d == c && before + h[c] < left) {
+          before += h[c];
+          d = c - 1;
+        }
+      s_digit = bin + d;
       s_left = left - before;
-    } else if (before + h0 < left && before + h0 + h1 >= left) {
-      s_digit = bin - 1;
-      s_left = left - before - h0;
+      s_count = d == 3 ? h[3] : d == 2 ? h[2] : d == 1 ? h[1] : h[0];
     }
     __syncthreads();
     prefix |= s_digit << shift;
+    found |= mask << shift;
     left = s_left;
+    const int cnt = (int)s_count;
+    if (pass == 2 || cnt > kList) continue;
+    // few enough: into a list, each lane's behind those of the lanes before it
+    int c = 0;
+    each([&](int, uint32_t key) { c += key != 0u && (key & found) == prefix; });
+    if (__builtin_amdgcn_ballot_w64(c != 0) != 0) {
+      int to = (int)lane_scan((uint32_t)c);
+      const int all = __builtin_amdgcn_readlane(to, 63);
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&s_n, (uint32_t)all);
+      to += (int)__builtin_amdgcn_readfirstlane(at) - c;
+      each([&](int, uint32_t key) {
+        if (key != 0u && (key & found) == prefix) s_list[to++] = key;
+      });
+    }
+    __syncthreads();
+    if (wave == 0) {                           // the left-th largest of the list
+      uint32_t k[kList / 64], t = prefix;
+#pragma unroll
+      for (int y = 0; y < kList / 64; ++y) k[y] = 64 * y + lane < cnt ? s_list[64 * y + lane] : 0u;
+      auto above = [&](uint32_t v) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int y = 0; y < kList / 64; ++y) m += __popcll(__builtin_amdgcn_ballot_w64(k[y] > v));
+        return m;
+      };
+      for (uint32_t bit = 1u << (shift - 1); bit != 0; bit >>= 1)
+        if (above((t | bit) - 1) >= left) t |= bit;
+      const uint32_t gt = above(t);
+      if (lane == 0) {
+        s_digit = t;
+        s_left = left - gt;
+      }
+    }
+    __syncthreads();
+    prefix = s_digit;
+    left = s_left;
+    break;
   }
   // stays: above the threshold, and the first `left` equal to it
   int sel = 0, eq = 0;
-  each([&](int i, uint32_t key) {
-    const bool in = i < n, must = in && (i < lo || i >= hi), free = in && !must && !none;
-    sel += __popcll(__builtin_amdgcn_ballot_w64(must || (free && key > prefix)));
-    eq += __popcll(__builtin_amdgcn_ballot_w64(free && key == prefix));
+  each([&](int, uint32_t key) {
+    sel += __popcll(__builtin_amdgcn_ballot_w64(key > prefix));
+    eq += __popcll(__builtin_amdgcn_ballot_w64(key == prefix));
   });
   if (lane == 0) {
     s_sel[wave] = sel;
     s_eq[wave] = eq;
   }
   __syncthreads();
-  int at = 0, eqs = 0;         // kept slots and threshold equals before this wave
-  for (int x = 0; x < wave; ++x) {
-    at += s_sel[x];
-    eqs += s_eq[x];
-  }
-  at += min(eqs, (int)left);
-  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  // kept slots and threshold equals before this wave
+  int eqs = (int)waves_before(s_eq, lane, wave);
+  int at = (int)waves_before(s_sel, lane, wave) + min(eqs, (int)left);
   each([&](int i, uint32_t key) {
-    const bool in = i < n, must = in && (i < lo || i >= hi), free = in && !must && !none;
-    const bool same = free && key == prefix;
-    const uint64_t eqm = __builtin_amdgcn_ballot_w64(same);
-    const bool stays = must || (free && key > prefix) ||
-                       (same && eqs + __popcll(eqm & below) < (int)left);
-    const uint64_t m = __builtin_amdgcn_ballot_w64(stays);
-    if (stays) idx[at + __popcll(m & below)] = i;
+    uint64_t m = __builtin_amdgcn_ballot_w64(key > prefix);
+    const uint64_t eqm = __builtin_amdgcn_ballot_w64(key == prefix);
+    if (eqm != 0) {
+      m |= __builtin_amdgcn_ballot_w64(key == prefix && eqs + lanes_below(eqm) < (int)left);
+      eqs += __popcll(eqm);
+    }
+    if ((m >> lane) & 1) idx[at + lanes_below(m)] = i + lane;
     at += __popcll(m);
-    eqs += __popcll(eqm);
   });
 }
 
-// The kept keys moved.  K parts take rows_k rows d of one (b, g) and 1024 kept
-// slots: a lane an element, so a load touches the few lines that 64 kept slots
-// span (eight elements a lane, for 16-byte stores, touched 64 of them); the
-// slots stay in registers over the rows.  V parts take rows of D elements, 16
-// bytes a lane, and the weights.
-constexpr int kMoveK = 4;           // slots of a thread
-constexpr int kMoveV = 64;          // slots of a V part
+// The kept keys moved.  A wave of a K part takes 512 kept slots, eight
+// consecutive ones a lane, over rows_k rows d: the stretch of the source row that
+// they span comes in 16-byte pieces, goes through LDS and leaves as 16-byte
+// pieces of the packed row (a 2-byte load and store per element moved the same
+// rows at 2.7 TB/s, bound by the address unit).  Stretches longer than a window
+// of 4096 slots take several passes over the rows.  V parts take slots_v rows of
+// D elements, 16 bytes a lane, and the weights.
+constexpr int kMoveJ = 512, kMoveWin = 4096, kMoveP = kMoveWin / 512;
+
+// eight elements of a row from slot i on (zeros past n)
+LOOM_DEV u32x4_t row_slots8(const uint16_t* row, int i, int n) {
+  u32x4_t v = u32x4_t{0u, 0u, 0u, 0u};
+  if (i + 8 <= n) {
+    __builtin_memcpy(&v, row + i, 16);
+  } else {
+#pragma unroll 1
+    for (int e = 0; e < 8 && i + e < n; ++e) {
+      const uint32_t h = (uint32_t)row[i + e] << (16 * (e & 1));
+      v[0] |= e / 2 == 0 ? h : 0u;
+      v[1] |= e / 2 == 1 ? h : 0u;
+      v[2] |= e / 2 == 2 ? h : 0u;
+      v[3] |= e / 2 == 3 ? h : 0u;
+    }
+  }
+  return v;
+}
+
+// One window of a wave's rows, NP pieces of 512 slots to a row, 8 / NP rows at a
+// time: eight 16-byte loads a lane are in flight whatever stretch the kept slots
+// span.
+template <int NP>
+LOOM_DEV void move_rows(const EvictParams& p, const uint16_t* src, uint16_t* dst, int rows,
+                        const int (&at)[8], int w0, int len, bool whole, int j, int n, int lane,
+                        uint16_t* win) {
+  constexpr int RB = kMoveP / NP;
+  u32x4_t piece[RB][NP];
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      if (r0 + rb < rows)
+#pragma unroll
+        for (int u = 0; u < NP; ++u)
+          if (u * 512 < len)
+            piece[rb][u] = row_slots8(src + (int64_t)(r0 + rb) * p.S, w0 + u * 512 + 8 * lane, p.S);
+  };
+  fetch(0);
+  for (int r0 = 0; r0 < rows; r0 += RB) {
+    lds_order();
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      if (r0 + rb < rows)
+#pragma unroll
+        for (int u = 0; u < NP; ++u)
+          if (u * 512 < len)
+            *reinterpret_cast<u32x4_t*>(win + (rb * NP + u) * 512 + 8 * lane) = piece[rb][u];
+    lds_order();
+    fetch(r0 + RB);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      if (r0 + rb < rows) {
+        const uint16_t* from = win + rb * NP * 512;
+        uint16_t* to = dst + (int64_t)(r0 + rb) * p.So;
+        uint16_t h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = from[whole ? at[e] - w0 : min(max(at[e] - w0, 0), len - 1)];
+        if (whole && j + 8 <= n) {
+          __builtin_memcpy(to, h, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (j + e < n && at[e] >= w0 && at[e] < w0 + len) to[e] = h[e];
+        }
+      }
+  }
+}
+
 __global__ void __launch_bounds__(256) cache_move_kernel(EvictParams p) {
+  __shared__ __attribute__((aligned(16))) uint16_t s_win[4][kMoveWin];
   const int bg = blockIdx.y, b = bg / p.G, tid = threadIdx.x;
   const int n = min(cache_len(p.lens, b, p.S), p.keep);
   const int* const idx = p.index + (int64_t)bg * p.keep;
   const int D = p.D;
   int x = blockIdx.x;
   if (x < p.nk) {
-    const int j0 = x % p.njk * (256 * kMoveK) + tid, d0 = x / p.njk * p.rows_k;
-    if (j0 - tid >= n) return;
-    int at[kMoveK];
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int jc = x % p.njk * kMoveJ;
+    const int d0 = (x / p.njk * 4 + wave) * p.rows_k, rows = min(D - d0, p.rows_k);
+    if (jc >= n || rows <= 0) return;
+    const int j = jc + 8 * lane;                // this lane's kept slots j .. j + 7
+    int at[8];
+    if (j + 8 <= n) {
+      __builtin_memcpy(at, idx + j, 32);
+    } else {
 #pragma unroll
-    for (int u = 0; u < kMoveK; ++u) at[u] = idx[min(j0 + 256 * u, n - 1)];
-    const int d1 = min(D, d0 + p.rows_k);
-    const uint16_t* src = p.k + ((int64_t)bg * D + d0) * p.S;
-    uint16_t* dst = p.k_out + ((int64_t)bg * D + d0) * p.So;
-#pragma unroll 4
-    for (int d = d0; d < d1; ++d) {
-      uint16_t e[kMoveK];
-#pragma unroll
-      for (int u = 0; u < kMoveK; ++u) e[u] = src[at[u]];
-#pragma unroll
-      for (int u = 0; u < kMoveK; ++u)
-        if (j0 + 256 * u < n) dst[j0 + 256 * u] = e[u];
-      src += p.S;
-      dst += p.So;
+      for (int e = 0; e < 8; ++e) at[e] = idx[min(j + e, n - 1)];
+    }
+    const int first = __builtin_amdgcn_readfirstlane(at[0]);
+    const int last = __builtin_amdgcn_readlane(at[7], 63);
+    const uint16_t* const src = p.k + ((int64_t)bg * D + d0) * p.S;
+    uint16_t* const dst = p.k_out + ((int64_t)bg * D + d0) * p.So + j;
+    // rows of whole 16-byte pieces are read at their boundaries
+    const int s0 = p.S % 8 == 0 ? first & ~7 : first;
+    for (int w0 = s0; w0 <= last; w0 += kMoveWin) {
+      const int len = min(kMoveWin, last + 1 - w0);
+      const bool whole = last - s0 < kMoveWin;
+      auto rows_of = [&](auto np) {
+        move_rows<decltype(np)::value>(p, src, dst, rows, at, w0, len, whole, j, n, lane,
+                                       s_win[wave]);
+      };
+      if (len <= 512) rows_of(std::integral_constant<int, 1>{});
+      else if (len <= 1024) rows_of(std::integral_constant<int, 2>{});
+      else if (len <= 2048) rows_of(std::integral_constant<int, 4>{});
+      else rows_of(std::integral_constant<int, 8>{});
     }
     return;
   }
   x -= p.nk;
-  const int j0 = x * kMoveV, jn = min(kMoveV, n - j0);
+  const int j0 = x * p.slots_v, jn = min(p.slots_v, n - j0);
   if (jn <= 0) return;
   if (tid < jn) p.w_out[(int64_t)bg * p.So + j0 + tid] = p.w[(int64_t)bg * p.S + idx[j0 + tid]];
-  const int cpr = D / 8;
+  // eight pieces of a thread at a time, 256 apart
+  const int cpr = D / 8, end = jn * cpr;
   const uint16_t* const src = p.v + (int64_t)bg * p.S * D;
   uint16_t* const dst = p.v_out + ((int64_t)bg * p.So + j0) * D;
-#pragma unroll 4
-  for (int e = tid; e < jn * cpr; e += 256) {
-    const int j = e / cpr, c = e - j * cpr;
-    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(src + (int64_t)idx[j0 + j] * D + c * 8);
-    *reinterpret_cast<u32x4_t*>(dst + (int64_t)j * D + c * 8) = v;
+  for (int e0 = tid; e0 < end; e0 += 8 * 256) {
+    int64_t from[8];
+    u32x4_t v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int e = min(e0 + 256 * u, end - 1), j = e / cpr;
+      from[u] = (int64_t)idx[j0 + j] * D + (e - j * cpr) * 8;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const u32x4_t*>(src + from[u]);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (e0 + 256 * u < end) *reinterpret_cast<u32x4_t*>(dst + (int64_t)(e0 + 256 * u) * 8) = v[u];
   }
 }
 
@@ -435,16 +612,21 @@ int loom_hip_cache_evict(const void* k, const void* v, const void* weights, cons
   if (loom_validate_only()) return loom_ok(err, errlen);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 sel((unsigned)(B * G)), selb(kSel);
-  if (S <= 4 * kSel) hipLaunchKernelGGL(cache_select_kernel<4>, sel, selb, 0, st, p);
-  else if (S <= 16 * kSel) hipLaunchKernelGGL(cache_select_kernel<16>, sel, selb, 0, st, p);
-  else hipLaunchKernelGGL(cache_select_kernel<0>, sel, selb, 0, st, p);
+  auto select = [&](auto kern) { hipLaunchKernelGGL(kern, sel, selb, 0, st, p); };
+  if (S <= 2 * kSel) select(cache_select_kernel<2>);
+  else if (S <= 4 * kSel) select(cache_select_kernel<4>);
+  else if (S <= 8 * kSel) select(cache_select_kernel<8>);
+  else if (S <= 16 * kSel) select(cache_select_kernel<16>);
+  else select(cache_select_kernel<0>);
   int rc = loom_check_launch(err, errlen, "cache_evict (select)");
   if (rc) return rc;
-  // rows of a K part: as many (up to 16) as leave about 1024 parts
-  p.njk = (int)cdiv64(keep, 256 * kMoveK);
-  p.rows_k = (int)std::max<int64_t>(2, std::min<int64_t>(16, B * G * p.njk * D / 1024));
-  p.nk = (int)(p.njk * cdiv64(D, p.rows_k));
-  const dim3 grid((unsigned)(p.nk + cdiv64(keep, kMoveV)), (unsigned)(B * G));
+  // rows of a K part's wave: as many (up to eight) as leave about 4096 waves
+  p.njk = (int)cdiv64(keep, kMoveJ);
+  p.rows_k = (int)std::max<int64_t>(2, std::min<int64_t>(8, B * G * p.njk * D / 4096));
+  p.nk = (int)(p.njk * cdiv64(D, 4 * p.rows_k));
+  // slots of a V part: eight 16-byte pieces a thread, fewer for about 1024 parts
+  p.slots_v = (int)std::max<int64_t>(8, std::min<int64_t>(16384 / D, std::min<int64_t>(256, cdiv64(B * G * keep, 1024))));
+  const dim3 grid((unsigned)(p.nk + cdiv64(keep, p.slots_v)), (unsigned)(B * G));
   hipLaunchKernelGGL(cache_move_kernel, grid, dim3(256), 0, st, p);
   return loom_check_launch(err, errlen, "cache_evict (move)");
 }
