@@ -20,6 +20,7 @@ import functools
 import json
 import math
 import os
+import threading
 
 import torch
 
@@ -829,44 +830,52 @@ def _cache_plan(func: str, sig: tuple, extra: tuple):
 
 
 def _cache_enter(func: str, tensors, extra=()):
-    """(plan, device index) of a call; raises what is wrong with a tensor."""
-    sig = []
+    """(plan, device index, device pointers) of a call; raises what is wrong
+    with a tensor (the form of all of them first, then their devices)."""
+    sig, ptrs, dev, odd = [], [], None, False
     for t in tensors:
         if t is None:
             sig.append(None)
+            ptrs.append(None)
         elif isinstance(t, torch.Tensor):
             sig.append((t.dtype, t.shape))
+            i = t.get_device()
+            if dev is None:
+                dev = i
+            if i != dev or i < 0 or not t.is_contiguous():
+                odd = True
+                ptrs.append(None)
+            else:
+                ptrs.append(t.data_ptr())
         else:
             raise TypeError(f"{func}: expected torch.Tensors, got {type(t).__name__}")
     plan = _cache_plan(func, tuple(sig), extra)
-    dev = None
-    for t, name in zip(tensors, plan[4]):
-        if t is None:
-            continue
-        i = t.get_device()
-        if not t.is_contiguous():
-            raise ValueError(f"{name}: must be contiguous")
-        if i < 0:
-            raise ValueError(f"{name}: must be on a ROCm device, got {t.device}")
-        if dev is None:
-            dev = i
-        elif i != dev:
-            raise ValueError(f"{name}: on {t.device}, the call's tensors are on cuda:{dev}")
-    return plan, dev
+    if odd:
+        there = [(t, n) for t, n in zip(tensors, plan[4]) if t is not None]
+        for t, name in there:
+            if not t.is_contiguous():
+                raise ValueError(f"{name}: must be contiguous")
+        for t, name in there:
+            _check_device(t, name, there[0][0].device)
+    return plan, dev, ptrs
+
+
+_cache_err = threading.local()
 
 
 def _cache_run(plan, dev, *args):
     """The entry point on the current stream of the tensors' device, which
     becomes the current one for the call where it is not."""
+    buf = getattr(_cache_err, "buf", None)
+    if buf is None:
+        buf = _cache_err.buf = ctypes.create_string_buffer(512)
     if dev == torch.cuda.current_device():
-        _run(plan, *args, _raw_stream(dev))
+        rc = plan[0](*args, _raw_stream(dev), buf, 512)
     else:
         with torch.cuda.device(dev):
-            _run(plan, *args, _raw_stream(dev))
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+            rc = plan[0](*args, _raw_stream(dev), buf, 512)
+    if rc != 0:
+        raise LoomHipError(plan[1], rc, buf.value.decode(errors="replace"))
 
 
 def cache_append(k, v, lens, new_k, new_v, lens_out=None, *, counts=None, weights=None):
@@ -877,11 +886,12 @@ def cache_append(k, v, lens, new_k, new_v, lens_out=None, *, counts=None, weight
     b takes its first ``counts[b]`` tokens (int32; all T by default); tokens past
     the capacity S are dropped.  With ``weights`` [B,G,S] (see cache_decode) the
     new keys' become zero.  ``lens_out`` must not be ``lens``."""
-    plan, dev = _cache_enter("cache_append", (k, v, weights, lens, new_k, new_v, counts, lens_out))
+    plan, dev, ptrs = _cache_enter("cache_append",
+                                   (k, v, weights, lens, new_k, new_v, counts, lens_out))
     if lens_out is None:
         lens_out = torch.empty_like(lens)
-    _cache_run(plan, dev, k.data_ptr(), v.data_ptr(), _ptr(weights), lens.data_ptr(),
-               new_k.data_ptr(), new_v.data_ptr(), _ptr(counts), lens_out.data_ptr(), *plan[2])
+        ptrs[7] = lens_out.data_ptr()
+    _cache_run(plan, dev, *ptrs, *plan[2])
     return lens_out
 
 
@@ -909,24 +919,23 @@ def cache_decode(k, v, q, lens, out=None, workspace=None, *, prefix_k=None, pref
     1/sqrt(D)."""
     if weights_out is None:
         weights_out = weights
-    plan, dev = _cache_enter("cache_decode", (prefix_k, prefix_v, k, v, q, lens, weights,
-                                              weights_out, out))
+    plan, dev, ptrs = _cache_enter("cache_decode", (prefix_k, prefix_v, k, v, q, lens, weights,
+                                                    weights_out, out))
     dims = plan[2]
     if scale is None:
         scale = 1.0 / math.sqrt(dims[3]) if dims[3] > 0 else 1.0
     if out is None:
         out = torch.empty_like(q)
+        ptrs[8] = out.data_ptr()
     need = cache_decode_workspace_bytes(*dims, weights is not None)
     if workspace is None:
         workspace = torch.empty(max(need, 4), dtype=torch.uint8, device=q.device)
         wp = workspace.data_ptr()
     else:
         wp = _check_workspace(workspace, need, q.device, "cache_decode")
-    # P == 0: an empty prefix is no prefix
-    pk, pv = (prefix_k.data_ptr(), prefix_v.data_ptr()) if dims[4] else (None, None)
-    _cache_run(plan, dev, pk, pv, k.data_ptr(), v.data_ptr(), q.data_ptr(), lens.data_ptr(),
-               _ptr(weights), _ptr(weights_out), out.data_ptr(), wp, workspace.numel(), *dims,
-               float(scale))
+    if dims[4] == 0:      # an empty prefix is no prefix
+        ptrs[0] = ptrs[1] = None
+    _cache_run(plan, dev, *ptrs, wp, workspace.numel(), *dims, float(scale))
     return out
 
 
@@ -943,25 +952,28 @@ def cache_evict(k, v, weights, lens, keep, *, recent=0, sinks=0, capacity=None, 
     slots they came from, -1 behind them.  ``capacity`` defaults to that of the
     outputs given, else S."""
     keep, recent, sinks = int(keep), int(recent), int(sinks)
-    plan, dev = _cache_enter("cache_evict", (k, v, weights, lens, k_out, v_out, weights_out,
-                                             lens_out, index),
-                             (keep, None if capacity is None else int(capacity)))
+    plan, dev, ptrs = _cache_enter("cache_evict", (k, v, weights, lens, k_out, v_out, weights_out,
+                                                   lens_out, index),
+                                   (keep, None if capacity is None else int(capacity)))
     B, G, D, S, So = plan[2][:5]
     if min(B, G, D, So, keep) <= 0:
         raise ValueError("cache_evict: extents and keep must be positive")
     if k_out is None:
         k_out = torch.empty((B, G, D, So), dtype=plan[3], device=k.device)
+        ptrs[4] = k_out.data_ptr()
     if v_out is None:
         v_out = torch.empty((B, G, So, D), dtype=plan[3], device=k.device)
+        ptrs[5] = v_out.data_ptr()
     if weights_out is None:
         weights_out = torch.empty((B, G, So), dtype=_fp32, device=k.device)
+        ptrs[6] = weights_out.data_ptr()
     if lens_out is None:
         lens_out = torch.empty_like(lens)
+        ptrs[7] = lens_out.data_ptr()
     if index is None:
         index = torch.empty((B, G, keep), dtype=_i32, device=k.device)
-    _cache_run(plan, dev, k.data_ptr(), v.data_ptr(), weights.data_ptr(), lens.data_ptr(),
-               k_out.data_ptr(), v_out.data_ptr(), weights_out.data_ptr(), lens_out.data_ptr(),
-               index.data_ptr(), B, G, D, S, So, keep, recent, sinks)
+        ptrs[8] = index.data_ptr()
+    _cache_run(plan, dev, *ptrs, B, G, D, S, So, keep, recent, sinks)
     return k_out, v_out, weights_out, lens_out, index
 
 
