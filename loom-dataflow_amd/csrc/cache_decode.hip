@@ -31,7 +31,7 @@ struct StepParams {
   float* w_out;
   uint16_t* out;
   int2* plan;       // [B]: a sequence's first chunk and their number
-  f32x4_t* ml;      // per partial row: base, sum of the rounded p, sum of p
+  f32x4_t* ml;      // per partial row: base, sum of p, sum of the rounded p
   float* o;         // per partial row: sum of p v, D values
   float* score;     // [B G, H, Sp] scores of the own keys, log2 domain
   int B, G, H, D, P, S, Sp;
@@ -162,11 +162,11 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
     const int64_t row = part_row(p, a, min(e / D, a.rows - 1));
     dma_load16(p.q + row * Dr + min(e % D, Dr - 8), lds_addr(sq) + j * 1024);
   }
-  if constexpr (KREG) {
+  issue(0, 0);
+  if constexpr (KREG) {     // (its wait covers V's copies, on their way before it)
     kload(0);
     kstore(0);
   }
-  issue(0, 0);
 
   u32x4_t qf[DSTEPS][QT];
   const float c2 = p.c2;
@@ -410,7 +410,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
     const int t0 = 16 * (QT * qw + qt);         // first row of the tile
     const int n = min(16, a.rows - t0);
     const int64_t row0 = a.out0 + t0;
-    if (r < n && g == 0) p.ml[row0 + r] = f32x4_t{m_run[qt], lacc[qt][0], lx[qt], 0.f};
+    if (r < n && g == 0) p.ml[row0 + r] = f32x4_t{m_run[qt], lx[qt], lacc[qt][0], 0.f};
     lds_order();
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -610,7 +610,7 @@ LOOM_DEV void join_parts(const StepParams& p, const Splits& sp, int u0, int NG, 
 #pragma unroll
   for (int u = 0; u < CH; ++u) {
     // a part without a key of finite score takes no part (its l is 0, not NaN)
-    if (u0 + u * NG >= sp.n || l[u][1] == 0.f) l[u][0] = -INFINITY;
+    if (u0 + u * NG >= sp.n || l[u][2] == 0.f) l[u][0] = -INFINITY;
     mc = fmaxf(mc, l[u][0]);
   }
   const float base = mc == -INFINITY ? 0.f : mc;
@@ -621,7 +621,7 @@ LOOM_DEV void join_parts(const StepParams& p, const Splits& sp, int u0, int NG, 
 #pragma unroll
   for (int u = 0; u < CH; ++u) {
     const float w = fast_exp2(l[u][0] - base);
-    den += w != 0.f ? w * l[u][1] : 0.f;
+    den += w != 0.f ? w * l[u][2] : 0.f;
     acc += w != 0.f ? o[u] * w : f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 }
@@ -680,16 +680,11 @@ LOOM_DEV void join_row(const StepParams& p, int bg, int h) {
 // heads; a group's first scores are on their way while M and l are found, four
 // threads to a head.
 LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
-  constexpr int HB = 256, HN = 8;
+  constexpr int HB = 256, HN = 8, UN = 8;
   __shared__ float s_M[HB], s_inv[HB];
   __shared__ f32x4_t s_w[kThreads];
   const int wkeys = p.wkeys, NG = 1024 / wkeys, LPG = wkeys / 4;
-  const int b = p.G == 1 ? bg : bg / p.G, g = bg - b * p.G;
-  const Splits sp0 = row_splits(p, b, g, 0);
-  const int len = seq_len(p, b);
-  if (j0 >= len) return;
   const int tid = threadIdx.x, grp = tid / LPG, lg = tid - grp * LPG;
-  f32x4_t sum = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const int j = min(j0 + 4 * lg, p.Sp - 4);    // Sp is a multiple of 64: whole pieces
   const float* const score = p.score + (int64_t)bg * p.H * p.Sp + j;
   f32x4_t sc[HN];
@@ -699,34 +694,51 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
       sc[x] = *reinterpret_cast<const f32x4_t*>(
           score + (int64_t)min(h0 + grp + NG * x, hn - 1) * p.Sp);
   };
+  load(0, min(p.H, HB));
+  const int b = p.G == 1 ? bg : bg / p.G, g = bg - b * p.G;
+  const Splits sp0 = row_splits(p, b, g, 0);
+  const int len = seq_len(p, b);
+  if (j0 >= len) return;
+  const float w_in = p.w[(int64_t)bg * p.S + min(j0 + tid, len - 1)];
+  f32x4_t sum = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // threads to a head: as many as leave 256 threads a head each
+  const int tph = p.H <= 32 ? 8 : p.H <= 64 ? 4 : 2, hpp = kThreads / tph;
   for (int hb = 0; hb < p.H; hb += HB) {
     const int hn = min(p.H, hb + HB);
-    load(hb, hn);
-    for (int h0 = hb; h0 < hn; h0 += 64) {
-      const int h = h0 + (tid >> 2), y = tid & 3;
+    if (hb > 0) load(hb, hn);
+#pragma unroll 1
+    for (int h0 = hb; h0 < hn; h0 += hpp) {
+      const int h = h0 + tid / tph, y = tid & (tph - 1);
       float M = -INFINITY, L = 0.f;
       if (h < hn) {
         Splits sp = sp0;
         sp.pre0 += h;
         sp.own0 += h;
-        for (int u0 = y; u0 < sp.n; u0 += 16) {
-          f32x4_t l[4];
+#pragma unroll 1
+        for (int u0 = y; u0 < sp.n; u0 += UN * tph) {
+          f32x2_t l[UN];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) l[x] = p.ml[split_at(sp, min(u0 + 4 * x, sp.n - 1))];
+          for (int x = 0; x < UN; ++x)
+            l[x] = *reinterpret_cast<const f32x2_t*>(
+                p.ml + split_at(sp, min(u0 + x * tph, sp.n - 1)));
+          float m = M;
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (u0 + 4 * x < sp.n && l[x][1] != 0.f) {
-              const float m = fmaxf(M, l[x][0]);
-              L = (M == -INFINITY ? 0.f : L * fast_exp2(M - m)) + l[x][2] * fast_exp2(l[x][0] - m);
-              M = m;
-            }
+          for (int x = 0; x < UN; ++x) {
+            // a part without a key of finite score takes no part (its sum is 0)
+            if (u0 + x * tph >= sp.n || l[x][1] == 0.f) l[x] = f32x2_t{-INFINITY, 0.f};
+            m = fmaxf(m, l[x][0]);
+          }
+          const float base = m == -INFINITY ? 0.f : m;
+          L *= fast_exp2(M - base);
+#pragma unroll
+          for (int x = 0; x < UN; ++x) L += l[x][1] * fast_exp2(l[x][0] - base);
+          M = m;
         }
       }
-#pragma unroll
-      for (int x = 1; x < 4; x <<= 1) {
+      for (int x = 1; x < tph; x <<= 1) {
         const float M2 = __shfl_xor(M, x), L2 = __shfl_xor(L, x);
-        const float m = fmaxf(M, M2);
-        L = (L != 0.f ? L * fast_exp2(M - m) : 0.f) + (L2 != 0.f ? L2 * fast_exp2(M2 - m) : 0.f);
+        const float m = fmaxf(M, M2), base = m == -INFINITY ? 0.f : m;
+        L = L * fast_exp2(M - base) + L2 * fast_exp2(M2 - base);
         M = m;
       }
       if (y == 0 && h < hn) {
@@ -735,6 +747,7 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
       }
     }
     __syncthreads();
+#pragma unroll 1
     for (int h0 = hb; h0 < hn; h0 += NG * HN) {
       if (h0 > hb) load(h0, hn);
 #pragma unroll
@@ -755,8 +768,7 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
     const float* f = reinterpret_cast<const float*>(s_w) + tid;
     float w = 0.f;
     for (int x = 0; x < NG; ++x) w += f[x * wkeys];
-    const int64_t at = (int64_t)bg * p.S + j0 + tid;
-    p.w_out[at] = p.w[at] + w;
+    p.w_out[(int64_t)bg * p.S + j0 + tid] = w_in + w;
   }
 }
 
