@@ -21,6 +21,15 @@ namespace {
 
 LOOM_DEV int cache_len(const int* lens, int b, int S) { return min(max(lens[b], 0), S); }
 
+// 16 bytes to any element of a row, non-temporal (as store_stream: the written
+// rows, which nothing here reads back, displace no rows still to be read and are
+// not left to the flush at the kernel's end: evictions of B8 G8 D64 S16383 93 ->
+// 79 us, B32 S8192 33 -> 29; appended prompts 39.4 -> 36.7)
+typedef u32x4_t any16_t __attribute__((aligned(2)));
+LOOM_DEV void store_any16(uint16_t* to, const u32x4_t& v) {
+  __builtin_nontemporal_store(v, reinterpret_cast<any16_t*>(to));
+}
+
 struct AppendParams {
   uint16_t* k;
   uint16_t* v;
@@ -83,7 +92,7 @@ __global__ void __launch_bounds__(256) cache_append_tile_kernel(AppendParams p) 
     const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p.nk + src);
     const u32x4_t y = *reinterpret_cast<const u32x4_t*>(p.nv + src);
     *reinterpret_cast<u32x4_t*>(smem + k * (DP * 2) + ((ch ^ tok_swz(k)) * 16)) = x;
-    *reinterpret_cast<u32x4_t*>(vo + (int64_t)k * D + ch * 8) = y;
+    store_stream(reinterpret_cast<u32x4_t*>(vo + (int64_t)k * D + ch * 8), y);
   }
   if (p.w && tid < kTok && k0 + tid >= n && k0 + tid < end) p.w[(int64_t)bg * S + k0 + tid] = 0.f;
   __syncthreads();
@@ -103,7 +112,7 @@ __global__ void __launch_bounds__(256) cache_append_tile_kernel(AppendParams p) 
     uint16_t* const to = p.k + ko + (int64_t)d * S + at;
     const u32x4_t v = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
     if (at >= n && at + 8 <= end) {
-      __builtin_memcpy(to, &v, 16);     // 16-byte aligned when S is a multiple of 8
+      store_any16(to, v);               // 16-byte aligned when S is a multiple of 8
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -410,7 +419,9 @@ LOOM_DEV void move_rows(const EvictParams& p, const uint16_t* src, uint16_t* dst
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[e] = from[whole ? at[e] - w0 : min(max(at[e] - w0, 0), len - 1)];
         if (whole && j + 8 <= n) {
-          __builtin_memcpy(to, h, 16);
+          u32x4_t v;
+          __builtin_memcpy(&v, h, 16);
+          store_any16(to, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -480,7 +491,8 @@ __global__ void __launch_bounds__(256) cache_move_kernel(EvictParams p) {
     for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const u32x4_t*>(src + from[u]);
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (e0 + 256 * u < end) *reinterpret_cast<u32x4_t*>(dst + (int64_t)(e0 + 256 * u) * 8) = v[u];
+      if (e0 + 256 * u < end)
+        store_stream(reinterpret_cast<u32x4_t*>(dst + (int64_t)(e0 + 256 * u) * 8), v[u]);
   }
 }
 

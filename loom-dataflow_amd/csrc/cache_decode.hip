@@ -14,6 +14,7 @@
 #include "common.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -39,6 +40,7 @@ struct StepParams {
   int chunks;       // chunks that the whole batch aims at
   int rtp, ntp, nsp, tile_p;   // the prefix: rows of a tile, tiles per head, splits, keys of one
   int nprefix;      // workgroups of the prefix
+  int once;         // own keys are read by non-temporal copies
   int wkeys;        // keys of a workgroup that gathers weights: 128 or 256
   float c2;         // scale * log2(e)
 };
@@ -48,6 +50,20 @@ LOOM_DEV int seq_len(const StepParams& p, int b) { return min(max(p.lens[b], 0),
 // ---------------------------------------------------------------------------
 // One part: up to RT query rows against the keys [s0, s1) of one K, V.
 // ---------------------------------------------------------------------------
+// dma_load16 of data that is read once: non-temporal, so the stream displaces
+// nothing that is read again.  Taken for the own keys of caches larger than the
+// 256 MB last-level cache (B48 G8 S4096 under a prefix 124 -> 113 us a step, B8 G8
+// S8192 43.5 -> 38.7); smaller ones may still lie there from the last step (B16
+// G8 S2048 29.3 against 31.6), and a prefix is read by many sequences
+LOOM_DEV void dma_once16(const void* g, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, off nt"
+      :
+      : "v"(g), "s"(lds)
+      : "memory", "m0");
+}
 LOOM_DEV int ck_swz(int d) { return (2 * (d & 3)) ^ (2 * ((d >> 3) & 1)); }
 template <int D>
 LOOM_DEV int cv_swz(int k) { return D >= 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3); }
@@ -58,6 +74,7 @@ struct Part {
   int ld;               // keys of a K row
   int s0, s1;           // this part's keys, s0 a multiple of 64
   int rows;             // query rows
+  bool once;            // no other workgroup reads these keys
   int i0;               // first row: of the (b, g)'s heads, or of head g's B H rows
   int g;                // the KV head of a prefix part, -1: rows are consecutive
   int64_t out0;         // partial row of row 0; the others follow
@@ -94,6 +111,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
   const uint16_t* __restrict__ kg = a.k;
   const uint16_t* __restrict__ vg = a.v;
   const int nblk = (s1 - s0 + kKeys - 1) / kKeys;
+  const bool once = __builtin_amdgcn_readfirstlane((int)a.once) != 0;
   const bool active = 16 * QT * qw < a.rows;    // this wave has rows
   // score stores of a block that every active wave issues at least (those of
   // its first row tile): younger than the next block's copies, so the wait for
@@ -107,7 +125,12 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
   // clamped (their keys are masked), rows d >= Dr come from zeros; V rows past
   // s1 repeat the last one, whose weight there is zero (slots behind a length
   // may hold NaN, and 0 NaN is NaN)
-  auto issue = [&](int s, int blk) {
+  auto copies = [&](int s, int blk, auto once) {
+    auto copy = [](const void* from, uint32_t to) {
+      to = __builtin_amdgcn_readfirstlane(to);
+      if constexpr (decltype(once)::value) dma_once16(from, to);
+      else dma_load16(from, to);
+    };
     const int kv0 = s0 + blk * kKeys;
     const uint32_t lk = lds_addr(stK(s)), lv = lds_addr(stV(s));
     if constexpr (!KREG) {
@@ -117,9 +140,9 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
         const int d = j * 8 + lane / 8;
         const int key = min(kv0 + ((lane % 8) ^ ck_swz(d)) * 8, ld - 8);
         if (j * 8 < Dr)                                 // wave-uniform
-          dma_load16(kg + (int64_t)d * ld + key, lk + j * 1024);
+          copy(kg + (int64_t)d * ld + key, lk + j * 1024);
         else
-          dma_load16(loom_zero_kb + lane * 4, lk + j * 1024);
+          dma_load16(loom_zero_kb + lane * 4, __builtin_amdgcn_readfirstlane(lk + j * 1024));
       }
     }
 #pragma unroll
@@ -128,8 +151,12 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
       const int kr = j * V_ROWS_PER_I + lane / (D / 8);
       const int c = min((lane % (D / 8)) ^ cv_swz<D>(kr), Dr / 8 - 1);
       const int key = min(kv0 + kr, s1 - 1);
-      dma_load16(vg + (int64_t)key * Dr + c * 8, lv + j * 1024);
+      copy(vg + (int64_t)key * Dr + c * 8, lv + j * 1024);
     }
+  };
+  auto issue = [&](int s, int blk) {
+    if (once) copies(s, blk, std::true_type{});
+    else copies(s, blk, std::false_type{});
   };
   // ---- KREG (ld not a multiple of 8): K pieces through registers
   const rsrc_t krs = make_rsrc(kg, KREG ? (uint32_t)(Dr * ld * 2) : 0u);
@@ -420,8 +447,8 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
       float* to = p.o + (row0 + lr0) * Dr + c;
 #pragma unroll 1
       for (int lr = lr0; lr < n; lr += 64 / PPR, to += 64 / PPR * Dr)
-        *reinterpret_cast<f32x4_t*>(to) =
-            *reinterpret_cast<const f32x4_t*>(mo + lr * OROW + c);
+        store_stream(reinterpret_cast<f32x4_t*>(to),
+                     *reinterpret_cast<const f32x4_t*>(mo + lr * OROW + c));
     }
     lds_order();
   }
@@ -535,6 +562,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(
     a.i0 = rt * tile;
     a.rows = min(tile, rows - a.i0);
     a.g = g;
+    a.once = false;
     a.out0 = ((int64_t)s * p.G + g) * rows + a.i0;
     a.score = nullptr;
   } else {                  // a chunk of a sequence's own keys
@@ -551,6 +579,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) cache_split_kernel(
     a.s0 = c.i * c.size;
     a.s1 = min(c.n, a.s0 + c.size);
     a.g = -1;
+    a.once = p.once != 0;
     a.rows = min(128, p.H - ht * 128);
     a.i0 = (int)(bg * p.H) + ht * 128;
     a.out0 = (int64_t)p.nsp * p.B * p.G * p.H + ((int64_t)(x / per) * p.G + g) * p.H + ht * 128;
@@ -908,6 +937,7 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   p.nsp = s.nsp;
   p.tile_p = s.tile_p;
   p.nprefix = s.nprefix;
+  p.once = s.nht == 1 && 4 * B * G * S * D > (int64_t)256 << 20;
   // 256 keys spread the heads' statistics over more of them (B32 H32 n6144 33.6
   // against 35.3 us for the step); 128 give few workgroups more of the CUs (B1
   // S4096 12.9 against 13.3, B16 H71 n1024 17.9 against 18.9)
