@@ -40,6 +40,7 @@ struct StepParams {
   int chunks;       // chunks that the whole batch aims at
   int rtp, ntp, nsp, tile_p;   // the prefix: rows of a tile, tiles per head, splits, keys of one
   int nprefix;      // workgroups of the prefix
+  int njoin, flat;  // workgroups that join rows; several rows to each
   int once;         // own keys are read by non-temporal copies
   int wkeys;        // keys of a workgroup that gathers weights: 128 or 256
   float c2;         // scale * log2(e)
@@ -655,14 +656,37 @@ LOOM_DEV void join_parts(const StepParams& p, const Splits& sp, int u0, int NG, 
   }
 }
 
-// One workgroup per row, its threads in groups of D / 4 (four d each), group y
-// taking parts y, y + NG, ...; the groups' (max, sum, row) meet in LDS.
+// out of a row's (max, sum, row); a row without a finite score is zero
 template <bool F16>
-LOOM_DEV void join_row(const StepParams& p, int bg, int h) {
+LOOM_DEV void store_row(const StepParams& p, int64_t row, int d, float den, const f32x4_t& acc) {
+  const float inv = den != 0.f ? 1.f / den : 0.f;
+  *reinterpret_cast<u32x2_t*>(p.out + row * p.D + d) =
+      u32x2_t{pack2<F16>(acc[0] * inv, acc[1] * inv), pack2<F16>(acc[2] * inv, acc[3] * inv)};
+}
+
+// Many rows: D / 4 threads to a row, each over all of its parts.
+template <bool F16>
+LOOM_DEV void join_rows(const StepParams& p, int x) {
+  const int TPR = p.D / 4, RPW = kThreads / TPR;
+  const int sub = (int)threadIdx.x / TPR, row = x * RPW + sub;
+  if (sub >= RPW || row >= p.B * p.G * p.H) return;
+  const int d = ((int)threadIdx.x - sub * TPR) * 4;
+  const int bg = row / p.H, h = row - bg * p.H, b = p.G == 1 ? bg : bg / p.G, g = bg - b * p.G;
+  const Splits sp = row_splits(p, b, g, h);
+  float M = -INFINITY, den = 0.f;
+  f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int u0 = 0; u0 < sp.n; u0 += 4) join_parts<4>(p, sp, u0, 1, d, M, den, acc);
+  store_row<F16>(p, row, d, den, acc);
+}
+
+// Few rows: one workgroup per row, its threads in groups of D / 4 (four d each),
+// group y taking parts y, y + NG, ...; the groups' (max, sum, row) meet in LDS.
+template <bool F16>
+LOOM_DEV void join_row(const StepParams& p, int row) {
   __shared__ f32x4_t s_acc[256];
   __shared__ float s_m[kJoinMax], s_den[kJoinMax];
   const int D = p.D;
-  const int b = p.G == 1 ? bg : bg / p.G, g = bg - b * p.G;
+  const int bg = row / p.H, h = row - bg * p.H, b = p.G == 1 ? bg : bg / p.G, g = bg - b * p.G;
   const Splits sp = row_splits(p, b, g, h);
   const int ns = sp.n;
   const int TPR = D / 4, NG = min(256 / TPR, kJoinMax);
@@ -698,9 +722,7 @@ LOOM_DEV void join_row(const StepParams& p, int bg, int h) {
     dt += s_den[y] * w;
     at += s_acc[y * TPR + (int)threadIdx.x] * w;
   }
-  const float inv = dt != 0.f ? 1.f / dt : 0.f;
-  *reinterpret_cast<u32x2_t*>(p.out + ((int64_t)bg * p.H + h) * D + d) =
-      u32x2_t{pack2<F16>(at[0] * inv, at[1] * inv), pack2<F16>(at[2] * inv, at[3] * inv)};
+  store_row<F16>(p, row, d, dt, at);
 }
 
 // The keys j0 .. j0 + p.wkeys - 1 of one (b, g): weights_out = weights + sum over its heads of
@@ -801,17 +823,19 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
   }
 }
 
-// A row per workgroup (blockIdx.x < H), then the weights' parts of the (b, g).
+// p.njoin workgroups of rows, then the weights' parts of every (b, g).
 template <bool F16, bool WT>
 __global__ void __launch_bounds__(256) cache_join_kernel(StepParams p) {
-  const int x = blockIdx.x, bg = blockIdx.y;
+  const int x = blockIdx.x;
   if constexpr (WT) {
-    if (x >= p.H) {
-      add_weights(p, bg, (x - p.H) * p.wkeys);
+    if (x >= p.njoin) {
+      const int nw = (p.S + p.wkeys - 1) / p.wkeys, bg = (x - p.njoin) / nw;
+      add_weights(p, bg, (x - p.njoin - bg * nw) * p.wkeys);
       return;
     }
   }
-  join_row<F16>(p, bg, x);
+  if (p.flat) join_rows<F16>(p, x);
+  else join_row<F16>(p, x);
 }
 
 // The launch's shape, from the extents alone.
@@ -879,8 +903,9 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
                      "cache_decode: head_dim %lld not built (a multiple of 8 up to 256)",
                      (long long)D);
   if (S > (1 << 29) || P > (1 << 29) || !loom_prod_le({B, G}, 65535) ||
-      !loom_prod_le({B, G, H}, 1 << 24) || !loom_prod_le({B, G, cdiv64(S, 256)}, 1 << 24) || !loom_prod_le({B, G, S, D}, (int64_t)1 << 50) ||
-      !loom_prod_le({G, P, D}, (int64_t)1 << 50))
+      !loom_prod_le({B, G, H}, 1 << 23) || !loom_prod_le({B, G, S, D}, (int64_t)1 << 50) ||
+      !loom_prod_le({G, P, D}, (int64_t)1 << 50) ||
+      (weights && !loom_prod_le({B, G, cdiv64(S, 128)}, 1 << 23)))
     return loom_fail(err, errlen, LOOM_EINVAL, "cache_decode: problem too large");
   // a capacity or prefix that is not a multiple of 8 takes buffer descriptors,
   // which address one (b, g)'s keys in 32 bits
@@ -937,6 +962,12 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   p.nsp = s.nsp;
   p.tile_p = s.tile_p;
   p.nprefix = s.nprefix;
+  // Several rows to a workgroup where rows are many or their parts few: B60 G8 H16
+  // P1584 39.0 -> 28.1 us a step, B30 G8 H12 P976 with weights 25.0 -> 21.0; but
+  // 1024 rows of 32 parts 24.5 -> 29.7
+  const int64_t parts = s.nsp + cdiv64(s.chunks, B);
+  p.flat = B * G * H > 2048 || (B * G * H >= 1024 && parts <= 16);
+  p.njoin = (int)(p.flat ? cdiv64(B * G * H, kThreads / (D / 4)) : B * G * H);
   p.once = s.nht == 1 && 4 * B * G * S * D > (int64_t)256 << 20;
   // 256 keys spread the heads' statistics over more of them (B32 H32 n6144 33.6
   // against 35.3 us for the step); 128 give few workgroups more of the CUs (B1
@@ -959,12 +990,11 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   }
   int rc = loom_check_launch(err, errlen, "cache_decode (split)");
   if (rc) return rc;
-  const unsigned rows = (unsigned)H, bgs = (unsigned)(B * G);
   if (weights)
     hipLaunchKernelGGL((cache_join_kernel<F16, true>),
-                       dim3(rows + (unsigned)cdiv64(S, p.wkeys), bgs), block, 0, st, p);
+                       dim3((unsigned)(p.njoin + B * G * cdiv64(S, p.wkeys))), block, 0, st, p);
   else
-    hipLaunchKernelGGL((cache_join_kernel<F16, false>), dim3(rows, bgs), block, 0, st, p);
+    hipLaunchKernelGGL((cache_join_kernel<F16, false>), dim3((unsigned)p.njoin), block, 0, st, p);
   return loom_check_launch(err, errlen, "cache_decode (join)");
 }
 
@@ -977,7 +1007,7 @@ size_t loom_hip_cache_decode_workspace_bytes(int64_t B, int64_t G, int64_t H, in
   if (B <= 0 || G <= 0 || H <= 0 || D <= 0 || P < 0 || S <= 0) return 0;
   // what does not fit is reported as no size at all fits
   if (P > (1 << 29) || S > (1 << 29) || D > (1 << 20) || !loom_prod_le({B, G}, 65535) ||
-      !loom_prod_le({B, G, H}, 1 << 24))
+      !loom_prod_le({B, G, H}, 1 << 23))
     return SIZE_MAX;
   const Shape s = shape_of(B, G, H, D, P, S);
   return align256((size_t)B * 8) + align256((size_t)s.rows * 16) +
