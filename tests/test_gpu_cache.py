@@ -149,6 +149,28 @@ def test_decode(lh, shape, e):
         check(lh, "step", *shape, TYPES[e], weights)
 
 
+@pytest.mark.parametrize("e", TYPES)
+def test_decode_shapes_of_a_launch(lh, e):
+    """The larger ways a step is laid out: prefix tiles of 128 rows, own tiles of
+    64 and 128, several rows to a joining workgroup, weights in parts of 256
+    keys, heads past 256, more than 256 sequences."""
+    t = TYPES[e]
+    check(lh, "128-row tiles", 33, 1, 31, 64, 16500, 72, [2 * b for b in range(33)], t)
+    check(lh, "128-row tiles, odd", 18, 4, 29, 64, 4099, 40, [2 * b for b in range(18)], t,
+          weights=False)
+    check(lh, "joined rows", 70, 4, 8, 80, 33, 40, [(7 * b) % 41 for b in range(70)], t)
+    check(lh, "joined rows, one part", 129, 2, 8, 128, 0, 64, [(7 * b) % 65 for b in range(129)], t)
+    check(lh, "parts of 256", 16, 2, 33, 64, 5, 2100, [131 * b for b in range(16)], t)
+    check(lh, "wide heads", 2, 1, 300, 64, 70, 520, [519, 64], t)
+    check(lh, "heads of 64", 5, 1, 64, 128, 130, 1001, [0, 250, 500, 750, 1001], t)
+    check(lh, "heads of 71", 3, 1, 71, 128, 131, 501, [0, 250, 501], t)
+
+
+def test_decode_caches_past_the_last_level_cache(lh):
+    check(lh, "large caches", 2, 1, 8, 128, 100, 300000, [300000, 123457], torch.bfloat16)
+    check(lh, "large caches, odd", 2, 1, 8, 128, 0, 300001, [300001, 64], torch.float16)
+
+
 @pytest.mark.parametrize("S", [2047, 2044, 2046])
 @pytest.mark.parametrize("P", [0, 515, 1021])
 @pytest.mark.parametrize("D", [64, 128, 256])
@@ -334,6 +356,10 @@ def evict_check(lh, B, G, D, S, So, lens, keep, recent, sinks, e=torch.bfloat16,
     (1, 1, 128, 9001, 9000, [9001], 9000, 1, 1), (2, 1, 64, 5000, 3001, [4999, 5000], 2999, 7, 3),
     (4, 1, 8, 77, 30, [-3, 1000, 31, 30], 30, 3, 3), (1, 1, 64, 70000, 30000, [69999], 30000, 9, 0),
     (65, 2, 16, 150, 60, [(11 * i) % 151 for i in range(65)], 50, 5, 1),
+    # kept slots far apart (several windows of a row), and ever closer
+    (1, 1, 64, 70000, 704, [69999], 600, 9, 0), (1, 1, 40, 70001, 701, [70001], 600, 9, 0),
+    (1, 2, 64, 16384, 2049, [16383], 2048, 0, 0), (1, 2, 64, 16377, 3000, [16377], 2999, 0, 0),
+    (1, 1, 72, 8192, 6000, [8192], 5555, 100, 4),
 ], ids=lambda c: "x".join(map(str, c[:5])) + f"-{c[6]}")
 def test_evict(lh, case):
     for e in TYPES.values():
@@ -561,6 +587,50 @@ def test_graph_replays_follow_the_lengths(lh):
         torch.cuda.synchronize()
         for o, r in zip(outs, ref):
             assert torch.equal(o, r), lens
+
+
+def test_threads_on_their_own_streams(lh):
+    """Four host threads, each with its stream, caches and sizes: the results of
+    calls made alone, bit for bit."""
+    import threading
+    ts = [make(2 + i, 2, 8, 64 + 64 * (i % 2), 100 * i, 256 + 64 * i,
+               [(50 * b + 7 * i) % 257 for b in range(2 + i)], torch.bfloat16, seed=50 + i)
+          for i in range(4)]
+    d = [{n: None if x is None else x.cuda() for n, x in t.items()} for t in ts]
+
+    def work(x):
+        w = x["weights"].clone()
+        o = lh.cache_decode(x["k"], x["v"], x["q"], x["lens"], prefix_k=x["prefix_k"],
+                            prefix_v=x["prefix_v"], weights=w)
+        r = lh.cache_evict(x["k"], x["v"], w, x["lens"], 40, recent=4, sinks=1,
+                           k_out=torch.zeros_like(x["k"]), v_out=torch.zeros_like(x["v"]),
+                           weights_out=torch.zeros_like(w))
+        return (o, w, *r)
+
+    want = [work(x) for x in d]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in d], []
+
+    def run(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(8):
+                    got[i].append(work(d[i]))
+            s.synchronize()
+        except Exception as e:      # noqa: BLE001  (reported by the test)
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert not errors, errors
+    for i in range(4):
+        for r in got[i]:
+            for a, b in zip(r, want[i]):
+                assert torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float()))
 
 
 def test_two_streams_at_once(lh):
