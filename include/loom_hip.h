@@ -317,7 +317,9 @@ size_t loom_hip_cache_decode_workspace_bytes(int64_t B, int64_t G, int64_t H, in
  * they may be the same tensor, else must not overlap):
  *   weights_out[b,g,j] = weights[b,g,j] + sum over h of row (b,g,h)'s softmax
  * weight of own key j, for j < n; other elements are left as they are.
- * S (P) not a multiple of 8 needs D*S (D*P) < 2^30. */
+ * S (P) not a multiple of 8 needs D*S (D*P) < 2^30; B*G*H at most 2^23, with
+ * weights B*G*ceil(S/128) too.  Sums run in an order that the extents and lengths
+ * fix: equal calls give equal bits. */
 int loom_hip_cache_decode(const void* prefix_k, const void* prefix_v, const void* k, const void* v,
                           const void* q, const void* lens, const void* weights, void* weights_out,
                           void* out, void* workspace, size_t workspace_bytes, int64_t B, int64_t G,

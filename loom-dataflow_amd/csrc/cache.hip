@@ -42,7 +42,9 @@ struct AppendParams {
   int B, G, D, S, T;
 };
 
-// Few tokens: a thread per element of one (token, sequence).
+// Few tokens: a thread per element of one (token, sequence).  A token's K
+// elements lie S apart, a line of the cache each: latency bounds it (B32 G1 D128:
+// 2.4 us).
 __global__ void __launch_bounds__(256) cache_append_kernel(AppendParams p) {
   const int t = blockIdx.x, b = blockIdx.y;
   const int n = cache_len(p.lens, b, p.S);
@@ -65,7 +67,9 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendParams p) {
 // to LDS as they are, DP elements apart, and come back transposed: a lane of
 // ds_read_b64_tr_b16 gets four tokens of one d.  Each 32-lane pass reads 32
 // bytes of rows k..k+3 and k+8..k+11; rows are whole 256-byte bank windows, so
-// the XOR gives the eight rows distinct pairs of 16-byte chunks.
+// the XOR gives the eight rows distinct pairs of 16-byte chunks.  Bound by memory:
+// B8 G8 D128, prompts of 1024 to 4096 tokens (180 MB read and written) 38 us, 4.7
+// TB/s.
 constexpr int kTok = 64;
 LOOM_DEV int tok_swz(int k) { return 2 * ((k & 3) | ((k >> 1) & 4)); }
 
@@ -189,6 +193,7 @@ LOOM_DEV uint32_t waves_before(const uint32_t* v, int lane, int wave) {
 // each run four of its waves).  With KPT > 0 the keys stay in registers (KPT a
 // lane, slots 64 apart; in LDS, with rolled loops, 23 us against 15 at 16 a
 // lane), else (KPT 0, longer caches) every pass reads the weights again.
+// 4096 weights 6.0 us, 32 x 8192 8.6 us, 64 x 16383 11.8 us.
 template <int KPT>
 __global__ void __launch_bounds__(kSel) cache_select_kernel(EvictParams p) {
   __shared__ __attribute__((aligned(16))) uint32_t hist[kCopyStep * kCopies], s_list[kList];
@@ -549,7 +554,10 @@ int loom_hip_cache_append(void* k, void* v, void* weights, const void* lens, con
   p.T = (int)T;
   if (loom_validate_only()) return loom_ok(err, errlen);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (T < 16) {
+  // a thread per element up to three tokens (B32 G8 D128, one token: 3.6 us
+  // against 4.6 in tiles; two 4.0 and 4.6), tiles above (four 4.8 and 4.6, 16
+  // 7.7 and 6.8, 64 16.5 and 8.5)
+  if (T < 4) {
     hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)T, (unsigned)B), dim3(256), 0, st, p);
   } else {
     // slots that a sequence's tokens reach from any length: T and the part of a

@@ -11,6 +11,23 @@
 //     out = sum_j p_j v_j;
 //     weights_out[b, g, j] = weights[b, g, j] + sum_h p_j for the own keys.
 //   A row without keys is zero.
+//
+// gfx950 mapping.  The own keys are bound by streaming K and V once (H heads
+// give H operations a byte); the prefix, whose K and V all B H rows of a head
+// share, by the matrix cores or, in short calls, by latency.  Two launches:
+//   - cache_split_kernel: every workgroup takes a *part*, some query rows
+//     against a range of keys of one K, V, and leaves (base, sum, sum of p v):
+//     parts of the prefix (tiles of 32, 64 or 128 of the B H rows, key splits)
+//     and chunks of each sequence's own keys.  They run side by side, so that the
+//     prefix's arithmetic hides behind the caches' stream (B48 G8 H8 P16384 S4096:
+//     prefix alone 51 us, own keys alone 98, together 113);
+//   - cache_join_kernel: joins a row's parts and, from the scores that the chunks
+//     left in the workspace, adds the weights.  Scores are kept in fp32: weights
+//     are sums of many steps.  Rereading K instead would cost as many bytes at 32
+//     heads, more below.
+// Rounding: scores, bases and sums are fp32; p is rounded to 16 bits for its
+// product with v, and out is divided by the sum of the rounded p, so that one
+// heavy key's rounding cancels.  The weights use the unrounded p and their own sum.
 #include "common.h"
 
 #include <cmath>
@@ -91,6 +108,16 @@ LOOM_DEV int64_t part_row(const StepParams& p, const Part& a, int lr) {
   return ((int64_t)b * p.G + a.g) * p.H + (i - b * p.H);
 }
 
+// Four waves, 64 keys a stage, two stages (64 KB up to D 128, so two workgroups
+// fit a CU and one's arithmetic covers the other's waits).  As in
+// decode.hip: K [d][key] and V [key][d] lie in LDS as the tensors have them,
+// copied by LDS DMA (K through registers where its rows start off 16-byte
+// boundaries, KREG), and reach the MFMAs by transposed reads,
+//   S^T[key, row] = K^T . Q^T,   O^T[d, row] += V^T . P^T.
+// KG 2: two waves share 16 QT rows, each taking one 32-key half of every stage,
+// and merge at the end: 32 rows, for the heads of one KV head.  KG 1: a wave takes
+// 16 QT rows of its own: 64 or 128 rows that share the stages.  WT: the scores
+// of own keys are stored and the unrounded p summed.
 template <int D, bool F16, bool WT, int QT, int KG, bool KREG>
 LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
   constexpr int W = kThreads / 64;

@@ -784,9 +784,10 @@ _CACHE_SPECS = {
 
 @functools.lru_cache(maxsize=1024)
 def _cache_plan(func: str, sig: tuple, extra: tuple):
-    """(entry point, its name, extents, 16-bit type) of a call's signature, which
-    holds (dtype, shape) of every tensor argument (None where it is left out);
-    kept by value for the last 1024 signatures.  Raises what is wrong with it."""
+    """(entry point, its name, extents, 16-bit type, arguments' names, workspace
+    bytes) of a call's signature, which holds (dtype, shape) of every tensor
+    argument (None where it is left out); kept by value for the last 1024
+    signatures.  Raises what is wrong with it."""
     at = {"cache_append": (0, 4), "cache_decode": (2, 4), "cache_evict": (0, 0)}[func]
     names = [a[0].rstrip("?") for a in _CACHE_SPECS[func](*(0,) * (5 if func == "cache_append"
                                                                     else 6))]
@@ -826,7 +827,8 @@ def _cache_plan(func: str, sig: tuple, extra: tuple):
         if tuple(s[1]) != shape:
             raise ValueError(f"{name.rstrip('?')}: expected shape {shape}, got {tuple(s[1])}")
     name = "loom_hip_" + func + ("_f16" if e == _f16 and func == "cache_decode" else "")
-    return getattr(_lib, name), name, dims, e, names
+    need = cache_decode_workspace_bytes(*dims, sig[6] is not None) if func == "cache_decode" else 0
+    return getattr(_lib, name), name, dims, e, names, need
 
 
 def _cache_enter(func: str, tensors, extra=()):
@@ -861,6 +863,7 @@ def _cache_enter(func: str, tensors, extra=()):
 
 
 _cache_err = threading.local()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _cache_run(plan, dev, *args):
@@ -869,7 +872,7 @@ def _cache_run(plan, dev, *args):
     buf = getattr(_cache_err, "buf", None)
     if buf is None:
         buf = _cache_err.buf = ctypes.create_string_buffer(512)
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = plan[0](*args, _raw_stream(dev), buf, 512)
     else:
         with torch.cuda.device(dev):
@@ -895,7 +898,6 @@ def cache_append(k, v, lens, new_k, new_v, lens_out=None, *, counts=None, weight
     return lens_out
 
 
-@functools.lru_cache(maxsize=1024)
 def cache_decode_workspace_bytes(B, G, H, D, P, S, weights=False) -> int:
     return int(_lib.loom_hip_cache_decode_workspace_bytes(B, G, H, D, P, S, int(bool(weights))))
 
@@ -927,7 +929,7 @@ def cache_decode(k, v, q, lens, out=None, workspace=None, *, prefix_k=None, pref
     if out is None:
         out = torch.empty_like(q)
         ptrs[8] = out.data_ptr()
-    need = cache_decode_workspace_bytes(*dims, weights is not None)
+    need = plan[5]
     if workspace is None:
         workspace = torch.empty(max(need, 4), dtype=torch.uint8, device=q.device)
         wp = workspace.data_ptr()
