@@ -850,16 +850,22 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
   }
 }
 
-// p.njoin workgroups of rows, then the weights' parts of every (b, g).
+// p.njoin workgroups of rows and, with weights, those of every (b, g)'s keys; what
+// takes longest first: rows where a thread walks all parts of one (flat), else
+// the weights (B32 S8192 39.7 us a step against 42.8 the other way round, B16
+// H71 19.6 against 21.0).
 template <bool F16, bool WT>
 __global__ void __launch_bounds__(256) cache_join_kernel(StepParams p) {
-  const int x = blockIdx.x;
+  int x = blockIdx.x;
   if constexpr (WT) {
-    if (x >= p.njoin) {
-      const int nw = (p.S + p.wkeys - 1) / p.wkeys, bg = (x - p.njoin) / nw;
-      add_weights(p, bg, (x - p.njoin - bg * nw) * p.wkeys);
+    const int nw = (p.S + p.wkeys - 1) / p.wkeys, all = p.B * p.G * nw;
+    const int y = p.flat ? x - p.njoin : x;    // the weights' workgroup
+    if (y >= 0 && y < all) {
+      const int bg = y / nw;
+      add_weights(p, bg, (y - bg * nw) * p.wkeys);
       return;
     }
+    if (!p.flat) x -= all;
   }
   if (p.flat) join_rows<F16>(p, x);
   else join_row<F16>(p, x);
