@@ -150,9 +150,9 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
   auto stK = [&](int s) { return (lds_char_t*)(smem + s * STAGE); };
   auto stV = [&](int s) { return (lds_char_t*)(smem + s * STAGE + K_BYTES); };
   // ---- DMA of block `blk` into stage s: K pieces past the row's end are
-  // clamped (their keys are masked), rows d >= Dr come from zeros; V rows past
-  // s1 repeat the last one, whose weight there is zero (slots behind a length
-  // may hold NaN, and 0 NaN is NaN)
+  // clamped (their keys are masked), rows d >= Dr come from zeros, and so do V
+  // rows past s1 (slots behind a length may hold anything, and a weight of zero
+  // times NaN or infinity is NaN)
   auto copies = [&](int s, int blk, auto once) {
     auto copy = [](const void* from, uint32_t to) {
       to = __builtin_amdgcn_readfirstlane(to);
@@ -178,8 +178,10 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
       const int j = wave * V_INSTR + i;
       const int kr = j * V_ROWS_PER_I + lane / (D / 8);
       const int c = min((lane % (D / 8)) ^ cv_swz<D>(kr), Dr / 8 - 1);
-      const int key = min(kv0 + kr, s1 - 1);
-      copy(vg + (int64_t)key * Dr + c * 8, lv + j * 1024);
+      const int key = kv0 + kr;
+      const void* const from = key < s1 ? (const void*)(vg + (int64_t)key * Dr + c * 8)
+                                        : (const void*)(loom_zero_kb + lane * 4);
+      copy(from, lv + j * 1024);
     }
   };
   auto issue = [&](int s, int blk) {

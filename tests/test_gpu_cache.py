@@ -237,6 +237,19 @@ def test_decode_nan_and_inf_values_reach_their_rows_only(lh):
     assert not bad[1, 0, 33:].any()
 
 
+def test_decode_infinite_values(lh):
+    """An infinity in the last key's V: the masked keys behind it add nothing."""
+    for n, H in ((33, 4), (5, 40), (97, 71)):
+        t = make(1, 1, H, 64, 0, 104, [n], torch.bfloat16, seed=n)
+        t["v"][0, 0, n - 1, 3] = math.inf
+        t["v"][0, 0, n - 1, 9] = -math.inf
+        o, _ = step(lh, t)
+        o = o.float().cpu()
+        assert (o[..., 3] == math.inf).all() and (o[..., 9] == -math.inf).all()
+        o[..., 3] = o[..., 9] = 0
+        assert torch.isfinite(o).all()
+
+
 def test_decode_arguments(lh):
     """Outputs and workspace given, an empty prefix tensor, weights elsewhere."""
     t = make(2, 2, 4, 64, 0, 40, [40, 33], torch.bfloat16, seed=7)
