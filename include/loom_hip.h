@@ -296,8 +296,8 @@ int loom_hip_ssd_prologue_f16(const void* x, const void* dt, const void* A, cons
  * behind every sequence's n keys: the first c = clamp(counts[b], 0, T) of its T
  * tokens (all T with counts null); tokens past slot S-1 are dropped.  With
  * weights [B,G,S] fp32 (null: none) the new keys' weights become zero.
- * lens_out[b] = min(n + c, S); lens_out must not overlap lens or counts.  Moves
- * 16-bit elements of either type. */
+ * lens_out[b] = min(n + c, S).  k, v, weights and lens_out overlap neither the other
+ * tensors nor each other.  Moves 16-bit elements of either type. */
 int loom_hip_cache_append(void* k, void* v, void* weights, const void* lens, const void* new_k,
                           const void* new_v, const void* counts, void* lens_out, int64_t B,
                           int64_t G, int64_t D, int64_t S, int64_t T, void* stream, char* err,

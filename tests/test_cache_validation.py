@@ -65,6 +65,8 @@ def test_append_extents(dims, code, word):
     ({0: P(0, 2)}, "aligned"), ({1: P(1, 2)}, "aligned"), ({4: P(4, 8)}, "aligned"),
     ({5: P(5, 2)}, "aligned"), ({3: P(3, 2)}, "aligned"), ({2: P(2, 2)}, "aligned"),
     ({7: P(3)}, "overlap"), ({7: P(3, 4)}, "overlap"), ({7: P(6)}, "overlap"),
+    ({4: P(0, 4096)}, "overlap"), ({5: P(1)}, "overlap"), ({1: P(0)}, "overlap"),
+    ({2: P(0, 64)}, "overlap"), ({3: P(1, 64)}, "overlap"), ({7: P(2, 4)}, "overlap"),
 ])
 def test_append_pointers(ptrs, word):
     rc, msg = append(ptrs)
