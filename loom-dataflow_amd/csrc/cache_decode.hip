@@ -59,7 +59,7 @@ struct StepParams {
   int nprefix;      // workgroups of the prefix
   int njoin, flat;  // workgroups that join rows; several rows to each
   int once;         // own keys are read by non-temporal copies
-  int wkeys;        // keys of a workgroup that gathers weights: 128 or 256
+  int wkeys;        // keys of a workgroup that gathers weights: 128 to 1024
   float c2;         // scale * log2(e)
 };
 
@@ -774,15 +774,19 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
   auto load = [&](int h0, int hn) {            // heads h0 + grp + NG x below hn
 #pragma unroll
     for (int x = 0; x < HN; ++x)
-      sc[x] = *reinterpret_cast<const f32x4_t*>(
-          score + (int64_t)min(h0 + grp + NG * x, hn - 1) * p.Sp);
+      if (h0 + NG * x < hn)                    // (the same for all groups)
+        sc[x] = *reinterpret_cast<const f32x4_t*>(
+            score + (int64_t)min(h0 + grp + NG * x, hn - 1) * p.Sp);
   };
   const int b = p.G == 1 ? bg : bg / p.G, g = bg - b * p.G;
   const int len = seq_len(p, b);
   if (j0 >= len) return;
   load(0, min(p.H, HB));
   const Splits sp0 = row_splits(p, b, g, 0);
-  const float w_in = p.w[(int64_t)bg * p.S + min(j0 + tid, len - 1)];
+  float w_in[4];                               // of keys j0 + tid, 256 apart
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (256 * u < wkeys) w_in[u] = p.w[(int64_t)bg * p.S + min(j0 + 256 * u + tid, len - 1)];
   f32x4_t sum = f32x4_t{0.f, 0.f, 0.f, 0.f};
   // threads to a head: as many as leave 256 threads a head each
   const int tph = p.H <= 32 ? 8 : p.H <= 64 ? 4 : 2, hpp = kThreads / tph;
@@ -847,11 +851,15 @@ LOOM_DEV void add_weights(const StepParams& p, int bg, int j0) {
   }
   s_w[tid] = sum;
   __syncthreads();
-  if (tid < wkeys && j0 + tid < len) {
-    const float* f = reinterpret_cast<const float*>(s_w) + tid;
-    float w = 0.f;
-    for (int x = 0; x < NG; ++x) w += f[x * wkeys];
-    p.w_out[(int64_t)bg * p.S + j0 + tid] = w_in + w;
+  const float* const f = reinterpret_cast<const float*>(s_w);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int e = 256 * u + tid;
+    if (e < wkeys && j0 + e < len) {
+      float w = 0.f;
+      for (int x = 0; x < NG; ++x) w += f[x * wkeys + e];
+      p.w_out[(int64_t)bg * p.S + j0 + e] = w_in[u] + w;
+    }
   }
 }
 
@@ -1006,10 +1014,14 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   p.flat = B * G * H > 2048 || (B * G * H >= 1024 && parts <= 16);
   p.njoin = (int)(p.flat ? cdiv64(B * G * H, kThreads / (D / 4)) : B * G * H);
   p.once = s.nht == 1 && 4 * B * G * S * D > (int64_t)256 << 20;
-  // 256 keys spread the heads' statistics over more of them (B32 H32 n6144 33.6
-  // against 35.3 us for the step); 128 give few workgroups more of the CUs (B1
-  // S4096 12.9 against 13.3, B16 H71 n1024 17.9 against 18.9)
-  p.wkeys = B * G * cdiv64(S, 256) < 256 ? 128 : 256;
+  // Keys of a workgroup that gathers weights: many spread the heads' statistics over
+  // more of them and leave fewer groups without a head (G256 in all, H4 S4096 118,
+  // 105, 98 and 95 us a step with 128, 256, 512 and 1024, H32 146, 135, 133 and 131;
+  // B32 H32 S8192 42.0, 40.0, 38.8 and 39.9), as long as they leave workgroups for
+  // the CUs (B1 S4096 12.9 against 13.3 with 128 and 256, B16 H32 S4096 18.1 against
+  // 19.8 with 256 and 512)
+  auto parts_of = [&](int64_t keys) { return B * G * cdiv64(S, keys); };
+  p.wkeys = parts_of(1024) >= 1024 ? 1024 : parts_of(512) >= 256 ? 512 : parts_of(256) >= 256 ? 256 : 128;
   p.c2 = scale * 1.4426950408889634f;
   if (loom_validate_only()) return loom_ok(err, errlen);
   hipStream_t st = static_cast<hipStream_t>(stream);
