@@ -362,9 +362,9 @@ __global__ void __launch_bounds__(kSel) cache_select_kernel(EvictParams p) {
 // consecutive ones a lane, over rows_k rows d: the stretch of the source row that
 // they span comes in 16-byte pieces, goes through LDS and leaves as 16-byte
 // pieces of the packed row (a 2-byte load and store per element moved the same
-// rows at 2.7 TB/s, bound by the address unit).  Stretches longer than a window
-// of 4096 slots take several passes over the rows.  V parts take slots_v rows of
-// D elements, 16 bytes a lane, and the weights.
+// rows at 2.7 TB/s, bound by the address unit).  A stretch longer than a window of
+// 4096 slots goes through it piece by piece.  V parts take slots_v rows of D
+// elements, 16 bytes a lane, and the weights.
 constexpr int kMoveJ = 512, kMoveWin = 4096, kMoveP = kMoveWin / 512;
 
 // eight elements of a row from slot i on (zeros past n)
@@ -385,12 +385,24 @@ LOOM_DEV u32x4_t row_slots8(const uint16_t* row, int i, int n) {
   return v;
 }
 
-// One window of a wave's rows, NP pieces of 512 slots to a row, 8 / NP rows at a
-// time: eight 16-byte loads a lane are in flight whatever stretch the kept slots
-// span.
+// eight kept elements of a row, slots j .. j + 7 of n
+LOOM_DEV void store_slots8(uint16_t* to, const uint32_t (&h)[8], int j, int n) {
+  if (j + 8 <= n) {
+    store_any16(to, u32x4_t{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16,
+                            h[6] | h[7] << 16});
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (j + e < n) to[e] = (uint16_t)h[e];
+  }
+}
+
+// The rows of kept slots that span one window, NP pieces of 512 slots to a row, 8 / NP
+// rows at a time: eight 16-byte loads a lane are in flight whatever stretch the kept
+// slots span.
 template <int NP>
 LOOM_DEV void move_rows(const EvictParams& p, const uint16_t* src, uint16_t* dst, int rows,
-                        const int (&at)[8], int w0, int len, bool whole, int j, int n, int lane,
+                        const int (&at)[8], int s0, int len, int j, int n, int lane,
                         uint16_t* win) {
   constexpr int RB = kMoveP / NP;
   u32x4_t piece[RB][NP];
@@ -401,7 +413,7 @@ LOOM_DEV void move_rows(const EvictParams& p, const uint16_t* src, uint16_t* dst
 #pragma unroll
         for (int u = 0; u < NP; ++u)
           if (u * 512 < len)
-            piece[rb][u] = row_slots8(src + (int64_t)(r0 + rb) * p.S, w0 + u * 512 + 8 * lane, p.S);
+            piece[rb][u] = row_slots8(src + (int64_t)(r0 + rb) * p.S, s0 + u * 512 + 8 * lane, p.S);
   };
   fetch(0);
   for (int r0 = 0; r0 < rows; r0 += RB) {
@@ -419,20 +431,49 @@ LOOM_DEV void move_rows(const EvictParams& p, const uint16_t* src, uint16_t* dst
     for (int rb = 0; rb < RB; ++rb)
       if (r0 + rb < rows) {
         const uint16_t* from = win + rb * NP * 512;
-        uint16_t* to = dst + (int64_t)(r0 + rb) * p.So;
-        uint16_t h[8];
+        uint32_t h[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = from[whole ? at[e] - w0 : min(max(at[e] - w0, 0), len - 1)];
-        if (whole && j + 8 <= n) {
-          u32x4_t v;
-          __builtin_memcpy(&v, h, 16);
-          store_any16(to, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (j + e < n && at[e] >= w0 && at[e] < w0 + len) to[e] = h[e];
-        }
+        for (int e = 0; e < 8; ++e) h[e] = from[at[e] - s0];
+        store_slots8(dst + (int64_t)(r0 + rb) * p.So, h, j, n);
       }
+  }
+}
+
+// The rows of kept slots that lie further apart: window after window of a row, each
+// lane picking up what it has there, one store when the row is through (stores of
+// what each window held, 2 bytes each: B8 G8 S16383 -> 1024 95.9 us a call against
+// 66.5).
+LOOM_DEV void move_far(const EvictParams& p, const uint16_t* src, uint16_t* dst, int rows,
+                       const int (&at)[8], int s0, int last, int j, int n, int lane,
+                       uint16_t* win) {
+  u32x4_t piece[kMoveP];
+  auto fetch = [&](int row, int w0) {
+#pragma unroll
+    for (int u = 0; u < kMoveP; ++u)
+      if (u * 512 <= last - w0)
+        piece[u] = row_slots8(src + (int64_t)row * p.S, w0 + u * 512 + 8 * lane, p.S);
+  };
+  uint32_t h[8] = {};
+  fetch(0, s0);
+  for (int row = 0, w0 = s0; row < rows;) {
+    lds_order();
+#pragma unroll
+    for (int u = 0; u < kMoveP; ++u)
+      if (u * 512 <= last - w0)
+        *reinterpret_cast<u32x4_t*>(win + u * 512 + 8 * lane) = piece[u];
+    lds_order();
+    const bool end = last - w0 < kMoveWin;
+    const int row1 = row + end, w1 = end ? s0 : w0 + kMoveWin;
+    if (row1 < rows) fetch(row1, w1);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // clamped: lanes without a slot here read the same two places
+      const uint32_t x = win[min(max(at[e] - w0, 0), kMoveWin - 1)];
+      h[e] = (uint32_t)(at[e] - w0) < (uint32_t)kMoveWin ? x : h[e];
+    }
+    if (end) store_slots8(dst + (int64_t)row * p.So, h, j, n);
+    row = row1;
+    w0 = w1;
   }
 }
 
@@ -462,18 +503,15 @@ __global__ void __launch_bounds__(256) cache_move_kernel(EvictParams p) {
     uint16_t* const dst = p.k_out + ((int64_t)bg * D + d0) * p.So + j;
     // rows of whole 16-byte pieces are read at their boundaries
     const int s0 = p.S % 8 == 0 ? first & ~7 : first;
-    for (int w0 = s0; w0 <= last; w0 += kMoveWin) {
-      const int len = min(kMoveWin, last + 1 - w0);
-      const bool whole = last - s0 < kMoveWin;
-      auto rows_of = [&](auto np) {
-        move_rows<decltype(np)::value>(p, src, dst, rows, at, w0, len, whole, j, n, lane,
-                                       s_win[wave]);
-      };
-      if (len <= 512) rows_of(std::integral_constant<int, 1>{});
-      else if (len <= 1024) rows_of(std::integral_constant<int, 2>{});
-      else if (len <= 2048) rows_of(std::integral_constant<int, 4>{});
-      else rows_of(std::integral_constant<int, 8>{});
-    }
+    const int len = last + 1 - s0;
+    auto rows_of = [&](auto np) {
+      move_rows<decltype(np)::value>(p, src, dst, rows, at, s0, len, j, n, lane, s_win[wave]);
+    };
+    if (len <= 512) rows_of(std::integral_constant<int, 1>{});
+    else if (len <= 1024) rows_of(std::integral_constant<int, 2>{});
+    else if (len <= 2048) rows_of(std::integral_constant<int, 4>{});
+    else if (len <= kMoveWin) rows_of(std::integral_constant<int, 8>{});
+    else move_far(p, src, dst, rows, at, s0, last, j, n, lane, s_win[wave]);
     return;
   }
   x -= p.nk;
@@ -654,9 +692,14 @@ int loom_hip_cache_evict(const void* k, const void* v, const void* weights, cons
   int rc = loom_check_launch(err, errlen, "cache_evict (select)");
   if (rc) return rc;
   // rows of a K part's wave: as many (two to four) as leave about 4096 waves
-  // (B8 G8 S16383: four rows 79.2 us a call, eight 80.3, sixteen 85.8, two 89.3)
+  // (B8 G8 S16383: four rows 79.2 us a call, eight 80.3, sixteen 85.8, two 89.3);
+  // one or two where the kept slots of a full cache are spread over several windows,
+  // which a wave takes one after another (B8 G8 S16383 -> 1024: four rows 99.6, two
+  // 66.5; B32 S16384 -> 512: two 54.2, one 42.7)
   p.njk = (int)cdiv64(keep, kMoveJ);
-  p.rows_k = (int)std::max<int64_t>(2, std::min<int64_t>(4, B * G * p.njk * D / 4096));
+  const bool far = S >= kMoveWin / kMoveJ * keep;
+  p.rows_k = (int)std::max<int64_t>(
+      far ? 1 : 2, std::min<int64_t>(far ? 2 : 4, B * G * p.njk * D / 4096));
   p.nk = (int)(p.njk * cdiv64(D, 4 * p.rows_k));
   // slots of a V part: eight 16-byte pieces a thread, fewer for about 1024 parts
   p.slots_v = (int)std::max<int64_t>(
