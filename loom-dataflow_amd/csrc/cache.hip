@@ -192,8 +192,9 @@ LOOM_DEV uint32_t waves_before(const uint32_t* v, int lane, int wave) {
 // slot numbers: the instructions per key bound this kernel (a CU's four SIMDs
 // each run four of its waves).  With KPT > 0 the keys stay in registers (KPT a
 // lane, slots 64 apart; in LDS, with rolled loops, 23 us against 15 at 16 a
-// lane), else (KPT 0, longer caches) every pass reads the weights again.
-// 4096 weights 6.0 us, 32 x 8192 8.6 us, 64 x 16383 11.8 us.
+// lane), else (KPT 0, longer caches) every pass reads the weights again,
+// eight a lane at a time (8 x 70000: 57 us against 88 one by one).  4096 weights
+// 6.0 us, 32 x 8192 8.6 us, 64 x 16383 11.8 us, 8 x 32768 19.0 us.
 template <int KPT>
 __global__ void __launch_bounds__(kSel) cache_select_kernel(EvictParams p) {
   __shared__ __attribute__((aligned(16))) uint32_t hist[kCopyStep * kCopies], s_list[kList];
@@ -244,8 +245,14 @@ __global__ void __launch_bounds__(kSel) cache_select_kernel(EvictParams p) {
 #pragma unroll
       for (int u = 0; u < KPT; ++u) f(i0 + u * 64, reg[u]);
     } else {
-      for (int u = 0; u < per && i0 + u * 64 < n; ++u)
-        f(i0 + u * 64, key_of(i0 + u * 64, load(i0 + u * 64 + lane)));
+      for (int u0 = 0; u0 < per && i0 + u0 * 64 < n; u0 += 8) {
+        float y[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) y[u] = load(i0 + (u0 + u) * 64 + lane);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (u0 + u < per) f(i0 + (u0 + u) * 64, key_of(i0 + (u0 + u) * 64, y[u]));
+      }
     }
   };
   uint32_t left = (uint32_t)p.keep;            // how many stay; n > keep keys are above 0
@@ -688,6 +695,7 @@ int loom_hip_cache_evict(const void* k, const void* v, const void* weights, cons
   else if (S <= 4 * kSel) select(cache_select_kernel<4>);
   else if (S <= 8 * kSel) select(cache_select_kernel<8>);
   else if (S <= 16 * kSel) select(cache_select_kernel<16>);
+  else if (S <= 32 * kSel) select(cache_select_kernel<32>);
   else select(cache_select_kernel<0>);
   int rc = loom_check_launch(err, errlen, "cache_evict (select)");
   if (rc) return rc;

@@ -373,6 +373,11 @@ def evict_check(lh, B, G, D, S, So, lens, keep, recent, sinks, e=torch.bfloat16,
     (1, 1, 64, 70000, 704, [69999], 600, 9, 0), (1, 1, 40, 70001, 701, [70001], 600, 9, 0),
     (1, 2, 64, 16384, 2049, [16383], 2048, 0, 0), (1, 2, 64, 16377, 3000, [16377], 2999, 0, 0),
     (1, 1, 72, 8192, 6000, [8192], 5555, 100, 4),
+    (3, 1, 64, 12288, 600, [12288, 700, 4097], 599, 5, 4), (2, 1, 24, 9000, 90, [9000, 8999], 77, 0, 0),
+    # weights in registers up to 32768 slots, read again past them
+    (2, 1, 16, 20001, 5000, [20001, 16385], 4999, 100, 4),
+    (2, 1, 8, 32768, 32000, [32768, 32767], 31999, 0, 3),
+    (2, 1, 8, 32769, 40, [32769, 1500], 40, 9, 9), (1, 1, 8, 263000, 100, [262145], 99, 0, 0),
 ], ids=lambda c: "x".join(map(str, c[:5])) + f"-{c[6]}")
 def test_evict(lh, case):
     for e in TYPES.values():
@@ -394,6 +399,9 @@ def test_evict_ties_and_odd_weights(lh):
     w[0, 0] = math.nan
     for keep in (20, 299, 400):
         evict_check(lh, 2, 2, 64, S, 400, [S, 600], keep, 10, 5, w=w.clone())
+    for S2 in (30000, 40000):     # ties over all of a long cache
+        w2 = torch.randint(0, 2, (1, 1, S2), generator=g).float()
+        evict_check(lh, 1, 1, 8, S2, 20000, [S2], 20000, 10, 5, w=w2)
     # values that differ in their last bit only
     w = (torch.full((1, 1, S), 1.0).view(torch.int32)
          + torch.randperm(S, generator=g).int()).view(torch.float32)
