@@ -903,7 +903,9 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P, int64_t S)
     // stages (B32 H32 P8192 21.8 us against 25.0, P2048 14.4 against 15.8)
     s.rtp = rows <= 32 ? 32 : G * cdiv64(rows, 128) * cdiv64(P, kKeys) < 8 * 256 ? 64 : 128;
     s.ntp = (int)cdiv64(rows, s.rtp);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / (G * s.ntp), 64));
+    // splits for half of the workgroups, the own keys' parts run beside them (D256
+    // B32 G8 H4 P4096 S2048: all of them 98.5 us a step, half 86.2)
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(slots / 2 / (G * s.ntp), 64));
     s.tile_p = (int)(cdiv64(std::max<int64_t>(cdiv64(P, want), 2 * kKeys), kKeys) * kKeys);
     s.nsp = (int)cdiv64(P, s.tile_p);
     s.nprefix = (int)(G * s.ntp * s.nsp);
