@@ -166,6 +166,19 @@ def test_decode_shapes_of_a_launch(lh, e):
     check(lh, "heads of 71", 3, 1, 71, 128, 131, 501, [0, 250, 501], t)
 
 
+@pytest.mark.parametrize("e", TYPES)
+def test_decode_weights_of_many_keys(lh, e):
+    """512 and 1024 keys to a workgroup that gathers weights: several of them to a
+    sequence, lengths at their ends, one to many heads."""
+    t = TYPES[e]
+    lens = [0, 1, 511, 512, 513, 1023, 1024, 1025, 1100, 256, 255, 257]
+    check(lh, "parts of 512", 24, 4, 5, 16, 0, 1100, [lens[b % 12] for b in range(24)], t)
+    check(lh, "parts of 512, heads", 100, 1, 33, 16, 9, 1540, [lens[b % 12] + 436 for b in range(100)], t)
+    check(lh, "parts of 1024", 64, 8, 1, 8, 0, 1101, [lens[b % 12] for b in range(64)], t)
+    check(lh, "parts of 1024, heads", 173, 3, 19, 8, 7, 1025, [lens[b % 12] for b in range(173)], t)
+    check(lh, "parts of 1024, many heads", 520, 1, 257, 8, 0, 1032, [lens[b % 12] for b in range(520)], t)
+
+
 def test_decode_caches_past_the_last_level_cache(lh):
     check(lh, "large caches", 2, 1, 8, 128, 100, 300000, [300000, 123457], torch.bfloat16)
     check(lh, "large caches, odd", 2, 1, 8, 128, 0, 300001, [300001, 64], torch.float16)
