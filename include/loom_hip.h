@@ -313,10 +313,11 @@ size_t loom_hip_cache_decode_workspace_bytes(int64_t B, int64_t G, int64_t H, in
  * of the prefix that every sequence shares (prefix_k [G,D,P], prefix_v [G,P,D];
  * both null with P = 0) and the n keys of (b, g) together.  `scale` (finite and
  * positive) multiplies q.k.  A row without keys, or whose scores are all -inf,
- * gives zeros.  With weights and weights_out [B,G,S] fp32 (both or neither;
- * they may be the same tensor, else must not overlap):
+ * gives zeros.  With weights and weights_out [B,G,S] fp32 (both or neither):
  *   weights_out[b,g,j] = weights[b,g,j] + sum over h of row (b,g,h)'s softmax
  * weight of own key j, for j < n; other elements are left as they are.
+ * out, weights_out and the workspace overlap neither the other tensors nor each
+ * other, except that weights_out may be weights and out may be q.
  * S (P) not a multiple of 8 needs D*S (D*P) < 2^30; B*G*H at most 2^23, with
  * weights B*G*ceil(S/128) too.  Sums run in an order that the extents and lengths
  * fix: equal calls give equal bits. */

@@ -548,27 +548,6 @@ __global__ void __launch_bounds__(256) cache_move_kernel(EvictParams p) {
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// A tensor's bytes (none of one that is left out).
-struct Span {
-  const void* p;
-  int64_t n;
-};
-bool overlap(const Span& a, const Span& b) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-  return a.p && b.p && x < y + (uint64_t)b.n && y < x + (uint64_t)a.n;
-}
-// Whether an output shares a byte with an input or another output.
-template <int I, int O>
-bool outputs_overlap(const Span (&in)[I], const Span (&out)[O]) {
-  for (int o = 0; o < O; ++o) {
-    for (const Span& i : in)
-      if (overlap(i, out[o])) return true;
-    for (int x = 0; x < o; ++x)
-      if (overlap(out[x], out[o])) return true;
-  }
-  return false;
-}
-
 }  // namespace
 
 extern "C" {
@@ -596,9 +575,9 @@ int loom_hip_cache_append(void* k, void* v, void* weights, const void* lens, con
                      "cache_append: v, new_k and new_v must be 16-byte aligned, k 16-byte (2-byte "
                      "when S is not a multiple of 8), the others 4-byte");
   const int64_t cache = B * G * S * D * 2, added = B * T * G * D * 2;
-  const Span in[] = {{new_k, added}, {new_v, added}, {lens, B * 4}, {counts, B * 4}},
-             out[] = {{k, cache}, {v, cache}, {weights, B * G * S * 4}, {lens_out, B * 4}};
-  if (outputs_overlap(in, out))
+  const LoomSpan in[] = {{new_k, added}, {new_v, added}, {lens, B * 4}, {counts, B * 4}},
+                 out[] = {{k, cache}, {v, cache}, {weights, B * G * S * 4}, {lens_out, B * 4}};
+  if (loom_outputs_overlap(in, out))
     return loom_fail(err, errlen, LOOM_EINVAL,
                      "cache_append: k, v, weights and lens_out must not overlap the other tensors "
                      "or each other");
@@ -663,10 +642,10 @@ int loom_hip_cache_evict(const void* k, const void* v, const void* weights, cons
                      "cache_evict: v and v_out must be 16-byte aligned, k and k_out 16-byte (2-byte "
                      "when their capacity is not a multiple of 8)");
   const int64_t kin = B * G * S * D * 2, kout = B * G * S_out * D * 2;
-  const Span in[] = {{k, kin}, {v, kin}, {weights, B * G * S * 4}, {lens, B * 4}},
-             out[] = {{k_out, kout}, {v_out, kout}, {weights_out, B * G * S_out * 4},
-                      {lens_out, B * 4}, {index, B * G * keep * 4}};
-  if (outputs_overlap(in, out))
+  const LoomSpan in[] = {{k, kin}, {v, kin}, {weights, B * G * S * 4}, {lens, B * 4}},
+                 out[] = {{k_out, kout}, {v_out, kout}, {weights_out, B * G * S_out * 4},
+                          {lens_out, B * 4}, {index, B * G * keep * 4}};
+  if (loom_outputs_overlap(in, out))
     return loom_fail(err, errlen, LOOM_EINVAL,
                      "cache_evict: outputs must not overlap the inputs or each other");
   EvictParams p{};

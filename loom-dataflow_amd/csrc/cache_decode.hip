@@ -966,16 +966,25 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
     return loom_fail(err, errlen, LOOM_EINVAL,
                      "cache_decode: tensors must be 16-byte aligned (k and prefix_k 2-byte when "
                      "their extent is not a multiple of 8; lens and weights 4-byte)");
-  const uintptr_t w0 = reinterpret_cast<uintptr_t>(weights);
-  const uintptr_t w1 = reinterpret_cast<uintptr_t>(weights_out);
-  if (w0 != w1 && w0 < w1 + (uint64_t)(B * G * S * 4) && w1 < w0 + (uint64_t)(B * G * S * 4))
-    return loom_fail(err, errlen, LOOM_EINVAL,
-                     "cache_decode: weights_out is weights itself or does not overlap it");
   const size_t need = loom_hip_cache_decode_workspace_bytes(B, G, H, D, P, S, weights != nullptr);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return loom_fail(err, errlen, LOOM_EINVAL,
                      "cache_decode: workspace needs %zu bytes (16-byte aligned), got %zu", need,
                      workspace_bytes);
+  // The workspace is written while tensors are read, out and weights_out while
+  // lens, weights and the workspace are: a shared byte gives results that depend on
+  // the order of workgroups.  Two are safe: weights_out on weights (every element is
+  // read and written by one thread) and out on q (read before the join writes)
+  const int64_t cache = B * G * S * D * 2, prefix = G * P * D * 2, rows = B * G * H * D * 2,
+                summed = B * G * S * 4;
+  const LoomSpan in[] = {{prefix_k, prefix}, {prefix_v, prefix}, {k, cache}, {v, cache},
+                         {lens, B * 4}, {out == q ? nullptr : q, rows},
+                         {weights_out == weights ? nullptr : weights, summed}},
+                 outs[] = {{out, rows}, {weights_out, summed}, {workspace, (int64_t)need}};
+  if (loom_outputs_overlap(in, outs))
+    return loom_fail(err, errlen, LOOM_EINVAL,
+                     "cache_decode: out, weights_out and the workspace must not overlap the other "
+                     "tensors or each other (but weights_out may be weights, out may be q)");
   StepParams p{};
   p.pk = static_cast<const uint16_t*>(prefix_k);
   p.pv = static_cast<const uint16_t*>(prefix_v);

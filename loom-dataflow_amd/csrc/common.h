@@ -218,6 +218,27 @@ static inline bool loom_prod_le(std::initializer_list<int64_t> xs, int64_t limit
 }
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// A tensor's bytes (none of one that is left out).
+struct LoomSpan {
+  const void* p;
+  int64_t n;
+};
+static inline bool loom_overlap(const LoomSpan& a, const LoomSpan& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.p && b.p && x < y + (uint64_t)b.n && y < x + (uint64_t)a.n;
+}
+// Whether an output shares a byte with an input or another output.
+template <int I, int O>
+static inline bool loom_outputs_overlap(const LoomSpan (&in)[I], const LoomSpan (&out)[O]) {
+  for (int o = 0; o < O; ++o) {
+    for (const LoomSpan& i : in)
+      if (loom_overlap(i, out[o])) return true;
+    for (int x = 0; x < o; ++x)
+      if (loom_overlap(out[x], out[o])) return true;
+  }
+  return false;
+}
+
 // The reference bounds every loom.sym by the extent of the loop it tiles
 // (its upper_bound, exported as natural_ub:
 // lib/passes/lcs/src/staged_etg_builder.cpp:1420-1430) and aligns the inner
