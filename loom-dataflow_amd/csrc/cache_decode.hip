@@ -30,6 +30,7 @@
 // heavy key's rounding cancels.  The weights use the unrounded p and their own sum.
 #include "common.h"
 
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -55,6 +56,7 @@ struct StepParams {
   int B, G, H, D, P, S, Sp;
   int nht;          // row tiles of a (b, g)'s H heads
   int chunks;       // chunks that the whole batch aims at
+  int most;         // chunks that it has at most
   int rtp, ntp, nsp, tile_p;   // the prefix: rows of a tile, tiles per head, splits, keys of one
   int nprefix;      // workgroups of the prefix
   int njoin, flat;  // workgroups that join rows; several rows to each
@@ -487,8 +489,9 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
 // Where chunk c of the batch's own keys lies.  t, a multiple of 64, is the chunk
 // that gives about p.chunks of them over all sequences whatever their lengths,
 // at least 128 keys (64 leave more parts to join than they save: B1 S16384 with
-// weights 25.8 against 18.8 us a step, B32 of 256 to 1024 keys 16.0 and 13.7); a
-// sequence takes as many as t asks for, of equal size, sequences in order.
+// weights 25.8 against 18.8 us a step, B32 of 256 to 1024 keys 16.0 and 13.7), and
+// larger while that gives more than p.most of them; a sequence takes as many as t
+// asks for, of equal size, sequences in order.
 // Every workgroup works it out from the lengths, so nothing is planned on the
 // host and a replayed graph follows them.
 struct Chunk {
@@ -500,6 +503,10 @@ LOOM_DEV int chunk_keys(const StepParams& p, int64_t total) {
   const int64_t per = (total + p.chunks - 1) / p.chunks;
   return (int)min((int64_t)1 << 30, max((int64_t)2, (per + kKeys - 1) / kKeys) * kKeys);
 }
+// The next larger t.  It ends: the first t gives at most p.chunks + B chunks, p.most
+// is at least 2 B where it is set, so t grows by less than half (random batches took
+// up to nine tries, most one).
+LOOM_DEV int more_keys(int t) { return t + max(kKeys, t / 32 / kKeys * kKeys); }
 LOOM_DEV int wave_scan(int v, int lane) {   // inclusive
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
@@ -518,9 +525,12 @@ LOOM_DEV Chunk find_chunk(const StepParams& p, int c) {
   Chunk r{-1, 0, 0, 1, 0, 0};
   if (p.B <= 64) {          // each wave by itself: one load, no barrier
     const int n = lane < p.B ? seq_len(p, lane) : 0;
-    const int t = chunk_keys(p, wave_sum64(n));
-    const int cnt = (n + t - 1) / t;
-    const int inc = wave_scan(cnt, lane);
+    int t = chunk_keys(p, wave_sum64(n)), cnt, inc;
+    for (;; t = more_keys(t)) {
+      cnt = (n + t - 1) / t;
+      inc = wave_scan(cnt, lane);
+      if (__builtin_amdgcn_readlane(inc, 63) <= p.most) break;
+    }
     const uint64_t m = __builtin_amdgcn_ballot_w64(c < inc);
     if (m == 0) return r;
     r.b = __builtin_ctzll(m);
@@ -536,15 +546,21 @@ LOOM_DEV Chunk find_chunk(const StepParams& p, int c) {
     if (lane == 0) s_sum[wave] = total;
     if (tid == 0) s_r[0] = -1;
     __syncthreads();
-    const int t = chunk_keys(p, s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
+    int t = chunk_keys(p, s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
     int base = 0;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + tid;
       const int n = b < p.B ? seq_len(p, b) : 0;
-      const int cnt = (n + t - 1) / t;
-      const int inc = wave_scan(cnt, lane);
-      if (lane == 63) s_cnt[wave] = inc;
-      __syncthreads();
+      int cnt, inc, all;
+      for (;; t = more_keys(t)) {   // (p.most is set up to 256 sequences only)
+        cnt = (n + t - 1) / t;
+        inc = wave_scan(cnt, lane);
+        if (lane == 63) s_cnt[wave] = inc;
+        __syncthreads();
+        all = s_cnt[0] + s_cnt[1] + s_cnt[2] + s_cnt[3];
+        if (all <= p.most) break;
+        __syncthreads();
+      }
       int at = base + inc - cnt;
       for (int x = 0; x < wave; ++x) at += s_cnt[x];
       if (c >= at && c < at + cnt) {
@@ -553,7 +569,7 @@ LOOM_DEV Chunk find_chunk(const StepParams& p, int c) {
         s_r[2] = cnt;
         s_r[3] = at;
       }
-      base += s_cnt[0] + s_cnt[1] + s_cnt[2] + s_cnt[3];
+      base += all;
       __syncthreads();
       if (c < base) break;
     }
@@ -886,7 +902,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(StepParams p) {
 
 // The launch's shape, from the extents alone.
 struct Shape {
-  int nht, chunks, rtp, ntp, nsp, tile_p, nprefix;
+  int nht, chunks, most, rtp, ntp, nsp, tile_p, nprefix;
   int64_t max_chunks, Sp, rows;
 };
 
@@ -910,13 +926,18 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P, int64_t S)
     s.nsp = (int)cdiv64(P, s.tile_p);
     s.nprefix = (int)(G * s.ntp * s.nsp);
   }
-  // Chunks of the whole batch: one round of workgroups, less what rounding up to
-  // whole chunks adds to it (B32 of 4096 to 8192 keys with weights: 46.1 us at
-  // 512 chunks, of which 16 wait for a second round, against 39.9); with few
-  // chunks to a sequence two rounds, which even out their sizes better (B48 G8
-  // of 1024 to 4096 keys 116 against 107 us), unless prefix parts fill the gaps
+  // Chunks of the whole batch: one round of workgroups, less about what rounding up
+  // to whole chunks adds to it (B32 of 4096 to 8192 keys with weights: 46.1 us at
+  // 512 chunks, of which 16 wait for a second round, against 39.9).  Rounding up
+  // adds anything up to B - 1, so without a prefix, whose parts run beside them, the
+  // chunks grow until they are no more than a round (B57 H32 of 8000 keys 513
+  // workgroups 64.6 us, 456 of them 52.7; B47 G4 H2 D80 of 3056 keys 564 54.3, 376
+  // 44.0; B11 G8 H5 D256 of 4032 keys 264 of 256 99.0, 176 75.8).  With few chunks to
+  // a sequence two rounds, which even out their sizes better (B48 G8 of 1024 to 4096
+  // keys 116 against 107 us), unless prefix parts fill the gaps
   const int64_t each = std::max<int64_t>(1, slots / (G * s.nht));
   s.chunks = (int)(each >= 2 * B ? each - B * 5 / 8 : P > 0 ? each : 2 * each);
+  s.most = each >= 2 * B && P == 0 ? (int)each : INT_MAX;
   s.max_chunks = s.chunks + B;
   s.rows = s.nsp * B * G * H + s.max_chunks * G * H;
   return s;
@@ -1013,6 +1034,7 @@ int cache_decode_impl(const void* prefix_k, const void* prefix_v, const void* k,
   p.Sp = (int)s.Sp;
   p.nht = s.nht;
   p.chunks = s.chunks;
+  p.most = s.most;
   p.rtp = s.rtp;
   p.ntp = s.ntp;
   p.nsp = s.nsp;
