@@ -28,6 +28,9 @@
 // Rounding: scores, bases and sums are fp32; p is rounded to 16 bits for its
 // product with v, and out is divided by the sum of the rounded p, so that one
 // heavy key's rounding cancels.  The weights use the unrounded p and their own sum.
+// f16 rounds below 2^-14 to multiples of 2^-24, so its p are held 2^7 times larger
+// (the base lies that far below the largest score): a key down to 2^-21 of the heaviest
+// of its part keeps all eleven bits, one below 2^-32 is lost, as below 2^-25 without.
 #include "common.h"
 
 #include <climits>
@@ -229,6 +232,9 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
 
   u32x4_t qf[DSTEPS][QT];
   const float c2 = p.c2;
+  // log2 of what the largest p starts at, and how far it may rise: to 2^15, half of
+  // f16's largest number (bf16 has fp32's exponents)
+  constexpr float kLift = F16 ? 7.f : 0.f, kRise = kLift + 8.f;
   float m_run[QT], lx[QT];
   f32x4_t ot[DT][QT], lacc[QT];
   const u32x4_t ones = u32x4_t{kOnePair<F16>, kOnePair<F16>, kOnePair<F16>, kOnePair<F16>};
@@ -325,10 +331,11 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
           mx = fmaxf(mx, v);
         }
       lmax[qt] = mx;
-      big |= mx > 8.f;
+      big |= mx > kRise;
     }
     // lazy online softmax: a row's base is set by its first block with a
     // finite score and moves (O and the sums rescale) when one rises 2^8 above
+    // that block's largest
     if (first || __builtin_amdgcn_ballot_w64(big) != 0) {
       bool unset_left = false;
 #pragma unroll
@@ -337,7 +344,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const bool unset = first && lacc[qt][0] == 0.f;
-        const float shift = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
+        const float shift = unset ? (mx == -INFINITY ? 0.f : mx - kLift) : fmaxf(mx - kLift, 0.f);
         const float alpha = unset ? 1.f : fast_exp2(-shift);
         lacc[qt] *= alpha;
         lx[qt] *= alpha;
