@@ -898,14 +898,20 @@ def cache_append(k, v, lens, new_k, new_v, lens_out=None, *, counts=None, weight
     return lens_out
 
 
+#: the workspace of a step past the extents that cache_decode takes (SIZE_MAX)
+_NO_SIZE = (1 << 64) - 1
+
+
 def cache_decode_workspace_bytes(B, G, H, D, P, S, weights=False) -> int:
     return int(_lib.loom_hip_cache_decode_workspace_bytes(B, G, H, D, P, S, int(bool(weights))))
 
 
 def cache_decode_workspace(B, G, H, D, P, S, weights, device):
     """A cache_decode workspace (uint8 tensor) for these extents."""
-    return torch.empty(max(cache_decode_workspace_bytes(B, G, H, D, P, S, weights), 4),
-                       dtype=torch.uint8, device=device)
+    need = cache_decode_workspace_bytes(B, G, H, D, P, S, weights)
+    if need == _NO_SIZE:
+        raise ValueError("cache_decode: problem too large")
+    return torch.empty(max(need, 4), dtype=torch.uint8, device=device)
 
 
 def cache_decode(k, v, q, lens, out=None, workspace=None, *, prefix_k=None, prefix_v=None,
@@ -930,14 +936,17 @@ def cache_decode(k, v, q, lens, out=None, workspace=None, *, prefix_k=None, pref
         out = torch.empty_like(q)
         ptrs[8] = out.data_ptr()
     need = plan[5]
-    if workspace is None:
-        workspace = torch.empty(max(need, 4), dtype=torch.uint8, device=q.device)
+    if need == _NO_SIZE:      # too large: the entry point says so
+        wp, size = None, 0
+    elif workspace is None:
+        size = max(need, 4)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
         wp = workspace.data_ptr()
     else:
-        wp = _check_workspace(workspace, need, q.device, "cache_decode")
+        wp, size = _check_workspace(workspace, need, q.device, "cache_decode"), workspace.numel()
     if dims[4] == 0:      # an empty prefix is no prefix
         ptrs[0] = ptrs[1] = None
-    _cache_run(plan, dev, *ptrs, wp, workspace.numel(), *dims, float(scale))
+    _cache_run(plan, dev, *ptrs, wp, size, *dims, float(scale))
     return out
 
 
