@@ -969,6 +969,11 @@ def cache_evict(k, v, weights, lens, keep, *, recent=0, sinks=0, capacity=None, 
     B, G, D, S, So = plan[2][:5]
     if min(B, G, D, So, keep) <= 0:
         raise ValueError("cache_evict: extents and keep must be positive")
+    # before anything is allocated, and before ctypes takes 64 bits of an int
+    if keep > So or not 0 <= recent <= keep or not 0 <= sinks <= keep - recent:
+        raise LoomHipError(plan[1], 1, f"cache_evict: must satisfy 1 <= keep <= capacity, 0 <= "
+                           f"recent, sinks and recent + sinks <= keep (keep={keep} "
+                           f"recent={recent} sinks={sinks} capacity={So})")
     if k_out is None:
         k_out = torch.empty((B, G, D, So), dtype=plan[3], device=k.device)
         ptrs[4] = k_out.data_ptr()

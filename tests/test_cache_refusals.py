@@ -56,3 +56,20 @@ def test_no_workspace_is_that_large():
         lh.cache_decode_workspace(70000, 1, 1, 8, 0, 8, False, "cpu")
     assert lh.cache_decode_workspace(2, 1, 1, 8, 0, 8, False, "cpu").numel() == \
         lh.cache_decode_workspace_bytes(2, 1, 1, 8, 0, 8)
+
+
+def evict(keep, S=64, **kw):
+    return lh.cache_evict(meta(2, 1, 8, S), meta(2, 1, S, 8), meta(2, 1, S, dtype=torch.float32),
+                          meta(2, dtype=torch.int32), keep, **kw)
+
+
+@pytest.mark.parametrize("keep,kw", [
+    (65, {}), (1 << 40, {}), (1 << 64, {}), (33, {"capacity": 32}), ((1 << 64) + 5, {}),
+    (8, {"recent": 9}), (8, {"recent": -1}), (8, {"sinks": -1}), (8, {"recent": 4, "sinks": 5}),
+    # a multiple of 2^64 more than what would fit
+    (8, {"recent": 1 << 64}), (8, {"sinks": (1 << 64) + 2}), (8, {"recent": -(1 << 64)}),
+])
+def test_evict_keeps_at_most_the_capacity(made_up_device, keep, kw):
+    with pytest.raises(lh.LoomHipError, match="keep") as e:
+        evict(keep, **kw)
+    assert e.value.code == 1
