@@ -23,8 +23,10 @@
 //     prefix alone 51 us, own keys alone 98, together 113);
 //   - cache_join_kernel: joins a row's parts and, from the scores that the chunks
 //     left in the workspace, adds the weights.  Scores are kept in fp32: weights
-//     are sums of many steps.  Rereading K instead would cost as many bytes at 32
-//     heads, more below.
+//     are sums of many steps.  Written and read they are 8 H bytes a key, a second
+//     reading of K 2 D: as many at 32 heads of D 128, and fewer scores below.  Above
+//     that (71 heads of D 64: 568 bytes against 128) K would be the smaller; no
+//     kernel here scores it twice, and what that would take is not measured.
 // Rounding: scores, bases and sums are fp32; p is rounded to 16 bits for its
 // product with v, and out is divided by the sum of the rounded p, so that one
 // heavy key's rounding cancels.  The weights use the unrounded p and their own sum.
@@ -77,7 +79,10 @@ LOOM_DEV int seq_len(const StepParams& p, int b) { return min(max(p.lens[b], 0),
 // nothing that is read again.  Taken for the own keys of caches larger than the
 // 256 MB last-level cache (B48 G8 S4096 under a prefix 124 -> 113 us a step, B8 G8
 // S8192 43.5 -> 38.7); smaller ones may still lie there from the last step (B16
-// G8 S2048 29.3 against 31.6), and a prefix is read by many sequences
+// G8 S2048 29.3 against 31.6), and a prefix is read by many sequences.  The rule
+// knows the capacity, not the lengths: large caches that hold little pay up to 5%
+// (B48 G8 H8 S8192 holding 1024 to 1536 keys each 55.6 against 53.1 us, 100 to 400
+// keys 20.6 against 20.0)
 LOOM_DEV void dma_once16(const void* g, uint32_t lds) {
   asm volatile(
       "s_mov_b32 m0, %1\n\t"
@@ -915,7 +920,12 @@ struct Shape {
 
 Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P, int64_t S) {
   Shape s{};
-  const int64_t slots = D > 128 ? 256 : 512;   // workgroups that run at once
+  // Workgroups that a launch is sized for: what runs at once, one a CU past D 128 and
+  // two up to it.  Up to D 64 three would fit (164 registers, 32 KB), but sizes for
+  // 768 gain without a prefix (B32 H32 of 4096 to 8192 keys 22.1 -> 19.4 us a step, B32
+  // G8 H8 of 1024 to 4096 41.8 -> 38.9) and lose under one or with equal lengths (B16 G8
+  // H4 P4095 S2048 18.6 -> 20.6, B57 H32 of 8000 keys 31.7 -> 33.2)
+  const int64_t slots = D > 128 ? 256 : 512;
   s.nht = H <= 32 ? 1 : (int)cdiv64(H, 128);
   s.Sp = cdiv64(S, kKeys) * kKeys;
   if (P > 0) {
@@ -927,7 +937,10 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t P, int64_t S)
     s.rtp = rows <= 32 ? 32 : G * cdiv64(rows, 128) * cdiv64(P, kKeys) < 8 * 256 ? 64 : 128;
     s.ntp = (int)cdiv64(rows, s.rtp);
     // splits for half of the workgroups, the own keys' parts run beside them (D256
-    // B32 G8 H4 P4096 S2048: all of them 98.5 us a step, half 86.2)
+    // B32 G8 H4 P4096 S2048: all of them 98.5 us a step, half 86.2), and at most 64,
+    // whose parts a row joins in one round of loads: with up to 256 B1 H32 takes
+    // 19.3 us at P16384 against 16.6 and 28.3 at 65536 against 25.0, though 36.2 at
+    // 131072 against 47.1 (G2 H16 P65536 29.3 against 31.3)
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(slots / 2 / (G * s.ntp), 64));
     s.tile_p = (int)(cdiv64(std::max<int64_t>(cdiv64(P, want), 2 * kKeys), kKeys) * kKeys);
     s.nsp = (int)cdiv64(P, s.tile_p);
