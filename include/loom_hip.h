@@ -347,6 +347,85 @@ int loom_hip_cache_evict(const void* k, const void* v, const void* weights, cons
                          int64_t B, int64_t G, int64_t D, int64_t S, int64_t S_out, int64_t keep,
                          int64_t recent, int64_t sinks, void* stream, char* err, size_t errlen);
 
+/* ---- memory that does not grow with the sequence ----------------------------
+ * What a decoder of windowed and linear attention layers does over prompts and in
+ * steps; the reference has no counterpart.  All extents must be positive. */
+
+/* Bytes of loom_hip_window_attention's workspace; 0 where it needs none (the
+ * workspace may then be null).  It holds nothing between calls; calls that overlap
+ * in time need one each. */
+size_t loom_hip_window_attention_workspace_bytes(int64_t B, int64_t G, int64_t H, int64_t D,
+                                                 int64_t T, int64_t S, int64_t window,
+                                                 int64_t sinks);
+
+/* Attention of new tokens over a sliding window of the caches that
+ * loom_hip_cache_append fills, and their first `sinks` keys: k [B,G,D,S] (keys
+ * transposed), v [B,G,S,D], lens [B] the lengths after the new tokens were
+ * appended.  Of sequence b's n = clamp(lens[b], 0, S) keys the last c =
+ * clamp(counts[b], 0, T) (T with counts null) are the new tokens', and row t < c of
+ * q, out [B,T,G,H,D] (H query heads to each KV head) is at position p = n - c + t:
+ *   out = sum over j <= p, j > p - window or j < sinks, of softmax_j(scale q.k_j) v_j.
+ * A row that sees no key (p < 0), or whose scores are all -inf, gives zeros; rows
+ * t >= c are left as they are.  What a key that a row does not see holds (NaN,
+ * infinities) does not reach the row.  T = 1 is a decoding step.  `scale` is finite
+ * and positive, window at least 1 (from S on: every key up to p), sinks at least 0,
+ * D a multiple of 8 up to 256 (else LOOM_HIP_EUNSUP), B*G <= 65535, S and T*H at
+ * most 2^29, B*G*ceil(T*H/32) at most 2^23; S not a multiple of 8 needs D*S < 2^30.
+ * out and the workspace overlap neither the other tensors nor each other, except
+ * that out may be q.  Equal calls give equal bits. */
+int loom_hip_window_attention(const void* k, const void* v, const void* q, const void* lens,
+                              const void* counts, void* out, void* workspace,
+                              size_t workspace_bytes, int64_t B, int64_t G, int64_t H, int64_t D,
+                              int64_t T, int64_t S, int64_t window, int64_t sinks, float scale,
+                              void* stream, char* err, size_t errlen);
+int loom_hip_window_attention_f16(const void* k, const void* v, const void* q, const void* lens,
+                                  const void* counts, void* out, void* workspace,
+                                  size_t workspace_bytes, int64_t B, int64_t G, int64_t H,
+                                  int64_t D, int64_t T, int64_t S, int64_t window, int64_t sinks,
+                                  float scale, void* stream, char* err, size_t errlen);
+
+/* Bytes of loom_hip_linear_attention's workspace, as above. */
+size_t loom_hip_linear_attention_workspace_bytes(int64_t B, int64_t G, int64_t H, int64_t D,
+                                                 int64_t E, int64_t T);
+
+/* Linear attention with a decay for each head, over T tokens: q [B,T,G,H,D], k
+ * [B,T,G,D], v [B,T,G,E], log_decay [G,H] fp32 (at most 0; -inf: a head without
+ * memory), state, state_out [B,G,H,D,E] fp32.  With a = exp(log_decay[g,h]), S_-1 =
+ * state[b,g,h] (0 with state null):
+ *   S_t = a S_(t-1) + k_t v_t^T,   out[b,t,g,h] = scale S_t^T q_t
+ * for the first c = clamp(counts[b], 0, T) tokens (T with counts null);
+ * state_out[b,g,h] = S_(c-1), and out's rows t >= c are left as they are.  What
+ * tokens behind c, or later than a row, hold does not reach it.  `scale` is finite
+ * and positive, D and E multiples of 8 up to 256 (else LOOM_HIP_EUNSUP), B*G*H at
+ * most 2^20, T at most 2^29.  out, state_out and the workspace overlap neither the
+ * other tensors nor each other, except that state_out may be state.  Equal calls
+ * give equal bits. */
+int loom_hip_linear_attention(const void* q, const void* k, const void* v, const void* log_decay,
+                              const void* state, const void* counts, void* out, void* state_out,
+                              void* workspace, size_t workspace_bytes, int64_t B, int64_t G,
+                              int64_t H, int64_t D, int64_t E, int64_t T, float scale,
+                              void* stream, char* err, size_t errlen);
+int loom_hip_linear_attention_f16(const void* q, const void* k, const void* v,
+                                  const void* log_decay, const void* state, const void* counts,
+                                  void* out, void* state_out, void* workspace,
+                                  size_t workspace_bytes, int64_t B, int64_t G, int64_t H,
+                                  int64_t D, int64_t E, int64_t T, float scale, void* stream,
+                                  char* err, size_t errlen);
+
+/* The same for one token, its state updated in place: q, out [B,G,H,D], [B,G,H,E],
+ * k [B,G,D], v [B,G,E].  A sequence with counts[b] <= 0 has none: its state and its
+ * rows of out are left as they are. */
+int loom_hip_linear_attention_step(const void* q, const void* k, const void* v,
+                                   const void* log_decay, void* state, const void* counts,
+                                   void* out, int64_t B, int64_t G, int64_t H, int64_t D,
+                                   int64_t E, float scale, void* stream, char* err,
+                                   size_t errlen);
+int loom_hip_linear_attention_step_f16(const void* q, const void* k, const void* v,
+                                       const void* log_decay, void* state, const void* counts,
+                                       void* out, int64_t B, int64_t G, int64_t H, int64_t D,
+                                       int64_t E, float scale, void* stream, char* err,
+                                       size_t errlen);
+
 /* ---- MLIR memref descriptors ---------------------------------------------
  * A materialized variant is an MLIR function over memrefs; a caller lowered
  * through MLIR's C interface (`_mlir_ciface_<func>`, whose arguments are

@@ -57,12 +57,17 @@ _SIGS = {
     "loom_hip_cache_append": [_vp] * 8 + [_i64] * 5 + [_vp, *_ERR],
     "loom_hip_cache_decode": [_vp] * 10 + [_sz] + [_i64] * 6 + [_f32, _vp, *_ERR],
     "loom_hip_cache_evict": [_vp] * 9 + [_i64] * 8 + [_vp, *_ERR],
+    "loom_hip_window_attention": [_vp] * 7 + [_sz] + [_i64] * 8 + [_f32, _vp, *_ERR],
+    "loom_hip_linear_attention": [_vp] * 9 + [_sz] + [_i64] * 6 + [_f32, _vp, *_ERR],
+    "loom_hip_linear_attention_step": [_vp] * 7 + [_i64] * 5 + [_f32, _vp, *_ERR],
 }
 # f16 twins: same arguments, 16-bit tensors in IEEE binary16
 for _name in ("loom_hip_matmul", "loom_hip_batch_matmul", "loom_hip_split_k_matmul_gather",
               "loom_hip_attention", "loom_hip_flash_decode",
               "loom_hip_helion_mamba2_chunk_scan_kernel", "loom_hip_ssd_bmm_chunk",
-              "loom_hip_ssd_chunk_state_passing", "loom_hip_ssd_prologue", "loom_hip_cache_decode"):
+              "loom_hip_ssd_chunk_state_passing", "loom_hip_ssd_prologue", "loom_hip_cache_decode",
+              "loom_hip_window_attention", "loom_hip_linear_attention",
+              "loom_hip_linear_attention_step"):
     _SIGS[_name + "_f16"] = _SIGS[_name]
 for _name, _args in _SIGS.items():
     _fn = getattr(_lib, _name)
@@ -74,6 +79,10 @@ _lib.loom_hip_flash_decode_workspace_bytes.argtypes = [_i64] * 5
 _lib.loom_hip_flash_decode_workspace_bytes.restype = _sz
 _lib.loom_hip_cache_decode_workspace_bytes.argtypes = [_i64] * 6 + [ctypes.c_int]
 _lib.loom_hip_cache_decode_workspace_bytes.restype = _sz
+_lib.loom_hip_window_attention_workspace_bytes.argtypes = [_i64] * 8
+_lib.loom_hip_window_attention_workspace_bytes.restype = _sz
+_lib.loom_hip_linear_attention_workspace_bytes.argtypes = [_i64] * 6
+_lib.loom_hip_linear_attention_workspace_bytes.restype = _sz
 _lib.loom_hip_version.restype = ctypes.c_char_p
 _lib.loom_hip_materialize_variants.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p),
                                                ctypes.c_int, ctypes.c_char_p, _sz, *_ERR]
@@ -143,7 +152,9 @@ EXPORTED = tuple(_SIGS) + tuple(_CIFACE) + ("loom_hip_peak_hbm_read", "loom_hip_
                                             "loom_hip_dispatch_memref_f16",
                                             "loom_hip_check_memref") + ("loom_hip_split_k_workspace_bytes",
                            "loom_hip_flash_decode_workspace_bytes",
-                           "loom_hip_cache_decode_workspace_bytes", "loom_hip_version",
+                           "loom_hip_cache_decode_workspace_bytes",
+                           "loom_hip_window_attention_workspace_bytes",
+                           "loom_hip_linear_attention_workspace_bytes", "loom_hip_version",
                            "loom_hip_materialize_variants", "loom_hip_parse_variant",
                            "loom_hip_dispatch", "loom_hip_dispatch_f16", "loom_hip_check_variant",
                            "loom_hip_workspace_bytes",
@@ -831,7 +842,7 @@ def _cache_plan(func: str, sig: tuple, extra: tuple):
     return getattr(_lib, name), name, dims, e, names, need
 
 
-def _cache_enter(func: str, tensors, extra=()):
+def _cache_enter(func: str, tensors, extra=(), plan_of=_cache_plan):
     """(plan, device index, device pointers) of a call; raises what is wrong
     with a tensor (the form of all of them first, then their devices)."""
     sig, ptrs, dev, odd = [], [], None, False
@@ -851,7 +862,7 @@ def _cache_enter(func: str, tensors, extra=()):
                 ptrs.append(t.data_ptr())
         else:
             raise TypeError(f"{func}: expected torch.Tensors, got {type(t).__name__}")
-    plan = _cache_plan(func, tuple(sig), extra)
+    plan = plan_of(func, tuple(sig), extra)
     if odd:
         there = [(t, n) for t, n in zip(tensors, plan[4]) if t is not None]
         for t, name in there:
@@ -991,6 +1002,177 @@ def cache_evict(k, v, weights, lens, keep, *, recent=0, sinks=0, capacity=None, 
         ptrs[8] = index.data_ptr()
     _cache_run(plan, dev, *ptrs, B, G, D, S, So, keep, recent, sinks)
     return k_out, v_out, weights_out, lens_out, index
+
+# ---------------------------------------------------------------------------
+# memory that does not grow with the sequence: attention over a sliding window,
+# linear attention with a decay for each head
+# ---------------------------------------------------------------------------
+
+# Tensor arguments in the entry points' order, as in _CACHE_SPECS.
+_BOUNDED_SPECS = {
+    "window_attention": lambda B, G, H, D, T, S: (
+        ("k", "e", (B, G, D, S)), ("v", "e", (B, G, S, D)), ("q", "e", (B, T, G, H, D)),
+        ("lens", _i32, (B,)), ("counts?", _i32, (B,)), ("out?", "e", (B, T, G, H, D))),
+    "window_decode": lambda B, G, H, D, T, S: (
+        ("k", "e", (B, G, D, S)), ("v", "e", (B, G, S, D)), ("q", "e", (B, G, H, D)),
+        ("lens", _i32, (B,)), ("counts?", _i32, (B,)), ("out?", "e", (B, G, H, D))),
+    "linear_attention": lambda B, G, H, D, E, T: (
+        ("q", "e", (B, T, G, H, D)), ("k", "e", (B, T, G, D)), ("v", "e", (B, T, G, E)),
+        ("log_decay", _fp32, (G, H)), ("state?", _fp32, (B, G, H, D, E)), ("counts?", _i32, (B,)),
+        ("out?", "e", (B, T, G, H, E)), ("state_out?", _fp32, (B, G, H, D, E))),
+    "linear_attention_step": lambda B, G, H, D, E: (
+        ("q", "e", (B, G, H, D)), ("k", "e", (B, G, D)), ("v", "e", (B, G, E)),
+        ("log_decay", _fp32, (G, H)), ("state", _fp32, (B, G, H, D, E)), ("counts?", _i32, (B,)),
+        ("out?", "e", (B, G, H, E))),
+}
+
+
+@functools.lru_cache(maxsize=1024)
+def _bounded_plan(func: str, sig: tuple, extra: tuple):
+    """(entry point, its name, extents, 16-bit type, arguments' names, workspace
+    bytes, out's shape) of a call's signature; kept by value for the last 1024, as
+    _cache_plan's.  Raises what is wrong with it."""
+    window = func.startswith("window")
+    # q and, of a window, k, or v give the extents
+    ranks = {"window_attention": ((2, 5), (0, 4)), "window_decode": ((2, 4), (0, 4)),
+             "linear_attention": ((0, 5), (2, 4)), "linear_attention_step": ((0, 4), (2, 3))}[func]
+    names = [a[0].rstrip("?") for a in
+             _BOUNDED_SPECS[func](*(0,) * (5 if func == "linear_attention_step" else 6))]
+    for i, r in ranks:
+        if sig[i] is None or len(sig[i][1]) != r:
+            raise ValueError(f"{func}: {names[i]} must have {r} dims, got "
+                             f"{'None' if sig[i] is None else f'shape {tuple(sig[i][1])}'}")
+    q, x = (tuple(sig[i][1]) for i, _ in ranks)
+    B, G, H, D = q[0], *q[-3:]
+    T = q[1] if len(q) == 5 else 1
+    dims = (B, G, H, D, T, x[3]) if window else (B, G, H, D, x[-1], T)
+    spec = _BOUNDED_SPECS[func](*(dims[:5] if func == "linear_attention_step" else dims))
+    e = sig[ranks[0][0]][0]
+    if e not in (_bf16, _f16):
+        raise TypeError(f"q: expected torch.bfloat16 or torch.float16, got {e}")
+    for s, (name, kind, shape) in zip(sig, spec):
+        if s is None:
+            if not name.endswith("?"):
+                raise TypeError(f"{name}: expected a torch.Tensor, got NoneType")
+            continue
+        want = e if kind == "e" else kind
+        if s[0] != want:
+            raise TypeError(f"{name.rstrip('?')}: expected {want}, got {s[0]}")
+        if tuple(s[1]) != shape:
+            raise ValueError(f"{name.rstrip('?')}: expected shape {shape}, got {tuple(s[1])}")
+    name = "loom_hip_" + ("window_attention" if window else func) + ("_f16" if e == _f16 else "")
+    if window:
+        need = window_attention_workspace_bytes(*dims, *extra)
+    else:
+        need = linear_attention_workspace_bytes(*dims) if func == "linear_attention" else 0
+    out = spec[6 if func.startswith("linear") else 5][2]
+    return getattr(_lib, name), name, dims, e, names, need, out
+
+
+def _bounded_workspace(workspace, need, device, what):
+    """(the tensor, which has to live until the call is made; its pointer; its size)"""
+    if need == 0 or need == _NO_SIZE:      # none, or too large: the entry point says so
+        return None, None, 0
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        return workspace, workspace.data_ptr(), need
+    return workspace, _check_workspace(workspace, need, device, what), workspace.numel()
+
+
+def window_attention_workspace_bytes(B, G, H, D, T, S, window, sinks=0) -> int:
+    return int(_lib.loom_hip_window_attention_workspace_bytes(B, G, H, D, T, S, window, sinks))
+
+
+def _window(func, k, v, q, lens, window, out, workspace, sinks, counts, scale):
+    window, sinks = int(window), int(sinks)
+    if not 1 <= window < 1 << 63 or not 0 <= sinks < 1 << 63:   # (ctypes takes 64 bits of an int)
+        raise LoomHipError("loom_hip_window_attention", 1, f"{func}: window must be at least 1, "
+                           f"sinks at least 0 (window={window} sinks={sinks})")
+    plan, dev, ptrs = _cache_enter(func, (k, v, q, lens, counts, out), (window, sinks),
+                                   _bounded_plan)
+    dims = plan[2]
+    if scale is None:
+        scale = 1.0 / math.sqrt(dims[3]) if dims[3] > 0 else 1.0
+    if out is None:
+        out = torch.empty_like(q)
+        ptrs[5] = out.data_ptr()
+    _ws, wp, size = _bounded_workspace(workspace, plan[5], q.device, func)
+    _cache_run(plan, dev, *ptrs, wp, size, *dims, window, sinks, float(scale))
+    return out
+
+
+def window_attention(k, v, q, lens, window, out=None, workspace=None, *, sinks=0, counts=None,
+                     scale=None):
+    """Attention of new tokens over a sliding window of the caches they were
+    appended to, and the caches' first ``sinks`` keys.
+
+    k [B,G,D,S] (keys transposed), v [B,G,S,D], q [B,T,G,H,D] (H query heads to each
+    of G KV heads), lens [B] int32 -> out [B,T,G,H,D].  ``lens`` is what cache_append
+    returns for the same tokens: of sequence b's keys the last ``counts[b]`` (int32; all T by
+    default) are the new tokens', whose token t, at position p = lens[b] -
+    counts[b] + t, sees the keys j <= p with j > p - ``window`` or j < ``sinks``.
+    Rows behind a sequence's tokens are left as they are (unset where ``out`` is not
+    given).  ``scale`` defaults to 1/sqrt(D)."""
+    return _window("window_attention", k, v, q, lens, window, out, workspace, sinks, counts, scale)
+
+
+def window_decode(k, v, q, lens, window, out=None, workspace=None, *, sinks=0, counts=None,
+                  scale=None):
+    """window_attention of one new token to each sequence: q, out [B,G,H,D], as
+    cache_decode's.  (With ``counts``, int32, a sequence of 0 has none: its rows are
+    left as they are.)"""
+    return _window("window_decode", k, v, q, lens, window, out, workspace, sinks, counts, scale)
+
+
+def linear_attention_workspace_bytes(B, G, H, D, E, T) -> int:
+    return int(_lib.loom_hip_linear_attention_workspace_bytes(B, G, H, D, E, T))
+
+
+def linear_attention(q, k, v, log_decay, state=None, out=None, state_out=None, workspace=None, *,
+                     counts=None, scale=None):
+    """Linear attention with a decay for each head, over the T tokens of a prompt.
+
+    q [B,T,G,H,D] (H query heads to each of G key heads), k [B,T,G,D], v [B,T,G,E],
+    log_decay [G,H] fp32 (at most 0) -> (out [B,T,G,H,E], state_out [B,G,H,D,E] fp32):
+    S_t = exp(log_decay) S_(t-1) + k_t v_t^T, out_t = scale S_t^T q_t, from ``state``
+    (zero by default) on; state_out is the last S, and may be ``state``.  Sequence b
+    has ``counts[b]`` tokens (int32; all T by default); rows of out behind them are left as
+    they are (unset where ``out`` is not given).  ``scale`` defaults to
+    1/sqrt(D)."""
+    plan, dev, ptrs = _cache_enter("linear_attention",
+                                   (q, k, v, log_decay, state, counts, out, state_out), (),
+                                   _bounded_plan)
+    dims = plan[2]
+    if scale is None:
+        scale = 1.0 / math.sqrt(dims[3]) if dims[3] > 0 else 1.0
+    if out is None:
+        out = torch.empty(plan[6], dtype=plan[3], device=q.device)
+        ptrs[6] = out.data_ptr()
+    if state_out is None:
+        state_out = torch.empty(dims[:5], dtype=_fp32, device=q.device)
+        ptrs[7] = state_out.data_ptr()
+    _ws, wp, size = _bounded_workspace(workspace, plan[5], q.device, "linear_attention")
+    _cache_run(plan, dev, *ptrs, wp, size, *dims, float(scale))
+    return out, state_out
+
+
+def linear_attention_step(q, k, v, log_decay, state, out=None, *, counts=None, scale=None):
+    """linear_attention of one token to each sequence, its state updated in place.
+
+    q [B,G,H,D], k [B,G,D], v [B,G,E], log_decay [G,H] fp32, state [B,G,H,D,E] fp32 ->
+    out [B,G,H,E].  A sequence whose ``counts[b]`` (int32) is 0 has no token: its state
+    and its rows of out are left as they are."""
+    plan, dev, ptrs = _cache_enter("linear_attention_step",
+                                   (q, k, v, log_decay, state, counts, out), (), _bounded_plan)
+    dims = plan[2]
+    if scale is None:
+        scale = 1.0 / math.sqrt(dims[3]) if dims[3] > 0 else 1.0
+    if out is None:
+        out = torch.empty(plan[6], dtype=plan[3], device=q.device)
+        ptrs[6] = out.data_ptr()
+    _cache_run(plan, dev, *ptrs, *dims[:5], float(scale))
+    return out
+
 
 
 # ---------------------------------------------------------------------------
