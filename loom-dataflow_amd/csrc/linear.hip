@@ -15,8 +15,8 @@
 
 namespace {
 
-constexpr int kC = 64;            // tokens of a chunk
-constexpr int kIT = kC / 16, kM = kC / 32;
+constexpr int kC = 32;            // tokens of a chunk
+constexpr int kIT = kC / 16;      // tiles of queries
 
 struct LinearParams {
   const uint16_t* q;
@@ -85,8 +85,8 @@ LOOM_DEV const char* uniform(const char* p) {
       (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
 }
 
-// Chunked form.  A workgroup of W waves walks the chunks of 64 tokens of one (b, g, h)
-// and 16 W columns of E in order, each wave holding the state's D x 16 columns in the
+// Chunked form.  A workgroup of four waves walks the chunks of 32 tokens of one (b, g, h)
+// and 64 NT columns of E in order, each wave holding the state's D x 16 NT columns in the
 // accumulators of its MFMAs, fp32.  For a chunk of tokens 0 .. C-1 and the state S before
 // it:
 //   P_ij = scale a^(i-j) q_i.k_j (j <= i),
@@ -95,29 +95,29 @@ LOOM_DEV const char* uniform(const char* p) {
 // The MFMAs compute transposed tiles, S^T[e, d] . Q^T[d, i] and V^T[e, j] . P^T[j, i], so
 // that a wave's state feeds the first product from its own accumulators (packed to 16
 // bits: lane group g holds rows d = 16 t + 4 g + 0..3, and q's pieces are read in that
-// order), and P^T is built from the accumulators of K Q^T, a part of it to each wave,
-// shared through LDS.
+// order), and P^T is built from the accumulators of K Q^T, a quarter to a wave, shared
+// through LDS.
 // Rounding: S and P to 16 bits as operands, each once; a^(C-1-j) v_j as a sum of three
 // bf16 or two f16 numbers, so that the state keeps fp32's accuracy.  f16 operands are
 // scaled by powers of two where they leave its range.
 // ONLY_STATE: a segment's own state from zero (the first's from the initial state), which
 // later segments start from.
-template <int DK, int W, bool F16, bool ONLY_STATE>
-__global__ void __launch_bounds__(64 * W, 1) linear_chunk_kernel(LinearParams p) {
-  constexpr int SL = 16 * W;                    // columns of a workgroup
+template <int DK, int NT, bool F16, bool ONLY_STATE>
+__global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
+  constexpr int W = 4, SL = 16 * NT * W;        // columns of a workgroup
   constexpr int KROW = DK * 2, VROW = SL * 2;
   constexpr int Q_BYTES = ONLY_STATE ? 0 : kC * KROW, K_BYTES = kC * KROW, V_BYTES = kC * VROW;
   constexpr int STAGE = Q_BYTES + K_BYTES + V_BYTES;
   constexpr int QK_INSTR = K_BYTES / 1024 / W, V_INSTR = V_BYTES / 1024 / W;
   static_assert(QK_INSTR >= 1 && V_INSTR >= 1, "every wave issues copies");
   constexpr int KS = DK / 32, DT = DK / 16;
-  constexpr int MPW = W == 8 ? kM / 2 : kM;     // key pairs of the wave's part of P
   constexpr int TERMS = F16 ? 2 : 3;            // 16-bit numbers that hold a^(C-1-j) v_j
-  static_assert(W == 4 || W == 8, "four query tiles");
-  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
-  __shared__ __attribute__((aligned(16))) u32x4_t s_p[ONLY_STATE ? 1 : kIT * kM * 64];
+  static_assert(kC == 32 && (NT == 1 || NT == 2), "one step of the MFMA over a chunk's tokens");
+  constexpr int NS = 3;                         // stages: two chunks on their way
+  __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
+  __shared__ __attribute__((aligned(16))) u32x4_t s_p[ONLY_STATE ? 1 : 2 * kIT * 64];
   __shared__ float s_pow[kC + 1];
-  __shared__ float s_ps[kIT * kM];              // f16: what a part of P was scaled by
+  __shared__ float s_ps[2][kIT];                // f16: what a tile of P was scaled by
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -143,12 +143,6 @@ __global__ void __launch_bounds__(64 * W, 1) linear_chunk_kernel(LinearParams p)
   const int tokens = wanted ? (int)min((int64_t)(c - t0), seglen) : 0;
   const int nch = (tokens + kC - 1) / kC;
 
-  const float lg = p.g[gh];
-  if (tid <= kC) s_pow[tid] = (float)decay_pow(lg, tid);
-  // over a whole chunk, and over the last one
-  const Decay full = split_decay(decay_pow(lg, kC));
-  const Decay last = split_decay(decay_pow(lg, tokens - (nch - 1) * kC));
-
   // ---- copies of chunk ci into stage s: rows past the sequence and chunks past D or E
   // from zeros.  A whole chunk of whole rows takes each copy as the chunk's scalar base
   // plus this lane's offset, computed once (fast: all offsets fit 32 bits).
@@ -159,7 +153,7 @@ __global__ void __launch_bounds__(64 * W, 1) linear_chunk_kernel(LinearParams p)
   // token strides in bytes (at most 2^29)
   const uint32_t qs = (uint32_t)(GH * D * 2), ks_ = (uint32_t)(p.G * D * 2),
                  vs = (uint32_t)(p.G * E * 2);
-  const bool fast = D == DK && sl * SL + SL <= E && qs < (1u << 25) && vs < (1u << 25);
+  const bool fast = D == DK && sl * SL + SL <= E && qs < (1u << 26) && vs < (1u << 26);
   uint32_t qoff[QK_INSTR], koff[QK_INSTR], voff[V_INSTR];
   auto offsets = [&](auto& off, uint32_t stride, auto n) {
     constexpr int N = decltype(n)::value, INSTR = kC * N * 2 / 1024 / W;
@@ -204,34 +198,56 @@ __global__ void __launch_bounds__(64 * W, 1) linear_chunk_kernel(LinearParams p)
     rows(vb, vs, (E - sl * SL) / 8, voff, VC{}, base + Q_BYTES + K_BYTES);
   };
   if (nch > 0) issue(0, 0);
+  if (nch > 1) issue(1, 1);
 
-  // ---- the state: s[dt][i] is row d = 16 dt + 4 g4 + i, column ec
-  const int col0 = sl * SL + wave * 16, ec = col0 + r;
-  f32x4_t s[DT];
+  const float lg = p.g[gh];
+  if (tid <= kC) s_pow[tid] = (float)decay_pow(lg, tid);
+  // over a whole chunk, and over the last one.  A rounded factor near 1, applied over and
+  // over, would be off by its rounding times the chunks that a head remembers: what the
+  // factors so far are off by (relatively) is kept, and each makes up for it.
+  const Decay full = split_decay(decay_pow(lg, kC));
+  const Decay last = split_decay(decay_pow(lg, tokens - (nch - 1) * kC));
+  const float inv_full = full.hi > 1e-30f ? 1.f / full.hi : 0.f;
+  float owed = 0.f;
+
+  // ---- the state: s[dt][nt][i] is row d = 16 dt + 4 g4 + i, column `col(nt)`; two tiles
+  // of columns interleave by fours, so that a lane's outputs are eight in a row
+  const int col0 = sl * SL + wave * 16 * NT;
+  auto col = [&](int nt) { return col0 + (NT == 2 ? 8 * a4 + 4 * nt + c4 : r); };
+  f32x4_t s[DT][NT];
   const int64_t bgh = (int64_t)b * GH + gh, sz = (int64_t)D * E;
   // by buffer accesses, which the hardware checks against the state's end: rows past D
   // and columns past E read as zeros and are not written
   const uint32_t sbytes = (uint32_t)(D * E * 4);
-  const uint32_t sbase = ec < E ? (uint32_t)(4 * g4 * E + ec) * 4 : 1u << 30;
-  auto read_state = [&](const float* from, f32x4_t (&x)[DT]) {
+  auto at_state = [&](int dt, int nt, int i) {
+    return (col(nt) < E ? (uint32_t)(4 * g4 * E + col(nt)) * 4 : 1u << 30) +
+           (uint32_t)((16 * dt + i) * E) * 4;
+  };
+  auto read_state = [&](const float* from, f32x4_t (&x)[DT][NT]) {
     const rsrc_t rs = make_rsrc(from, sbytes);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[dt][i] = __uint_as_float(buf_load4(rs, sbase + (uint32_t)((16 * dt + i) * E) * 4));
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[dt][nt][i] = __uint_as_float(buf_load4(rs, at_state(dt, nt, i)));
   };
   auto write_state = [&](float* to) {
     const rsrc_t rs = make_rsrc(to, sbytes);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[dt][i]), rs,
-                                              sbase + (uint32_t)((16 * dt + i) * E) * 4, 0, 0);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[dt][nt][i]), rs,
+                                                at_state(dt, nt, i), 0, 0);
   };
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) s[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) s[dt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   if (p.nseg == 1 || (ONLY_STATE && seg == 0)) {
     if (p.state) read_state(p.state + bgh * sz, s);
     // (state_out may be state: the first segment reads a copy)
@@ -241,117 +257,155 @@ __global__ void __launch_bounds__(64 * W, 1) linear_chunk_kernel(LinearParams p)
     for (int u = seg == 0 ? 0 : 1; u <= seg; ++u) {
       const float w = (float)exp((double)(seg - u) * (double)seglen *
                                  (double)(lg < -1e30f ? -1e30f : lg));
-      f32x4_t x[DT];
+      f32x4_t x[DT][NT];
       read_state(p.ws + (bgh * p.nseg + u) * sz, x);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) s[dt] += x[dt] * w;
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[dt][nt] += x[dt][nt] * w;
     }
   }
 
-  // ---- factors, the same for every whole chunk
+  // ---- factors, the same for every whole chunk.  An operand's eight tokens of lane group
+  // g4: 4 g4 + 0..3 and 16 + 4 g4 + 0..3
   __syncthreads();          // (s_pow)
-  float w[kM][8], rise[kIT];
+  auto token = [&](int x) { return 16 * (x >> 2) + 4 * g4 + (x & 3); };
+  float w[8], rise[kIT];
 #pragma unroll
-  for (int m = 0; m < kM; ++m)
-#pragma unroll
-    for (int x = 0; x < 8; ++x) w[m][x] = s_pow[kC - 1 - (32 * m + 16 * (x >> 2) + 4 * g4 + (x & 3))];
+  for (int x = 0; x < 8; ++x) w[x] = s_pow[kC - 1 - token(x)];
 #pragma unroll
   for (int it = 0; it < kIT; ++it) rise[it] = p.scale * s_pow[16 * it + r + 1];
-  // this wave's part of P: queries 16 pit .., key pairs pm0 .. pm0 + MPW - 1
-  const int pit = wave & 3, pm0 = W == 8 ? wave >> 2 : 0;
-  float pf_fac[2 * MPW][4];
+  // This wave's part of P^T: of a tile of queries, the half of 16 tokens (a wave each), in
+  // f16 both (twice: both halves share what they are scaled by).
+  const int pit = F16 ? wave & 1 : wave >> 1, pt = F16 ? 0 : wave & 1;
+  constexpr int PT = F16 ? 2 : 1;
+  float pf_fac[4 * PT];
 #pragma unroll
-  for (int t = 0; t < 2 * MPW; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int lag = 16 * pit + r - (16 * (2 * pm0 + t) + 4 * g4 + e);
-      pf_fac[t][e] = lag >= 0 ? p.scale * s_pow[lag] : -1.f;    // -1: not seen
-    }
-  const bool stores = !ONLY_STATE && col0 < E;
+  for (int x = 0; x < 4 * PT; ++x) {
+    const int lag = 16 * (pit - pt) + r - token(x);
+    pf_fac[x] = lag >= 0 ? p.scale * s_pow[lag] : -1.f;       // -1: not seen
+  }
   const char* const ob = reinterpret_cast<const char*>(p.out + (tok0 * GH + gh) * E + col0);
-  const int64_t ooff = (int64_t)r * GH * E * 2 + 8 * g4;
+  const int64_t ooff = (int64_t)r * GH * E * 2 + 8 * NT * g4;
+  const bool stores = !ONLY_STATE && col0 < E;
   // stores of a chunk's rows, all of which a whole chunk issues
   constexpr int STORES = kIT;
 
+  // rows 16 t + r of q or k, elements d = 32 ks + 4 g4 .. and 32 ks + 16 + 4 g4 ..
+  auto row_op = [&](const lds_char_t* base, int t, int ks) {
+    const int row = 16 * t + r, sw = row_swz<DK>(row);
+    const lds_char_t* at = base + row * KROW + (g4 & 1) * 8;
+    typedef __attribute__((address_space(3))) u32x2_t lds_u32x2;
+    const u32x2_t lo = *reinterpret_cast<const lds_u32x2*>(at + ((4 * ks + (g4 >> 1)) ^ sw) * 16);
+    const u32x2_t hi =
+        *reinterpret_cast<const lds_u32x2*>(at + ((4 * ks + 2 + (g4 >> 1)) ^ sw) * 16);
+    return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+  };
+  // sixteen columns of K or V, transposed; chunk and half: where this lane's four of
+  // them lie in a row
+  auto col_op = [&](const lds_char_t* base, auto n, int chunk, int half) {
+    constexpr int N = decltype(n)::value;
+    const int row = 4 * g4 + a4;
+    const lds_char_t* at = base + row * (N * 2) + (chunk ^ row_swz<N>(row)) * 16 + half * 8;
+    const u32x2_t lo = lds_read_tr16(at);
+    const u32x2_t hi = lds_read_tr16(at + 16 * (N * 2));    // (the same swizzle)
+    return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+  };
+
+  // P^T of the chunk in a stage: its products over d = 32 ks .., and, of their sums, the
+  // operands that every wave reads, into s_p[to]
+  auto p_step = [&](const lds_char_t* st, int ks, f32x4_t (&x)[PT]) {
+    const u32x4_t q = row_op(st, pit, ks);
+#pragma unroll
+    for (int t = 0; t < PT; ++t) x[t] = mfma16t<F16>(row_op(st + Q_BYTES, pt + t, ks), q, x[t]);
+  };
+  auto p_store = [&](f32x4_t (&x)[PT], int to) {
+#pragma unroll
+    for (int t = 0; t < PT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float f = pf_fac[4 * t + e];
+        x[t][e] = f >= 0.f ? x[t][e] * f : 0.f;
+      }
+    if constexpr (F16) {
+      float mx = 0.f;
+#pragma unroll
+      for (int t = 0; t < PT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, finite_abs(x[t][e]));
+      const float sc = f16_scale(mx);
+#pragma unroll
+      for (int t = 0; t < PT; ++t) x[t] *= sc;
+      if (lane == 0) s_ps[to][pit] = sc;
+    }
+#pragma unroll
+    for (int t = 0; t < PT; ++t)
+      reinterpret_cast<u32x2_t*>(&s_p[(to * kIT + pit) * 64 + lane])[pt + t] =
+          u32x2_t{pack2<F16>(x[t][0], x[t][1]), pack2<F16>(x[t][2], x[t][3])};
+  };
+  // One barrier to a chunk: its P^T was built beside the chunk before, whose copies and
+  // its own had landed by then.
+  if constexpr (!ONLY_STATE) {
+    if (nch > 0) {
+      LOOM_WAIT_VMCNT(0);
+      barrier_nofence();
+      f32x4_t x[PT] = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) p_step((lds_char_t*)smem, ks, x);
+      p_store(x, 0);
+    }
+  }
+  int stage = 0;
   for (int ci = 0; ci < nch; ++ci) {
-    char* const st = smem + (ci & 1) * STAGE;
+    char* const st = smem + stage * STAGE;
     lds_char_t* const lq = (lds_char_t*)st;
     lds_char_t* const lk = (lds_char_t*)(st + Q_BYTES);
     lds_char_t* const lv = (lds_char_t*)(st + Q_BYTES + K_BYTES);
     const int left = tokens - ci * kC;
     lds_order();
-    // the copies of this chunk; the stores of the one before are younger
+    // the copies of the next chunk; the stores of the one before are younger
     if (stores && ci > 0) LOOM_WAIT_VMCNT(STORES);
     else LOOM_WAIT_VMCNT(0);
     LOOM_WAIT_LGKM0();
     barrier_nofence();
-    if (ci + 1 < nch) issue(~ci & 1, ci + 1);
-
-    // rows 16 t + r of q or k, elements d = 32 ks + 4 g4 .. and 32 ks + 16 + 4 g4 ..
-    auto row_op = [&](const lds_char_t* base, int t, int ks) {
-      const int row = 16 * t + r, sw = row_swz<DK>(row);
-      const lds_char_t* at = base + row * KROW + (g4 & 1) * 8;
-      typedef __attribute__((address_space(3))) u32x2_t lds_u32x2;
-      const u32x2_t lo = *reinterpret_cast<const lds_u32x2*>(at + ((4 * ks + (g4 >> 1)) ^ sw) * 16);
-      const u32x2_t hi =
-          *reinterpret_cast<const lds_u32x2*>(at + ((4 * ks + 2 + (g4 >> 1)) ^ sw) * 16);
-      return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
-    };
-    // column tile x of K^T or V^T, tokens 32 m + 4 g4 .. and 32 m + 16 + 4 g4 ..
-    auto col_op = [&](const lds_char_t* base, auto n, int m, int x) {
-      constexpr int N = decltype(n)::value;
-      const int row = 32 * m + 4 * g4 + a4;
-      const lds_char_t* at =
-          base + row * (N * 2) + ((2 * x + (c4 >> 1)) ^ row_swz<N>(row)) * 16 + (c4 & 1) * 8;
-      const u32x2_t lo = lds_read_tr16(at);
-      const u32x2_t hi = lds_read_tr16(at + 16 * (N * 2));    // (the same swizzle)
-      return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
-    };
-
-    if constexpr (!ONLY_STATE) {
-      // ---- this wave's part of P^T, as the operands that every wave reads
-      u32x4_t qf[KS];
+    if (ci + 2 < nch) issue(stage == 0 ? 2 : stage - 1, ci + 2);
+    stage = stage == 2 ? 0 : stage + 1;
+    float a = __builtin_fmaf(full.hi, owed, full.hi);
+    owed = __builtin_fmaf((full.hi - a) + full.lo, inv_full, owed);
+    if (left < kC) {          // the last, partial chunk
+      a = __builtin_fmaf(last.hi, owed, last.hi);
+      const int j0 = fresh(4 * g4);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qf[ks] = row_op(lq, pit, ks);
-#pragma unroll
-      for (int mm = 0; mm < MPW; ++mm) {
-        const int m = pm0 + mm;
-        if (2 * m > pit) continue;              // wave-uniform
-        f32x4_t x[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          x[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-          if (2 * m + t <= pit) {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-              x[t] = mfma16t<F16>(row_op(lk, 2 * m + t, ks), qf[ks], x[t]);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float f = pf_fac[2 * mm + t][e];
-            x[t][e] = f >= 0.f ? x[t][e] * f : 0.f;
-          }
-        }
-        if constexpr (F16) {
-          float mx = 0.f;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, finite_abs(x[t][e]));
-          const float sc = f16_scale(mx);
-#pragma unroll
-          for (int t = 0; t < 2; ++t) x[t] *= sc;
-          if (lane == 0) s_ps[pit * kM + m] = sc;
-        }
-        s_p[(pit * kM + m) * 64 + lane] =
-            u32x4_t{pack2<F16>(x[0][0], x[0][1]), pack2<F16>(x[0][2], x[0][3]),
-                    pack2<F16>(x[1][0], x[1][1]), pack2<F16>(x[1][2], x[1][3])};
-      }
+      for (int x = 0; x < 8; ++x) w[x] = s_pow[max(0, left - 1 - (16 * (x >> 2) + j0 + (x & 3)))];
     }
 
-    __builtin_amdgcn_sched_barrier(0);
-    // ---- S^T Q^T of the state before the chunk, times scale a^(i+1)
-    f32x4_t o[kIT];
+    // ---- v as operands, and a^(C-1-j) v as sums of 16-bit numbers
+    u32x4_t vf[NT], vt[TERMS][NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      vf[nt] = col_op(lv, VC{}, NT == 2 ? wave * 4 + c4 : wave * 2 + (c4 >> 1),
+                      NT == 2 ? nt : c4 & 1);
+    // f16: the second number 2^11 times larger, in sums of its own, so that it keeps
+    // its bits
+    constexpr float kLow = F16 ? 2048.f : 1.f;
+    auto weigh = [&](int nt, int x) {
+      float y0 = lo16<F16>(vf[nt][x]) * w[2 * x], y1 = hi16<F16>(vf[nt][x]) * w[2 * x + 1];
+#pragma unroll
+      for (int z = 0; z < TERMS; ++z) {
+        const uint32_t y = pack2<F16>(y0, y1);
+        vt[z][nt][x] = y;
+        if (z + 1 < TERMS) {
+          y0 = (y0 - lo16<F16>(y)) * kLow;
+          y1 = (y1 - hi16<F16>(y)) * kLow;
+        }
+      }
+    };
+
+    // ---- S^T Q^T of the state before the chunk, times scale a^(i+1); the next chunk's P^T
+    // (behind the last, of what lies there: never read).  Products that wait for each
+    // other are kept apart, and v's factors are worked out between them: a chain of
+    // products that follow each other directly took twice as long.
+    f32x4_t o[kIT][NT];
     if constexpr (!ONLY_STATE) {
       float sc = 1.f;
       if constexpr (F16) {
@@ -359,131 +413,136 @@ __global__ void __launch_bounds__(64 * W, 1) linear_chunk_kernel(LinearParams p)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, finite_abs(s[dt][i]));
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, finite_abs(s[dt][nt][i]));
         sc = f16_scale(mx);
       }
-      u32x4_t sp[KS];
+      const float back = F16 ? 1.f / sc : 1.f;
+      const lds_char_t* const next = (lds_char_t*)(smem + stage * STAGE);
+      f32x4_t px[PT] = {};
+#pragma unroll
+      for (int it = 0; it < kIT; ++it)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[it][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        f32x4_t x = s[2 * ks], y = s[2 * ks + 1];
-        if constexpr (F16) {
-          x *= sc;
-          y *= sc;
+        u32x4_t q[kIT];
+#pragma unroll
+        for (int it = 0; it < kIT; ++it) q[it] = row_op(lq, it, ks);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          f32x4_t x = s[2 * ks][nt], y = s[2 * ks + 1][nt];
+          if constexpr (F16) {
+            x *= sc;
+            y *= sc;
+          }
+          const u32x4_t sp = u32x4_t{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]),
+                                     pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3])};
+#pragma unroll
+          for (int it = 0; it < kIT; ++it) o[it][nt] = mfma16t<F16>(sp, q[it], o[it][nt]);
         }
-        sp[ks] = u32x4_t{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(y[0], y[1]),
-                         pack2<F16>(y[2], y[3])};
-      }
-      const float back = F16 ? 1.f / sc : 1.f;
+        p_step(next, ks, px);
+        // (all of v's 4 NT pieces over the steps)
 #pragma unroll
-      for (int it = 0; it < kIT; ++it) {
-        o[it] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) o[it] = mfma16t<F16>(sp[ks], row_op(lq, it, ks), o[it]);
-        o[it] *= rise[it] * back;
-        // (two tiles' reads at a time: all at once would not leave registers enough)
-        if (it & 1) __builtin_amdgcn_sched_barrier(0);
+        for (int x = 4 * NT * ks / KS; x < 4 * NT * (ks + 1) / KS; ++x) weigh(x / 4, x % 4);
       }
+      p_store(px, ~ci & 1);
+#pragma unroll
+      for (int it = 0; it < kIT; ++it)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[it][nt] *= rise[it] * back;
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4 * NT; ++x) weigh(x / 4, x % 4);
     }
 
-    __builtin_amdgcn_sched_barrier(0);
-    // ---- the state behind the chunk
-    u32x4_t vf[kM], vt[TERMS][kM];
+    // ---- the state behind the chunk, row tiles in pairs
 #pragma unroll
-    for (int m = 0; m < kM; ++m) vf[m] = col_op(lv, VC{}, m, wave);
-    Decay a = full;
-    if (left < kC) {          // the last, partial chunk
-      a = last;
-      const int j0 = fresh(4 * g4);
+    for (int d2 = 0; d2 < DT; d2 += 2) {
+      u32x4_t kt[2];
+      f32x4_t x[2][NT], y[2][NT];
 #pragma unroll
-      for (int m = 0; m < kM; ++m)
+      for (int u = 0; u < 2; ++u) {
+        kt[u] = col_op(lk, QK{}, 2 * (d2 + u) + (c4 >> 1), c4 & 1);
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          w[m][x] = s_pow[max(0, left - 1 - (32 * m + 16 * (x >> 2) + j0 + (x & 3)))];
-    }
-    // f16: the second number 2^11 times larger, in sums of its own, so that it keeps
-    // its bits
-    constexpr float kLow = F16 ? 2048.f : 1.f;
+        for (int nt = 0; nt < NT; ++nt) x[u][nt] = y[u][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
 #pragma unroll
-    for (int m = 0; m < kM; ++m)
+      for (int z = TERMS - 1; z >= 0; --z)      // the small ones first
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float y0 = lo16<F16>(vf[m][x]) * w[m][2 * x], y1 = hi16<F16>(vf[m][x]) * w[m][2 * x + 1];
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int z = 0; z < TERMS; ++z) {
-          const uint32_t y = pack2<F16>(y0, y1);
-          vt[z][m][x] = y;
-          if (z + 1 < TERMS) {
-            y0 = (y0 - lo16<F16>(y)) * kLow;
-            y1 = (y1 - hi16<F16>(y)) * kLow;
+          for (int nt = 0; nt < NT; ++nt) {
+            f32x4_t& t = F16 && z == 1 ? y[u][nt] : x[u][nt];
+            t = mfma16t<F16>(kt[u], vt[z][nt], t);
           }
-        }
-      }
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      f32x4_t x = f32x4_t{0.f, 0.f, 0.f, 0.f}, y = x;
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int m = 0; m < kM; ++m) {
-        const u32x4_t kt = col_op(lk, QK{}, m, dt);
-        if constexpr (F16) {
-          x = mfma16t<F16>(kt, vt[0][m], x);
-          y = mfma16t<F16>(kt, vt[1][m], y);
-        } else {              // (the small ones in sums of their own: half the chain)
-          x = mfma16t<F16>(kt, vt[0][m], x);
-          y = mfma16t<F16>(kt, vt[TERMS - 1][m], y);
-          y = mfma16t<F16>(kt, vt[1][m], y);
-        }
-      }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float z = F16 ? __builtin_fmaf(y[i], 1.f / kLow, x[i]) : x[i] + y[i];
-        s[dt][i] = __builtin_fmaf(s[dt][i], a.hi, __builtin_fmaf(s[dt][i], a.lo, z));
-      }
-      if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < 4; ++i) {
+            const float z =
+                F16 ? __builtin_fmaf(y[u][nt][i], 1.f / kLow, x[u][nt][i]) : x[u][nt][i];
+            s[d2 + u][nt][i] = __builtin_fmaf(s[d2 + u][nt][i], a, z);
+          }
     }
 
     if constexpr (!ONLY_STATE) {
-      __builtin_amdgcn_sched_barrier(0);
       // ---- V^T P^T of the chunk's own tokens
       // A token whose v is not finite makes its columns of the state so: then every
       // query takes its own product, tokens behind it as zeros, since a weight of zero
       // times an infinity would reach the queries ahead of them.
-      const bool alone = __builtin_amdgcn_ballot_w64(!(fabsf(s[0][0]) < INFINITY)) != 0;
-      LOOM_WAIT_LGKM0();
-      barrier_nofence();
+      bool odd = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) odd |= !(fabsf(s[0][nt][0]) < INFINITY);
+      const bool alone = __builtin_amdgcn_ballot_w64(odd) != 0;
 #pragma unroll
       for (int it = 0; it < kIT; ++it) {
+        const u32x4_t pf = s_p[((ci & 1) * kIT + it) * 64 + lane];
+        const float ps = F16 ? s_ps[ci & 1][it] : 1.f;
+        if constexpr (F16) {
 #pragma unroll
-        for (int m = 0; m <= it / 2; ++m) {
-          const u32x4_t pf = s_p[(it * kM + m) * 64 + lane];
-          float ps = 1.f;
-          if constexpr (F16) {
-            ps = s_ps[it * kM + m];
-            o[it] *= ps;
-          }
-          if (!alone || 32 * m + 31 <= 16 * it) {
-            o[it] = mfma16t<F16>(vf[m], pf, o[it]);
-          } else {
-            const int j0 = fresh(4 * g4);
+          for (int nt = 0; nt < NT; ++nt) o[it][nt] *= ps;
+        }
+        if (!alone) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) o[it][nt] = mfma16t<F16>(vf[nt], pf, o[it][nt]);
+        } else {
+          const int j0 = fresh(4 * g4);
 #pragma unroll 1
-            for (int x = 0; x < 16; ++x) {
-              u32x4_t keep;
+          for (int x = 0; x < 16; ++x) {
+            u32x4_t keep;
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const int j = 32 * m + 16 * (y >> 1) + j0 + 2 * (y & 1), i = 16 * it + x;
-                keep[y] = (j <= i ? 0xffffu : 0u) | (j + 1 <= i ? 0xffff0000u : 0u);
-              }
-              const f32x4_t z = mfma16t<F16>(vf[m] & keep, pf, o[it]);
-              if (r == x) o[it] = z;
+            for (int y = 0; y < 4; ++y) {
+              const int j = 16 * (y >> 1) + j0 + 2 * (y & 1), i = 16 * it + x;
+              keep[y] = (j <= i ? 0xffffu : 0u) | (j + 1 <= i ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const f32x4_t z = mfma16t<F16>(vf[nt] & keep, pf, o[it][nt]);
+              if (r == x) o[it][nt] = z;
             }
           }
-          if constexpr (F16) o[it] *= 1.f / ps;
         }
-        // ---- o[it][e] is token 16 it + r, column col0 + 4 g4 + e
-        const char* to = uniform(ob + (int64_t)(ci * kC + 16 * it) * GH * E * 2);
-        if (16 * it + r < left && col0 + 4 * g4 < E)
-          *reinterpret_cast<u32x2_t*>(const_cast<char*>(to) + ooff) =
-              u32x2_t{pack2<F16>(o[it][0], o[it][1]), pack2<F16>(o[it][2], o[it][3])};
+        if constexpr (F16) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) o[it][nt] *= 1.f / ps;
+        }
+        // ---- o[it][nt][e] is token 16 it + r, column col0 + 8 g4 + 4 nt + e (NT 2) or
+        // col0 + 4 g4 + e
+        char* to = const_cast<char*>(uniform(ob + (int64_t)(ci * kC + 16 * it) * GH * E * 2)) + ooff;
+        if (16 * it + r < left && col0 + 4 * NT * g4 < E) {
+          const u32x2_t x = u32x2_t{pack2<F16>(o[it][0][0], o[it][0][1]),
+                                    pack2<F16>(o[it][0][2], o[it][0][3])};
+          if constexpr (NT == 2)
+            *reinterpret_cast<u32x4_t*>(to) =
+                u32x4_t{x[0], x[1], pack2<F16>(o[it][NT - 1][0], o[it][NT - 1][1]),
+                        pack2<F16>(o[it][NT - 1][2], o[it][NT - 1][3])};
+          else
+            *reinterpret_cast<u32x2_t*>(to) = x;
+        }
       }
     }
   }
@@ -560,18 +619,17 @@ __global__ void __launch_bounds__(256) linear_step_kernel(LinearParams p, int L)
 
 // The launch's shape, from the extents alone.
 struct Shape {
-  int waves, nsl, nseg, cps;
+  int nt, nsl, nseg, cps;
 };
 Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t E, int64_t T) {
   Shape s{};
-  // 128 columns to a workgroup; 64 of states that are no wider, and past D 128, where the
-  // stages of 128 do not fit
-  s.waves = D > 128 || E <= 64 ? 4 : 8;
-  s.nsl = (int)cdiv64(E, 16 * s.waves);
+  // 128 columns to a workgroup; 64 of states that are no wider, and past D 128, whose
+  // states of 128 columns would not leave registers enough
+  s.nt = D > 128 || E <= 64 ? 1 : 2;
+  s.nsl = (int)cdiv64(E, 64 * s.nt);
   const int64_t wgs = B * G * H * s.nsl, chunks = cdiv64(T, kC);
-  // workgroups that run at once
-  const int64_t slots = D > 64 ? 256 : 512;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({slots / wgs, chunks / 4, 64}));
+  // two workgroups run on a CU at once
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({512 / wgs, chunks / 8, 64}));
   s.cps = (int)cdiv64(chunks, want);
   s.nseg = (int)cdiv64(chunks, s.cps);
   return s;
@@ -580,16 +638,16 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t E, int64_t T)
 template <bool F16, bool ONLY_STATE>
 void launch_chunks(const LinearParams& p, const Shape& s, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)p.B * p.G * p.H * s.nsl * (s.nseg - (ONLY_STATE ? 1 : 0)))),
-      block(64 * s.waves);
+      block(256);
   auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, st, p); };
   // the kernel built for 64, 128 or 256 (the next one up) runs any narrower key dim
-  if (p.D > 128) launch(linear_chunk_kernel<256, 4, F16, ONLY_STATE>);
+  if (p.D > 128) launch(linear_chunk_kernel<256, 1, F16, ONLY_STATE>);
   else if (p.D > 64) {
-    if (s.waves == 4) launch(linear_chunk_kernel<128, 4, F16, ONLY_STATE>);
-    else launch(linear_chunk_kernel<128, 8, F16, ONLY_STATE>);
+    if (s.nt == 1) launch(linear_chunk_kernel<128, 1, F16, ONLY_STATE>);
+    else launch(linear_chunk_kernel<128, 2, F16, ONLY_STATE>);
   } else {
-    if (s.waves == 4) launch(linear_chunk_kernel<64, 4, F16, ONLY_STATE>);
-    else launch(linear_chunk_kernel<64, 8, F16, ONLY_STATE>);
+    if (s.nt == 1) launch(linear_chunk_kernel<64, 1, F16, ONLY_STATE>);
+    else launch(linear_chunk_kernel<64, 2, F16, ONLY_STATE>);
   }
 }
 
