@@ -27,10 +27,11 @@ struct LinearParams {
   const int* counts;
   uint16_t* out;
   float* state_out;
-  float* ws;             // [B G H, nseg, D, E]: what a segment starts from
+  float* ws;             // [B G H, (nseg - 1) sub + 1, D, E]: the states of stretches
   int B, G, H, D, E, T;
   int nsl;               // slices of E
-  int nseg, cps;         // segments of a prompt, chunks to one
+  int nseg;              // segments of a prompt
+  int sub, cps;          // stretches of a segment, chunks to one
   float scale;
 };
 
@@ -85,35 +86,37 @@ LOOM_DEV const char* uniform(const char* p) {
       (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
 }
 
-// Chunked form.  A workgroup of four waves walks the chunks of 32 tokens of one (b, g, h)
-// and 64 NT columns of E in order, each wave holding the state's D x 16 NT columns in the
+// Chunked form.  A workgroup of W waves walks the chunks of 32 tokens of one (b, g, h)
+// and 16 W columns of E in order, each wave holding the state's D x 16 columns in the
 // accumulators of its MFMAs, fp32.  For a chunk of tokens 0 .. C-1 and the state S before
 // it:
 //   P_ij = scale a^(i-j) q_i.k_j (j <= i),
 //   out_i = sum_j P_ij v_j + scale a^(i+1) S^T q_i,
 //   S' = a^C S + sum_j k_j (a^(C-1-j) v_j)^T.
 // The MFMAs compute transposed tiles, S^T[e, d] . Q^T[d, i] and V^T[e, j] . P^T[j, i], so
-// that a wave's state feeds the first product from its own accumulators (packed to 16
-// bits: lane group g holds rows d = 16 t + 4 g + 0..3, and q's pieces are read in that
-// order), and P^T is built from the accumulators of K Q^T, a quarter to a wave, shared
-// through LDS.
+// that a wave's state feeds the first product from its own accumulators: the state's row
+// tiles are taken so that lane group g holds d = 32 t + 8 g + 0..7 in a pair of them, the
+// 16 bytes of q that it reads.  P^T is built from the accumulators of K Q^T, one chunk
+// ahead, by four waves (in f16 two), and shared through LDS: one barrier to a chunk.
 // Rounding: S and P to 16 bits as operands, each once; a^(C-1-j) v_j as a sum of three
 // bf16 or two f16 numbers, so that the state keeps fp32's accuracy.  f16 operands are
 // scaled by powers of two where they leave its range.
 // ONLY_STATE: a segment's own state from zero (the first's from the initial state), which
 // later segments start from.
-template <int DK, int NT, bool F16, bool ONLY_STATE>
-__global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
-  constexpr int W = 4, SL = 16 * NT * W;        // columns of a workgroup
+template <int DK, int W, bool F16, bool ONLY_STATE>
+__global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
+    linear_chunk_kernel(LinearParams p) {
+  constexpr int SL = 16 * W;                    // columns of a workgroup
   constexpr int KROW = DK * 2, VROW = SL * 2;
   constexpr int Q_BYTES = ONLY_STATE ? 0 : kC * KROW, K_BYTES = kC * KROW, V_BYTES = kC * VROW;
   constexpr int STAGE = Q_BYTES + K_BYTES + V_BYTES;
-  constexpr int QK_INSTR = K_BYTES / 1024 / W, V_INSTR = V_BYTES / 1024 / W;
-  static_assert(QK_INSTR >= 1 && V_INSTR >= 1, "every wave issues copies");
+  // stages: this chunk, the next (whose P^T is built) and the one on its way (a fourth
+  // took as long)
+  constexpr int NS = 3;
   constexpr int KS = DK / 32, DT = DK / 16;
   constexpr int TERMS = F16 ? 2 : 3;            // 16-bit numbers that hold a^(C-1-j) v_j
-  static_assert(kC == 32 && (NT == 1 || NT == 2), "one step of the MFMA over a chunk's tokens");
-  constexpr int NS = 3;                         // stages: two chunks on their way
+  static_assert(kC == 32, "one step of the MFMA over a chunk's tokens");
+  static_assert(V_BYTES / W == 1024, "a copy of v to each wave");
   __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
   __shared__ __attribute__((aligned(16))) u32x4_t s_p[ONLY_STATE ? 1 : 2 * kIT * 64];
   __shared__ float s_pow[kC + 1];
@@ -125,7 +128,7 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
   const int a4 = r >> 2, c4 = r & 3;
   // (b, g) outermost, then segments, heads, slices: those that share k and v side by side
   const int nsl = p.nsl, H = p.H, D = p.D, E = p.E, GH = p.G * H;
-  const int nseg = ONLY_STATE ? p.nseg - 1 : p.nseg;
+  const int nseg = ONLY_STATE ? (p.nseg - 1) * p.sub : p.nseg;
   int id = xcd_remap(blockIdx.x, gridDim.x);
   const int sl = id % nsl;
   id /= nsl;
@@ -135,15 +138,17 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
   const int b = bg / p.G, g = bg - b * p.G, gh = g * H + h;
   const int c =
       __builtin_amdgcn_readfirstlane(p.counts ? min(max(p.counts[b], 0), p.T) : p.T);
-  const int64_t seglen = (int64_t)p.cps * kC;
-  const int t0 = (int)(seg * seglen);           // (T < 2^29 and a segment within T)
-  // a segment's own state is asked for by those behind it only
-  const bool wanted = !ONLY_STATE || (seg + 1) * seglen < c;
+  // tokens of a segment, and of the stretches whose states the first launch leaves
+  const int64_t sublen = (int64_t)p.cps * kC, seglen = sublen * p.sub;
+  const int64_t mylen = ONLY_STATE ? sublen : seglen;
+  const int t0 = (int)(seg * mylen);            // (T < 2^29 and a segment within T)
+  // the state of a stretch is asked for by the segments behind it only
+  const bool wanted = !ONLY_STATE || (seg / p.sub + 1) * seglen < c;
   if (seg > 0 && (!wanted || t0 >= c)) return;
-  const int tokens = wanted ? (int)min((int64_t)(c - t0), seglen) : 0;
+  const int tokens = wanted ? (int)min((int64_t)(c - t0), mylen) : 0;
   const int nch = (tokens + kC - 1) / kC;
 
-  // ---- copies of chunk ci into stage s: rows past the sequence and chunks past D or E
+  // ---- copies of chunk ci into a stage: rows past the sequence and chunks past D or E
   // from zeros.  A whole chunk of whole rows takes each copy as the chunk's scalar base
   // plus this lane's offset, computed once (fast: all offsets fit 32 bits).
   const int64_t tok0 = (int64_t)b * p.T + t0;
@@ -154,12 +159,15 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
   const uint32_t qs = (uint32_t)(GH * D * 2), ks_ = (uint32_t)(p.G * D * 2),
                  vs = (uint32_t)(p.G * E * 2);
   const bool fast = D == DK && sl * SL + SL <= E && qs < (1u << 26) && vs < (1u << 26);
-  uint32_t qoff[QK_INSTR], koff[QK_INSTR], voff[V_INSTR];
+  // copies of a row of N elements times 32 tokens, 1 KB each, which the waves share (the
+  // last ones of fewer than W go to some of them)
+  constexpr int QK_ALL = K_BYTES / 1024, QK_INSTR = (QK_ALL + W - 1) / W;
+  uint32_t qoff[QK_INSTR], koff[QK_INSTR], voff[1];
   auto offsets = [&](auto& off, uint32_t stride, auto n) {
-    constexpr int N = decltype(n)::value, INSTR = kC * N * 2 / 1024 / W;
+    constexpr int N = decltype(n)::value, ALL = kC * N * 2 / 1024, INSTR = (ALL + W - 1) / W;
 #pragma unroll
     for (int i = 0; i < INSTR; ++i) {
-      const int e = (wave * INSTR + i) * 64 + lane, row = e / (N / 8);
+      const int e = (wave + W * i) * 64 + lane, row = e / (N / 8);
       off[i] = row * stride + ((e % (N / 8)) ^ row_swz<N>(row)) * 16;
     }
   };
@@ -173,32 +181,33 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
     const uint32_t base = lds_addr((lds_char_t*)(smem + s * STAGE));
     auto rows = [&](const uint16_t* from, uint32_t stride, int valid, auto& off, auto n,
                     uint32_t lds) {
-      constexpr int N = decltype(n)::value, INSTR = kC * N * 2 / 1024 / W;
+      constexpr int N = decltype(n)::value, ALL = kC * N * 2 / 1024, INSTR = (ALL + W - 1) / W;
       const char* at = uniform((const char*)from + (int64_t)ci * kC * stride);
-      if (fast && left >= kC) {
-#pragma unroll
-        for (int i = 0; i < INSTR; ++i)
-          dma_load16_s(off[i], at,
-                       __builtin_amdgcn_readfirstlane(lds + (wave * INSTR + i) * 1024));
-        return;
-      }
+      const bool whole = fast && left >= kC;
       const int ln = fresh(lane);
 #pragma unroll
       for (int i = 0; i < INSTR; ++i) {
-        const int j = wave * INSTR + i;
-        const int e = j * 64 + ln, row = e / (N / 8), ch = (e % (N / 8)) ^ row_swz<N>(row);
-        const void* src = row < left && ch < valid
-                              ? (const void*)(at + (int64_t)row * stride + ch * 16)
-                              : (const void*)(loom_zero_kb + lane * 4);
-        dma_load16(src, __builtin_amdgcn_readfirstlane(lds + j * 1024));
+        const int j = wave + W * i;
+        if (ALL % W && j >= ALL) break;         // wave-uniform
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + j * 1024);
+        if (whole) {
+          dma_load16_s(off[i], at, to);
+        } else {
+          const int e = j * 64 + ln, row = e / (N / 8), ch = (e % (N / 8)) ^ row_swz<N>(row);
+          const void* src = row < left && ch < valid
+                                ? (const void*)(at + (int64_t)row * stride + ch * 16)
+                                : (const void*)(loom_zero_kb + lane * 4);
+          dma_load16(src, to);
+        }
       }
     };
     if constexpr (!ONLY_STATE) rows(qb, qs, D / 8, qoff, QK{}, base);
     rows(kb, ks_, D / 8, koff, QK{}, base + Q_BYTES);
     rows(vb, vs, (E - sl * SL) / 8, voff, VC{}, base + Q_BYTES + K_BYTES);
   };
-  if (nch > 0) issue(0, 0);
-  if (nch > 1) issue(1, 1);
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (i < nch) issue(i, i);
 
   const float lg = p.g[gh];
   if (tid <= kC) s_pow[tid] = (float)decay_pow(lg, tid);
@@ -210,59 +219,50 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
   const float inv_full = full.hi > 1e-30f ? 1.f / full.hi : 0.f;
   float owed = 0.f;
 
-  // ---- the state: s[dt][nt][i] is row d = 16 dt + 4 g4 + i, column `col(nt)`; two tiles
-  // of columns interleave by fours, so that a lane's outputs are eight in a row
-  const int col0 = sl * SL + wave * 16 * NT;
-  auto col = [&](int nt) { return col0 + (NT == 2 ? 8 * a4 + 4 * nt + c4 : r); };
-  f32x4_t s[DT][NT];
+  // ---- the state: s[dt][i] is row d = 32 (dt / 2) + 8 g4 + 4 (dt % 2) + i, column ec.  By
+  // buffer accesses, which the hardware checks against the state's end: rows past D and
+  // columns past E read as zeros and are not written.
+  const int col0 = sl * SL + wave * 16, ec = col0 + r;
+  f32x4_t s[DT];
   const int64_t bgh = (int64_t)b * GH + gh, sz = (int64_t)D * E;
-  // by buffer accesses, which the hardware checks against the state's end: rows past D
-  // and columns past E read as zeros and are not written
   const uint32_t sbytes = (uint32_t)(D * E * 4);
-  auto at_state = [&](int dt, int nt, int i) {
-    return (col(nt) < E ? (uint32_t)(4 * g4 * E + col(nt)) * 4 : 1u << 30) +
-           (uint32_t)((16 * dt + i) * E) * 4;
+  const uint32_t sbase = ec < E ? (uint32_t)(8 * g4 * E + ec) * 4 : 1u << 30;
+  auto at_state = [&](int dt, int i) {
+    return sbase + (uint32_t)((32 * (dt >> 1) + 4 * (dt & 1) + i) * E) * 4;
   };
-  auto read_state = [&](const float* from, f32x4_t (&x)[DT][NT]) {
+  auto read_state = [&](const float* from, f32x4_t (&x)[DT]) {
     const rsrc_t rs = make_rsrc(from, sbytes);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[dt][nt][i] = __uint_as_float(buf_load4(rs, at_state(dt, nt, i)));
+      for (int i = 0; i < 4; ++i) x[dt][i] = __uint_as_float(buf_load4(rs, at_state(dt, i)));
   };
   auto write_state = [&](float* to) {
     const rsrc_t rs = make_rsrc(to, sbytes);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[dt][nt][i]), rs,
-                                                at_state(dt, nt, i), 0, 0);
+      for (int i = 0; i < 4; ++i)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[dt][i]), rs, at_state(dt, i), 0, 0);
   };
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[dt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < DT; ++dt) s[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // the first launch's states: slot 0 the initial one (state_out may be state: the first
+  // segment reads this copy), slot u + 1 that of stretch u
+  const int64_t slots = (int64_t)(p.nseg - 1) * p.sub + 1;
   if (p.nseg == 1 || (ONLY_STATE && seg == 0)) {
     if (p.state) read_state(p.state + bgh * sz, s);
-    // (state_out may be state: the first segment reads a copy)
-    if constexpr (ONLY_STATE) write_state(p.ws + bgh * p.nseg * sz);
+    if constexpr (ONLY_STATE) write_state(p.ws + bgh * slots * sz);
   } else if constexpr (!ONLY_STATE) {
+    const int to = seg * p.sub;
 #pragma unroll 1
-    for (int u = seg == 0 ? 0 : 1; u <= seg; ++u) {
-      const float w = (float)exp((double)(seg - u) * (double)seglen *
+    for (int u = seg == 0 ? 0 : 1; u <= to; ++u) {
+      const float w = (float)exp((double)(to - u) * (double)sublen *
                                  (double)(lg < -1e30f ? -1e30f : lg));
-      f32x4_t x[DT][NT];
-      read_state(p.ws + (bgh * p.nseg + u) * sz, x);
+      f32x4_t x[DT];
+      read_state(p.ws + (bgh * slots + u) * sz, x);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[dt][nt] += x[dt][nt] * w;
+      for (int dt = 0; dt < DT; ++dt) s[dt] += x[dt] * w;
     }
   }
 
@@ -275,34 +275,33 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
   for (int x = 0; x < 8; ++x) w[x] = s_pow[kC - 1 - token(x)];
 #pragma unroll
   for (int it = 0; it < kIT; ++it) rise[it] = p.scale * s_pow[16 * it + r + 1];
-  // This wave's part of P^T: of a tile of queries, the half of 16 tokens (a wave each), in
-  // f16 both (twice: both halves share what they are scaled by).
-  const int pit = F16 ? wave & 1 : wave >> 1, pt = F16 ? 0 : wave & 1;
-  constexpr int PT = F16 ? 2 : 1;
+  // A wave's part of P^T: of a tile of queries, the half of 16 tokens, in f16 both (which
+  // share what they are scaled by).  Of 8 waves (in f16 4) they take turns.
+  const int pit = F16 ? wave & 1 : (wave >> 1) & 1, pt = F16 ? 0 : wave & 1;
+  constexpr int PT = F16 ? 2 : 1, TURNS = W * PT / 4;
+  const int turn = wave / (W / TURNS);
   float pf_fac[4 * PT];
+  bool seen[4 * PT];
 #pragma unroll
   for (int x = 0; x < 4 * PT; ++x) {
     const int lag = 16 * (pit - pt) + r - token(x);
-    pf_fac[x] = lag >= 0 ? p.scale * s_pow[lag] : -1.f;       // -1: not seen
+    seen[x] = lag >= 0;
+    pf_fac[x] = p.scale * s_pow[max(lag, 0)];
   }
   const char* const ob = reinterpret_cast<const char*>(p.out + (tok0 * GH + gh) * E + col0);
-  const int64_t ooff = (int64_t)r * GH * E * 2 + 8 * NT * g4;
+  const int64_t ooff = (int64_t)r * GH * E * 2 + 8 * g4;
   const bool stores = !ONLY_STATE && col0 < E;
   // stores of a chunk's rows, all of which a whole chunk issues
   constexpr int STORES = kIT;
 
-  // rows 16 t + r of q or k, elements d = 32 ks + 4 g4 .. and 32 ks + 16 + 4 g4 ..
+  // rows 16 t + r of q or k, elements d = 32 ks + 8 g4 .. + 7
   auto row_op = [&](const lds_char_t* base, int t, int ks) {
-    const int row = 16 * t + r, sw = row_swz<DK>(row);
-    const lds_char_t* at = base + row * KROW + (g4 & 1) * 8;
-    typedef __attribute__((address_space(3))) u32x2_t lds_u32x2;
-    const u32x2_t lo = *reinterpret_cast<const lds_u32x2*>(at + ((4 * ks + (g4 >> 1)) ^ sw) * 16);
-    const u32x2_t hi =
-        *reinterpret_cast<const lds_u32x2*>(at + ((4 * ks + 2 + (g4 >> 1)) ^ sw) * 16);
-    return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    const int row = 16 * t + r;
+    return *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
+        base + row * KROW + ((4 * ks + g4) ^ row_swz<DK>(row)) * 16);
   };
-  // sixteen columns of K or V, transposed; chunk and half: where this lane's four of
-  // them lie in a row
+  // sixteen columns of K or V, transposed; chunk and half: where this lane's four of them
+  // lie in a row
   auto col_op = [&](const lds_char_t* base, auto n, int chunk, int half) {
     constexpr int N = decltype(n)::value;
     const int row = 4 * g4 + a4;
@@ -311,21 +310,21 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
     const u32x2_t hi = lds_read_tr16(at + 16 * (N * 2));    // (the same swizzle)
     return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
   };
-
-  // P^T of the chunk in a stage: its products over d = 32 ks .., and, of their sums, the
-  // operands that every wave reads, into s_p[to]
-  auto p_step = [&](const lds_char_t* st, int ks, f32x4_t (&x)[PT]) {
-    const u32x4_t q = row_op(st, pit, ks);
+  // P^T of the chunk in a stage, as the operands that every wave reads, into s_p[to]
+  auto build_p = [&](const lds_char_t* st, int to) {
+    f32x4_t x[PT] = {};
 #pragma unroll
-    for (int t = 0; t < PT; ++t) x[t] = mfma16t<F16>(row_op(st + Q_BYTES, pt + t, ks), q, x[t]);
-  };
-  auto p_store = [&](f32x4_t (&x)[PT], int to) {
+    for (int ks = 0; ks < KS; ++ks) {
+      const u32x4_t q = row_op(st, pit, ks);
+#pragma unroll
+      for (int t = 0; t < PT; ++t) x[t] = mfma16t<F16>(row_op(st + Q_BYTES, pt + t, ks), q, x[t]);
+    }
 #pragma unroll
     for (int t = 0; t < PT; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float f = pf_fac[4 * t + e];
-        x[t][e] = f >= 0.f ? x[t][e] * f : 0.f;
+        const float y = x[t][e] * pf_fac[4 * t + e];
+        x[t][e] = seen[4 * t + e] ? y : 0.f;
       }
     if constexpr (F16) {
       float mx = 0.f;
@@ -343,16 +342,11 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
       reinterpret_cast<u32x2_t*>(&s_p[(to * kIT + pit) * 64 + lane])[pt + t] =
           u32x2_t{pack2<F16>(x[t][0], x[t][1]), pack2<F16>(x[t][2], x[t][3])};
   };
-  // One barrier to a chunk: its P^T was built beside the chunk before, whose copies and
-  // its own had landed by then.
   if constexpr (!ONLY_STATE) {
     if (nch > 0) {
       LOOM_WAIT_VMCNT(0);
       barrier_nofence();
-      f32x4_t x[PT] = {};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) p_step((lds_char_t*)smem, ks, x);
-      p_store(x, 0);
+      if (turn == 0) build_p((lds_char_t*)smem, 0);
     }
   }
   int stage = 0;
@@ -368,8 +362,8 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
     else LOOM_WAIT_VMCNT(0);
     LOOM_WAIT_LGKM0();
     barrier_nofence();
-    if (ci + 2 < nch) issue(stage == 0 ? 2 : stage - 1, ci + 2);
-    stage = stage == 2 ? 0 : stage + 1;
+    if (ci + NS - 1 < nch) issue(stage == 0 ? NS - 1 : stage - 1, ci + NS - 1);
+    stage = stage == NS - 1 ? 0 : stage + 1;
     float a = __builtin_fmaf(full.hi, owed, full.hi);
     owed = __builtin_fmaf((full.hi - a) + full.lo, inv_full, owed);
     if (left < kC) {          // the last, partial chunk
@@ -378,22 +372,23 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
 #pragma unroll
       for (int x = 0; x < 8; ++x) w[x] = s_pow[max(0, left - 1 - (16 * (x >> 2) + j0 + (x & 3)))];
     }
+    if constexpr (!ONLY_STATE) {
+      if (ci + 1 < nch && turn == (ci + 1) % TURNS)
+        build_p((lds_char_t*)(smem + stage * STAGE), ~ci & 1);
+    }
 
-    // ---- v as operands, and a^(C-1-j) v as sums of 16-bit numbers
-    u32x4_t vf[NT], vt[TERMS][NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      vf[nt] = col_op(lv, VC{}, NT == 2 ? wave * 4 + c4 : wave * 2 + (c4 >> 1),
-                      NT == 2 ? nt : c4 & 1);
+    // ---- v as an operand, and a^(C-1-j) v as a sum of 16-bit numbers
+    const u32x4_t vf = col_op(lv, VC{}, wave * 2 + (c4 >> 1), c4 & 1);
+    u32x4_t vt[TERMS];
     // f16: the second number 2^11 times larger, in sums of its own, so that it keeps
     // its bits
     constexpr float kLow = F16 ? 2048.f : 1.f;
-    auto weigh = [&](int nt, int x) {
-      float y0 = lo16<F16>(vf[nt][x]) * w[2 * x], y1 = hi16<F16>(vf[nt][x]) * w[2 * x + 1];
+    auto weigh = [&](int x) {
+      float y0 = lo16<F16>(vf[x]) * w[2 * x], y1 = hi16<F16>(vf[x]) * w[2 * x + 1];
 #pragma unroll
       for (int z = 0; z < TERMS; ++z) {
         const uint32_t y = pack2<F16>(y0, y1);
-        vt[z][nt][x] = y;
+        vt[z][x] = y;
         if (z + 1 < TERMS) {
           y0 = (y0 - lo16<F16>(y)) * kLow;
           y1 = (y1 - hi16<F16>(y)) * kLow;
@@ -401,11 +396,9 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
       }
     };
 
-    // ---- S^T Q^T of the state before the chunk, times scale a^(i+1); the next chunk's P^T
-    // (behind the last, of what lies there: never read).  Products that wait for each
-    // other are kept apart, and v's factors are worked out between them: a chain of
-    // products that follow each other directly took twice as long.
-    f32x4_t o[kIT][NT];
+    // ---- S^T Q^T of the state before the chunk, times scale a^(i+1).  Products that wait
+    // for each other are kept apart, and v's factors are worked out between them.
+    f32x4_t o[kIT];
     if constexpr (!ONLY_STATE) {
       float sc = 1.f;
       if constexpr (F16) {
@@ -413,80 +406,57 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, finite_abs(s[dt][nt][i]));
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, finite_abs(s[dt][i]));
         sc = f16_scale(mx);
       }
       const float back = F16 ? 1.f / sc : 1.f;
-      const lds_char_t* const next = (lds_char_t*)(smem + stage * STAGE);
-      f32x4_t px[PT] = {};
 #pragma unroll
-      for (int it = 0; it < kIT; ++it)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) o[it][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int it = 0; it < kIT; ++it) o[it] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        u32x4_t q[kIT];
-#pragma unroll
-        for (int it = 0; it < kIT; ++it) q[it] = row_op(lq, it, ks);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          f32x4_t x = s[2 * ks][nt], y = s[2 * ks + 1][nt];
-          if constexpr (F16) {
-            x *= sc;
-            y *= sc;
-          }
-          const u32x4_t sp = u32x4_t{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]),
-                                     pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3])};
-#pragma unroll
-          for (int it = 0; it < kIT; ++it) o[it][nt] = mfma16t<F16>(sp, q[it], o[it][nt]);
+        f32x4_t x = s[2 * ks], y = s[2 * ks + 1];
+        if constexpr (F16) {
+          x *= sc;
+          y *= sc;
         }
-        p_step(next, ks, px);
-        // (all of v's 4 NT pieces over the steps)
+        const u32x4_t sp = u32x4_t{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]),
+                                   pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3])};
 #pragma unroll
-        for (int x = 4 * NT * ks / KS; x < 4 * NT * (ks + 1) / KS; ++x) weigh(x / 4, x % 4);
+        for (int it = 0; it < kIT; ++it) o[it] = mfma16t<F16>(sp, row_op(lq, it, ks), o[it]);
+#pragma unroll
+        for (int y4 = 4 * ks / KS; y4 < 4 * (ks + 1) / KS; ++y4) weigh(y4);
       }
-      p_store(px, ~ci & 1);
 #pragma unroll
-      for (int it = 0; it < kIT; ++it)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) o[it][nt] *= rise[it] * back;
+      for (int it = 0; it < kIT; ++it) o[it] *= rise[it] * back;
     } else {
 #pragma unroll
-      for (int x = 0; x < 4 * NT; ++x) weigh(x / 4, x % 4);
+      for (int x = 0; x < 4; ++x) weigh(x);
     }
 
-    // ---- the state behind the chunk, row tiles in pairs
+    // ---- the state behind the chunk, row tiles in fours
 #pragma unroll
-    for (int d2 = 0; d2 < DT; d2 += 2) {
-      u32x4_t kt[2];
-      f32x4_t x[2][NT], y[2][NT];
+    for (int d4 = 0; d4 < DT; d4 += 4) {
+      u32x4_t kt[4];
+      f32x4_t x[4], y[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        kt[u] = col_op(lk, QK{}, 2 * (d2 + u) + (c4 >> 1), c4 & 1);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) x[u][nt] = y[u][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < 4; ++u) {
+        kt[u] = col_op(lk, QK{}, 2 * (d4 + u - (u & 1)) + c4, u & 1);
+        x[u] = y[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
       for (int z = TERMS - 1; z >= 0; --z)      // the small ones first
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 4; ++u) {
+          f32x4_t& t = F16 && z == 1 ? y[u] : x[u];
+          t = mfma16t<F16>(kt[u], vt[z], t);
+        }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            f32x4_t& t = F16 && z == 1 ? y[u][nt] : x[u][nt];
-            t = mfma16t<F16>(kt[u], vt[z][nt], t);
-          }
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float z =
-                F16 ? __builtin_fmaf(y[u][nt][i], 1.f / kLow, x[u][nt][i]) : x[u][nt][i];
-            s[d2 + u][nt][i] = __builtin_fmaf(s[d2 + u][nt][i], a, z);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float z = F16 ? __builtin_fmaf(y[u][i], 1.f / kLow, x[u][i]) : x[u][i];
+          s[d4 + u][i] = __builtin_fmaf(s[d4 + u][i], a, z);
+        }
     }
 
     if constexpr (!ONLY_STATE) {
@@ -494,21 +464,14 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
       // A token whose v is not finite makes its columns of the state so: then every
       // query takes its own product, tokens behind it as zeros, since a weight of zero
       // times an infinity would reach the queries ahead of them.
-      bool odd = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) odd |= !(fabsf(s[0][nt][0]) < INFINITY);
-      const bool alone = __builtin_amdgcn_ballot_w64(odd) != 0;
+      const bool alone = __builtin_amdgcn_ballot_w64(!(fabsf(s[0][0]) < INFINITY)) != 0;
 #pragma unroll
       for (int it = 0; it < kIT; ++it) {
         const u32x4_t pf = s_p[((ci & 1) * kIT + it) * 64 + lane];
         const float ps = F16 ? s_ps[ci & 1][it] : 1.f;
-        if constexpr (F16) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) o[it][nt] *= ps;
-        }
+        if constexpr (F16) o[it] *= ps;
         if (!alone) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) o[it][nt] = mfma16t<F16>(vf[nt], pf, o[it][nt]);
+          o[it] = mfma16t<F16>(vf, pf, o[it]);
         } else {
           const int j0 = fresh(4 * g4);
 #pragma unroll 1
@@ -519,37 +482,23 @@ __global__ void __launch_bounds__(256, 2) linear_chunk_kernel(LinearParams p) {
               const int j = 16 * (y >> 1) + j0 + 2 * (y & 1), i = 16 * it + x;
               keep[y] = (j <= i ? 0xffffu : 0u) | (j + 1 <= i ? 0xffff0000u : 0u);
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const f32x4_t z = mfma16t<F16>(vf[nt] & keep, pf, o[it][nt]);
-              if (r == x) o[it][nt] = z;
-            }
+            const f32x4_t z = mfma16t<F16>(vf & keep, pf, o[it]);
+            if (r == x) o[it] = z;
           }
         }
-        if constexpr (F16) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) o[it][nt] *= 1.f / ps;
-        }
-        // ---- o[it][nt][e] is token 16 it + r, column col0 + 8 g4 + 4 nt + e (NT 2) or
-        // col0 + 4 g4 + e
+        if constexpr (F16) o[it] *= 1.f / ps;
+        // ---- o[it][e] is token 16 it + r, column col0 + 4 g4 + e
         char* to = const_cast<char*>(uniform(ob + (int64_t)(ci * kC + 16 * it) * GH * E * 2)) + ooff;
-        if (16 * it + r < left && col0 + 4 * NT * g4 < E) {
-          const u32x2_t x = u32x2_t{pack2<F16>(o[it][0][0], o[it][0][1]),
-                                    pack2<F16>(o[it][0][2], o[it][0][3])};
-          if constexpr (NT == 2)
-            *reinterpret_cast<u32x4_t*>(to) =
-                u32x4_t{x[0], x[1], pack2<F16>(o[it][NT - 1][0], o[it][NT - 1][1]),
-                        pack2<F16>(o[it][NT - 1][2], o[it][NT - 1][3])};
-          else
-            *reinterpret_cast<u32x2_t*>(to) = x;
-        }
+        if (16 * it + r < left && col0 + 4 * g4 < E)
+          *reinterpret_cast<u32x2_t*>(to) =
+              u32x2_t{pack2<F16>(o[it][0], o[it][1]), pack2<F16>(o[it][2], o[it][3])};
       }
     }
   }
 
   if constexpr (ONLY_STATE) {
     if (!wanted) return;
-    write_state(p.ws + (bgh * p.nseg + seg + 1) * sz);
+    write_state(p.ws + (bgh * slots + seg + 1) * sz);
   } else if (t0 + tokens == c) {      // the segment that the sequence ends in
     write_state(p.state_out + bgh * sz);
   }
@@ -619,35 +568,39 @@ __global__ void __launch_bounds__(256) linear_step_kernel(LinearParams p, int L)
 
 // The launch's shape, from the extents alone.
 struct Shape {
-  int nt, nsl, nseg, cps;
+  int waves, nsl, nseg, sub, cps;
 };
 Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t E, int64_t T) {
   Shape s{};
-  // 128 columns to a workgroup; 64 of states that are no wider, and past D 128, whose
-  // states of 128 columns would not leave registers enough
-  s.nt = D > 128 || E <= 64 ? 1 : 2;
-  s.nsl = (int)cdiv64(E, 64 * s.nt);
+  // 128 columns to a workgroup, 64 of states that are no wider
+  s.waves = E <= 64 ? 4 : 8;
+  s.nsl = (int)cdiv64(E, 16 * s.waves);
   const int64_t wgs = B * G * H * s.nsl, chunks = cdiv64(T, kC);
-  // two workgroups run on a CU at once
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({512 / wgs, chunks / 8, 64}));
-  s.cps = (int)cdiv64(chunks, want);
-  s.nseg = (int)cdiv64(chunks, s.cps);
+  // workgroups that run at once
+  const int64_t slots = s.waves == 4 && D <= 128 ? 512 : 256;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({slots / wgs, chunks / 4, 64}));
+  // two stretches to a segment where its first launch would leave most of the CUs idle
+  s.sub = want > 1 && wgs * (want - 1) < 128 ? 2 : 1;
+  s.cps = (int)cdiv64(chunks, want * s.sub);
+  s.nseg = (int)cdiv64(chunks, s.cps * s.sub);
   return s;
 }
 
 template <bool F16, bool ONLY_STATE>
 void launch_chunks(const LinearParams& p, const Shape& s, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)p.B * p.G * p.H * s.nsl * (s.nseg - (ONLY_STATE ? 1 : 0)))),
-      block(256);
+  const dim3 grid((unsigned)((int64_t)p.B * p.G * p.H * s.nsl *
+                             (ONLY_STATE ? (s.nseg - 1) * s.sub : s.nseg))),
+      block(64 * s.waves);
   auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, st, p); };
   // the kernel built for 64, 128 or 256 (the next one up) runs any narrower key dim
-  if (p.D > 128) launch(linear_chunk_kernel<256, 1, F16, ONLY_STATE>);
-  else if (p.D > 64) {
-    if (s.nt == 1) launch(linear_chunk_kernel<128, 1, F16, ONLY_STATE>);
-    else launch(linear_chunk_kernel<128, 2, F16, ONLY_STATE>);
+  if (s.waves == 4) {
+    if (p.D > 128) launch(linear_chunk_kernel<256, 4, F16, ONLY_STATE>);
+    else if (p.D > 64) launch(linear_chunk_kernel<128, 4, F16, ONLY_STATE>);
+    else launch(linear_chunk_kernel<64, 4, F16, ONLY_STATE>);
   } else {
-    if (s.nt == 1) launch(linear_chunk_kernel<64, 1, F16, ONLY_STATE>);
-    else launch(linear_chunk_kernel<64, 2, F16, ONLY_STATE>);
+    if (p.D > 128) launch(linear_chunk_kernel<256, 8, F16, ONLY_STATE>);
+    else if (p.D > 64) launch(linear_chunk_kernel<128, 8, F16, ONLY_STATE>);
+    else launch(linear_chunk_kernel<64, 8, F16, ONLY_STATE>);
   }
 }
 
@@ -724,6 +677,7 @@ int linear_impl(const void* q, const void* k, const void* v,
   p.ws = static_cast<float*>(workspace);
   p.nsl = s.nsl;
   p.nseg = s.nseg;
+  p.sub = s.sub;
   p.cps = s.cps;
   if (s.nseg > 1) {
     launch_chunks<F16, true>(p, s, st);
@@ -744,7 +698,7 @@ size_t loom_hip_linear_attention_workspace_bytes(int64_t B, int64_t G, int64_t H
   // what does not fit is reported as no size at all fits
   if (T > (1 << 29) || D > 256 || E > 256 || !loom_prod_le({B, G, H}, 1 << 20)) return SIZE_MAX;
   const Shape s = shape_of(B, G, H, D, E, T);
-  return s.nseg == 1 ? 0 : (size_t)(B * G * H * s.nseg) * D * E * 4;
+  return s.nseg == 1 ? 0 : (size_t)(B * G * H * ((s.nseg - 1) * s.sub + 1)) * D * E * 4;
 }
 
 int loom_hip_linear_attention(const void* q, const void* k, const void* v, const void* log_decay,
