@@ -43,6 +43,14 @@ LOOM_DEV int wv_swz(int k) { return D >= 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3);
 template <int D>
 LOOM_DEV int wq_swz(int lr) { return D >= 128 ? (lr & 15) : ((lr ^ (lr >> 3)) & 7); }
 
+// A value that the compiler does not know to be x: what rare paths compute from it is
+// worked out there, not ahead of a loop in registers that it needs.  (A spilled register
+// costs more than its load there: that load's wait is one for every copy on its way.)
+LOOM_DEV int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // dma_load16 of keys that no other workgroup reads: non-temporal
 LOOM_DEV void dma_once16(const void* g, uint32_t lds) {
   asm volatile(
@@ -177,7 +185,8 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
     const int j = wave * V_INSTR + i, kr = j * V_ROWS_PER_I + lane / (D / 8);
     voff[i] = (uint32_t)(kr * Dr + min((lane % (D / 8)) ^ wv_swz<D>(kr), Dr / 8 - 1) * 8) * 2;
   }
-  const bool once = p.once != 0;
+  // (tiles of few rows only: keys of larger ones are shared)
+  const bool once = KG == 2 && p.once != 0;
   auto issue = [&](int s, int blk) {
     const int kv0 = first_key(blk);
     const uint32_t lk = lds_addr(stK(s)), lv = lds_addr(stV(s));
@@ -198,14 +207,15 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
         dma_load16_s(voff[i], vg + (int64_t)kv0 * Dr, lv + (wave * V_INSTR + i) * 1024);
       return;
     }
+    const int ln = KG == 2 ? lane : fresh(lane);
     if constexpr (!KREG) {
 #pragma unroll
       for (int i = 0; i < K_INSTR; ++i) {
         const int j = wave * K_INSTR + i;
-        const int d = j * 8 + lane / 8;
-        const int key = min(kv0 + ((lane % 8) ^ wk_swz(d)) * 8, S - 8);
+        const int d = j * 8 + ln / 8;
+        const int key = min(kv0 + ((ln % 8) ^ wk_swz(d)) * 8, S - 8);
         const uint16_t* from = kg + (int64_t)d * S + key;
-        if (j * 8 >= Dr) dma_load16(loom_zero_kb + lane * 4, lk + j * 1024);
+        if (j * 8 >= Dr) dma_load16(loom_zero_kb + ln * 4, lk + j * 1024);
         else if (once) dma_once16(from, lk + j * 1024);
         else dma_load16(from, lk + j * 1024);
       }
@@ -213,11 +223,11 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
 #pragma unroll
     for (int i = 0; i < V_INSTR; ++i) {
       const int j = wave * V_INSTR + i;
-      const int kr = j * V_ROWS_PER_I + lane / (D / 8);
+      const int kr = j * V_ROWS_PER_I + ln / (D / 8);
       const int key = kv0 + kr;
       const bool seen = key <= a.pmax && (key >= a.low || key < a.ns);
       const void* from = seen ? (const void*)((const char*)(vg + (int64_t)kv0 * Dr) + voff[i])
-                              : (const void*)(loom_zero_kb + lane * 4);
+                              : (const void*)(loom_zero_kb + ln * 4);
       if (once) dma_once16(from, lv + j * 1024);
       else dma_load16(from, lv + j * 1024);
     }
@@ -348,11 +358,12 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
           for (int i = 0; i < 4; ++i)
             st[j][qt][i] = __builtin_fmaf(st[j][qt][i], c2, -m_run[qt]);
         if (edge) {
+          const int key0 = fresh(k0 + 4 * g);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int key = k0 + 16 * j + 4 * g + i;
+              const int key = key0 + 16 * j + i;
               if (key > pos[qt] || (key <= pos[qt] - p.window && key >= p.sinks))
                 st[j][qt][i] = -INFINITY;
             }
@@ -419,7 +430,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
 #pragma unroll
         for (int i = 0; i < 32 * VROW / 1024; ++i) {
           const u32x4_t w = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
-              vs + 32 * h * VROW + i * 1024 + lane * 16);
+              vs + 32 * h * VROW + i * 1024 + fresh(lane) * 16);
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             top = __builtin_elementwise_max(top,
@@ -427,6 +438,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
         }
         constexpr uint16_t kInf = F16 ? 0x7c00 : 0x7f80;
         if (__builtin_amdgcn_ballot_w64(top[0] >= kInf || top[1] >= kInf) != 0) {
+          const int key0 = fresh(k0 + 4 * g);
 #pragma unroll 1
           for (int c = 0; c < 16; ++c)
 #pragma unroll
@@ -438,7 +450,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
                 uint32_t m = 0;
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                  const int key = k0 + 16 * (x >> 1) + 4 * g + 2 * (x & 1) + y;
+                  const int key = key0 + 16 * (x >> 1) + 2 * (x & 1) + y;
                   if (key <= pc && (key > pc - p.window || key < p.sinks)) m |= 0xffffu << (16 * y);
                 }
                 keep[x] = m;
@@ -447,6 +459,8 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
               for (int dt = 0; dt < DT; ++dt) {
                 const f32x4_t o = mfma16t<F16>(v_op(dt) & keep, pf[qt], ot[dt][qt]);
                 if (r == c) ot[dt][qt] = o;
+                // (one at a time: the registers of several would be taken from the others)
+                __builtin_amdgcn_sched_barrier(0);
               }
             }
           continue;
@@ -461,44 +475,42 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
     }
   };
 
-  // ---- pipeline: NS stages (the first NS-1 issued above), waits placed by hand
-  for (int it0 = 0; it0 < nblk; it0 += NS) {
+  // ---- pipeline: NS stages (the first NS-1 issued above), waits placed by hand.  (Not
+  // unrolled over the stages: their addresses would not leave registers enough.)
+  int s = 0;
+#pragma unroll 1
+  for (int it = 0; it < nblk; ++it) {
+    const int younger = min(NS - 2, nblk - 1 - it);
+    if (younger >= 1) LOOM_WAIT_VMCNT(LPW);
+    else LOOM_WAIT_VMCNT(0);
+    // this wave's reads of the stage that is overwritten next, and KREG's stores
+    LOOM_WAIT_LGKM0();
+    barrier_nofence();
+    if constexpr (QDMA) {
+      if (it == 0) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const int it = it0 + s;
-      if (it < nblk) {
-        const int younger = min(NS - 2, nblk - 1 - it);
-        if (younger >= 1) LOOM_WAIT_VMCNT(LPW);
-        else LOOM_WAIT_VMCNT(0);
-        // this wave's reads of the stage that is overwritten next, and KREG's stores
-        LOOM_WAIT_LGKM0();
-        barrier_nofence();
-        if constexpr (QDMA) {
-          if (it == 0) {
+        for (int qt = 0; qt < QT; ++qt) {
+          const int lr = rw0 + 16 * qt + r;
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              const int lr = rw0 + 16 * qt + r;
-#pragma unroll
-              for (int ds = 0; ds < DSTEPS; ++ds) {
-                const u32x4_t raw =
-                    *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
-                        sQ + lr * QROW + ((4 * ds + g) ^ wq_swz<D>(lr)) * 16);
-                qf[ds][qt] = ds * 32 + g * 8 < Dr ? raw : u32x4_t{0u, 0u, 0u, 0u};
-              }
-            }
+          for (int ds = 0; ds < DSTEPS; ++ds) {
+            const u32x4_t raw = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
+                sQ + lr * QROW + ((4 * ds + g) ^ wq_swz<D>(lr)) * 16);
+            qf[ds][qt] = ds * 32 + g * 8 < Dr ? raw : u32x4_t{0u, 0u, 0u, 0u};
           }
-        }
-        const bool ahead = it + NS - 1 < nblk;
-        if constexpr (KREG) {
-          if (ahead) kload(it + NS - 1);
-        }
-        if (ahead) issue((s + NS - 1) % NS, it + NS - 1);
-        if (active) compute(s, it);
-        if constexpr (KREG) {
-          if (ahead) kstore((s + NS - 1) % NS);
         }
       }
     }
+    const int to = s == 0 ? NS - 1 : s - 1;     // the stage of block it - 1
+    const bool ahead = it + NS - 1 < nblk;
+    if constexpr (KREG) {
+      if (ahead) kload(it + NS - 1);
+    }
+    if (ahead) issue(to, it + NS - 1);
+    if (active) compute(s, it);
+    if constexpr (KREG) {
+      if (ahead) kstore(to);
+    }
+    s = s == NS - 1 ? 0 : s + 1;
   }
 
   // (without a block nothing has waited for the Q copies)
