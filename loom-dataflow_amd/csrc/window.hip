@@ -358,14 +358,16 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
           for (int i = 0; i < 4; ++i)
             st[j][qt][i] = __builtin_fmaf(st[j][qt][i], c2, -m_run[qt]);
         if (edge) {
-          const int key0 = fresh(k0 + 4 * g);
+          // (no short circuits: a branch for every key takes longer than a comparison)
+          const int ps = fresh(pos[qt]), lo = max(0, ps - p.window + 1);
+          const int at0 = k0 + 4 * g - lo, n = max(0, ps + 1 - lo), sk = min(p.sinks, ps + 1) - lo;
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int key = key0 + 16 * j + i;
-              if (key > pos[qt] || (key <= pos[qt] - p.window && key >= p.sinks))
-                st[j][qt][i] = -INFINITY;
+              const int at = at0 + 16 * j + i;
+              const bool sees = ((uint32_t)at < (uint32_t)n) | (at < sk);
+              st[j][qt][i] = sees ? st[j][qt][i] : -INFINITY;
             }
         }
 #pragma unroll
@@ -419,12 +421,15 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
         const u32x2_t hi = lds_read_tr16(q + 16 * VROW);    // keys k0 + 16 + 4 g + 0..3
         return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
       };
-      // Keys that some rows of the wave see and others do not: a weight of zero times
+      // Keys that some rows of the tile see and the wave's do not all: a weight of zero times
       // an infinity or NaN of theirs would reach the others.  Such values are looked
       // for (the largest magnitude's bits, two elements at a time) and, where there
       // are any, every row takes its own product, V's elements that it does not see
       // as zeros.
-      if (edge && pw0 != pw1) {
+      // (rows of one token see the same; and what no row sees lies there as zeros)
+      const bool mixed = a.pmin != a.pmax &&
+                         (k0 + 31 > pw0 || (k0 <= pw1 - p.window && k0 + 31 >= a.low));
+      if (mixed) {
         typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
         u16x2_t top = u16x2_t{0, 0};
 #pragma unroll
@@ -451,7 +456,8 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                   const int key = key0 + 16 * (x >> 1) + 2 * (x & 1) + y;
-                  if (key <= pc && (key > pc - p.window || key < p.sinks)) m |= 0xffffu << (16 * y);
+                  m |= (key <= pc) & ((key > pc - p.window) | (key < p.sinks)) ? 0xffffu << (16 * y)
+                                                                               : 0u;
                 }
                 keep[x] = m;
               }
@@ -679,6 +685,7 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t T, int64_t S,
   const int64_t most = D > 128 ? 128 : 256;
   s.tile = 32;
   while (s.tile < most && s.tile < rows && BG * cdiv64(rows, s.tile * 2) >= 256) s.tile *= 2;
+  if (D > 128 && s.tile == 64) s.tile = 32;
   s.ntiles = cdiv64(rows, s.tile);
   // the blocks of keys that a tile reads at most
   const int64_t span = std::min(S, std::min(window, S) + cdiv64(s.tile, H));
@@ -699,7 +706,6 @@ void launch_window(const WindowParams& p, const Shape& s, hipStream_t st) {
   if (p.D > 128) {
     switch (s.tile) {
       case 32: launch(window_tile_kernel<256, 1, 4, F16, KREG, SPLIT, 2, 2, 1, 256>, b4); break;
-      case 64: launch(window_tile_kernel<256, 1, 8, F16, KREG, SPLIT, 2, 2, 1, 256>, b8); break;
       default: launch(window_tile_kernel<256, 1, 8, F16, KREG, SPLIT, 1, 2, 1, 256>, b8); break;
     }
   } else if (p.D > 96) {

@@ -431,3 +431,20 @@ def test_threads_on_their_own_streams(lh):
     for i in range(len(d)):
         for r in got[i]:
             assert torch.equal(r, want[i])
+
+
+@pytest.mark.parametrize("H,T", [(40, 9), (64, 5), (130, 3)])
+def test_infinities_between_waves_of_one_tile(lh, H, T):
+    """Rows of a wave that all are one token's, beside waves of others in the tile: an
+    infinity that only these see stays with them."""
+    S, W, D = 300, 50, 64
+    t = make(1, 1, H, D, T, S, [S], None, W, 2, torch.bfloat16, seed=H)
+    t["v"][0, 0, S - 1, 5] = math.inf              # the last token sees it
+    t["v"][0, 0, S - T - W + 1, 9] = -math.inf     # the first does
+    want, tol = reference(t, [S], None, W, 2)
+    got = attend(lh, t, [S], None, W, 2).double().cpu()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine) and not fine.all()
+    zero = torch.zeros_like(want)
+    near(torch.where(fine, got, zero), torch.where(fine, want, zero),
+         torch.where(fine, tol, zero), "beside infinities of other waves")
