@@ -176,38 +176,53 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
   offsets(qoff, qs, QK{});
   offsets(koff, ks_, QK{});
   offsets(voff, vs, VC{});
-  auto issue = [&](int s, int ci) {
-    const int left = tokens - ci * kC;
-    const uint32_t base = lds_addr((lds_char_t*)(smem + s * STAGE));
-    auto rows = [&](const uint16_t* from, uint32_t stride, int valid, auto& off, auto n,
-                    uint32_t lds) {
-      constexpr int N = decltype(n)::value, ALL = kC * N * 2 / 1024, INSTR = (ALL + W - 1) / W;
-      const char* at = uniform((const char*)from + (int64_t)ci * kC * stride);
-      const bool whole = fast && left >= kC;
-      const int ln = fresh(lane);
+  // where the next chunk to be copied begins, and how many tokens are left there
+  const char *qat = reinterpret_cast<const char*>(qb), *kat = reinterpret_cast<const char*>(kb),
+             *vat = reinterpret_cast<const char*>(vb);
+  int ahead = tokens;
+  const uint32_t lds0 = lds_addr((lds_char_t*)smem) + wave * 1024;
+  auto issue = [&](int s) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + s * STAGE);
+    if (fast && ahead >= kC) {                  // wave-uniform
+      auto rows = [&](const char* at, auto& off, auto n, uint32_t lds) {
+        constexpr int N = decltype(n)::value, ALL = kC * N * 2 / 1024, INSTR = (ALL + W - 1) / W;
+        at = uniform(at);
 #pragma unroll
-      for (int i = 0; i < INSTR; ++i) {
-        const int j = wave + W * i;
-        if (ALL % W && j >= ALL) break;         // wave-uniform
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + j * 1024);
-        if (whole) {
-          dma_load16_s(off[i], at, to);
-        } else {
+        for (int i = 0; i < INSTR; ++i) {
+          if (ALL % W && wave + W * i >= ALL) break;
+          dma_load16_s(off[i], at, lds + W * i * 1024);
+        }
+      };
+      if constexpr (!ONLY_STATE) rows(qat, qoff, QK{}, to);
+      rows(kat, koff, QK{}, to + Q_BYTES);
+      rows(vat, voff, VC{}, to + Q_BYTES + K_BYTES);
+    } else {
+      auto rows = [&](const char* at, uint32_t stride, int valid, auto n, uint32_t lds) {
+        constexpr int N = decltype(n)::value, ALL = kC * N * 2 / 1024, INSTR = (ALL + W - 1) / W;
+        const int ln = fresh(lane);
+#pragma unroll
+        for (int i = 0; i < INSTR; ++i) {
+          const int j = wave + W * i;
+          if (ALL % W && j >= ALL) break;
           const int e = j * 64 + ln, row = e / (N / 8), ch = (e % (N / 8)) ^ row_swz<N>(row);
-          const void* src = row < left && ch < valid
+          const void* src = row < ahead && ch < valid
                                 ? (const void*)(at + (int64_t)row * stride + ch * 16)
                                 : (const void*)(loom_zero_kb + lane * 4);
-          dma_load16(src, to);
+          dma_load16(src, __builtin_amdgcn_readfirstlane(lds + W * i * 1024));
         }
-      }
-    };
-    if constexpr (!ONLY_STATE) rows(qb, qs, D / 8, qoff, QK{}, base);
-    rows(kb, ks_, D / 8, koff, QK{}, base + Q_BYTES);
-    rows(vb, vs, (E - sl * SL) / 8, voff, VC{}, base + Q_BYTES + K_BYTES);
+      };
+      if constexpr (!ONLY_STATE) rows(qat, qs, D / 8, QK{}, to);
+      rows(kat, ks_, D / 8, QK{}, to + Q_BYTES);
+      rows(vat, vs, (E - sl * SL) / 8, VC{}, to + Q_BYTES + K_BYTES);
+    }
+    qat += (int64_t)kC * qs;
+    kat += (int64_t)kC * ks_;
+    vat += (int64_t)kC * vs;
+    ahead -= kC;
   };
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i)
-    if (i < nch) issue(i, i);
+    if (i < nch) issue(i);
 
   const float lg = p.g[gh];
   if (tid <= kC) s_pow[tid] = (float)decay_pow(lg, tid);
@@ -288,7 +303,8 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
     seen[x] = lag >= 0;
     pf_fac[x] = p.scale * s_pow[max(lag, 0)];
   }
-  const char* const ob = reinterpret_cast<const char*>(p.out + (tok0 * GH + gh) * E + col0);
+  const char* ob = reinterpret_cast<const char*>(p.out + (tok0 * GH + gh) * E + col0);
+  const int64_t ostep = (int64_t)16 * GH * E * 2;
   const int64_t ooff = (int64_t)r * GH * E * 2 + 8 * g4;
   const bool stores = !ONLY_STATE && col0 < E;
   // stores of a chunk's rows, all of which a whole chunk issues
@@ -362,7 +378,7 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
     else LOOM_WAIT_VMCNT(0);
     LOOM_WAIT_LGKM0();
     barrier_nofence();
-    if (ci + NS - 1 < nch) issue(stage == 0 ? NS - 1 : stage - 1, ci + NS - 1);
+    if (ci + NS - 1 < nch) issue(stage == 0 ? NS - 1 : stage - 1);
     stage = stage == NS - 1 ? 0 : stage + 1;
     float a = __builtin_fmaf(full.hi, owed, full.hi);
     owed = __builtin_fmaf((full.hi - a) + full.lo, inv_full, owed);
@@ -488,7 +504,8 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
         }
         if constexpr (F16) o[it] *= 1.f / ps;
         // ---- o[it][e] is token 16 it + r, column col0 + 4 g4 + e
-        char* to = const_cast<char*>(uniform(ob + (int64_t)(ci * kC + 16 * it) * GH * E * 2)) + ooff;
+        char* to = const_cast<char*>(uniform(ob)) + ooff;
+        ob += ostep;
         if (16 * it + r < left && col0 + 4 * g4 < E)
           *reinterpret_cast<u32x2_t*>(to) =
               u32x2_t{pack2<F16>(o[it][0], o[it][1]), pack2<F16>(o[it][2], o[it][3])};
@@ -553,7 +570,7 @@ __global__ void __launch_bounds__(256) linear_step_kernel(LinearParams p, int L)
           x[i][y] = __builtin_fmaf(x[i][y], a.hi, __builtin_fmaf(x[i][y], a.lo, k * v[y]));
           o[y] = __builtin_fmaf(q, x[i][y], o[y]);
         }
-        *reinterpret_cast<f32x4_t*>(at + (int64_t)d * E) = x[i];
+        store_stream(reinterpret_cast<f32x4_t*>(at + (int64_t)d * E), x[i]);
       }
     }
   }
