@@ -152,9 +152,9 @@ def test_linear(lh, shape, e):
 
 
 @pytest.mark.parametrize("e", TYPES)
-@pytest.mark.parametrize("decay", [0.0, -1e-4, -0.7, -30.0, -1e4, -math.inf])
+@pytest.mark.parametrize("decay", [0.0, -1e-4, -0.7, -30.0, -1e4, -math.inf, 0.02])
 def test_decays(lh, decay, e):
-    """From heads that forget nothing to heads without memory."""
+    """From heads that forget nothing to heads without memory (and one that grows)."""
     check(lh, "decay", 2, 1, 2, 64, 64, 200, [200, 77], TYPES[e], decay=decay)
 
 
@@ -166,6 +166,36 @@ def test_long_prompts(lh, e):
     check(lh, "long", 1, 2, 1, 128, 128, 2500, None, t, decay=-1e-3)
     check(lh, "long, ragged", 3, 1, 1, 64, 64, 2049, [2049, 1024, 700], t)
     check(lh, "long, no state", 1, 1, 2, 128, 64, 1984, None, t, state=False, decay=0.0)
+
+
+@pytest.mark.parametrize("e", TYPES)
+def test_ends_of_chunks_and_stretches(lh, e):
+    """Sequences that end at, before and behind the ends of chunks of 32 tokens and of
+    the stretches that a long prompt is split into; states in place."""
+    counts = [0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 383, 384, 385, 639, 640]
+    B, T = len(counts), 640
+    for D, E in ((64, 64), (128, 96), (32, 200)):
+        print("ends", D, E, e, flush=True)
+        t = make(B, 1, 1, D, E, T, counts, TYPES[e], seed=D)
+        assert lh.linear_attention_workspace_bytes(B, 1, 1, D, E, T)      # (it is split)
+        want, tol, end, etol = reference(t, counts)
+        d = on_gpu(t)
+        out = torch.full((B, T, 1, 1, E), 7.0, dtype=TYPES[e], device="cuda")
+        _, s = lh.linear_attention(d["q"], d["k"], d["v"], d["log_decay"], d["state"], out,
+                                   d["state"], counts=ints(counts))
+        assert s is d["state"]
+        near(out, want, tol, f"ends D{D} E{E} {e}")
+        near(s, end, etol, f"ends D{D} E{E} {e} state")
+
+
+@pytest.mark.parametrize("e", TYPES)
+@pytest.mark.parametrize("D,E", [(128, 128), (64, 64), (256, 128), (48, 72)])
+def test_many_heads(lh, D, E, e):
+    """More heads than run at once: every prompt in one piece, over many chunks."""
+    B, G, H, T = 5, 40, 3, 190
+    counts = [190, 1, 100, 160, 31]
+    check(lh, "many heads", B, G, H, D, E, T, counts, TYPES[e], seed=D)
+    assert not lh.linear_attention_workspace_bytes(B, G, H, D, E, T)
 
 
 def test_decay_of_a_long_memory(lh):

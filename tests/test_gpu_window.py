@@ -448,3 +448,34 @@ def test_infinities_between_waves_of_one_tile(lh, H, T):
     zero = torch.zeros_like(want)
     near(torch.where(fine, got, zero), torch.where(fine, want, zero),
          torch.where(fine, tol, zero), "beside infinities of other waves")
+
+
+@pytest.mark.parametrize("S", [264, 261])
+@pytest.mark.parametrize("D,H,rows", [(128, 4, 256), (64, 4, 256), (96, 4, 256), (256, 2, 128),
+                                      (128, 2, 128), (64, 2, 128), (80, 2, 128), (128, 1, 64),
+                                      (56, 1, 64), (88, 1, 64), (200, 1, 32)])
+def test_every_tile(lh, D, H, rows, S):
+    """64 (b, g)s: as many rows as the tiles of 64, 128 and 256 are taken for, K's rows on
+    and off 16-byte boundaries, padded batches, infinities that some rows see."""
+    B, G, T, W, sinks = 8, 8, 256, 70, 3
+    e = torch.bfloat16 if D % 64 else torch.float16
+    assert H * T >= 4 * rows
+    lens = [S - b for b in range(B)]
+    counts = [T - 5 * b - (b == 3) * 200 for b in range(B)]
+    print("tile", D, H, rows, S, flush=True)
+    t = make(B, G, H, D, T, S, lens, counts, W, sinks, e, D)
+    t["v"][2, 3, 150, 5] = math.inf
+    t["v"][1, 7, 1, 9] = NAN
+    want, tol = reference(t, lens, counts, W, sinks)
+    got = attend(lh, t, lens, counts, W, sinks).double().cpu()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine) and not fine.all()
+    zero = torch.zeros_like(want)
+    near(torch.where(fine, got, zero), torch.where(fine, want, zero),
+         torch.where(fine, tol, zero), f"tile of {rows} D{D} S{S}")
+
+
+def test_many_heads_in_large_tiles(lh):
+    """71 heads: tokens that begin and end inside a tile and inside a wave's rows."""
+    check(lh, "71 heads", 64, 1, 71, 64, 15, 100, [100 - b for b in range(64)],
+          [15 - b % 7 for b in range(64)], 40, 2, torch.bfloat16)
