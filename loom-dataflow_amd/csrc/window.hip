@@ -12,6 +12,7 @@
 #include "common.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -71,11 +72,15 @@ struct Tile {
   int low, ns;      // seen keys: j < ns, and low <= j <= pmax
   int pmin, pmax;
   int nsb, wb0, nblk;
+  int mb0, mb1;     // blocks mb0 .. mb1 - 1: keys that all rows see
+  int nedge;        // blocks ahead of these in the order that they are taken in
 };
 LOOM_DEV Tile tile_of(const WindowParams& p, int b, int tile, int RT) {
   Tile a;
-  const int n = min(max(p.lens[b], 0), p.S);
-  const int c = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+  // (the same for the workgroup, stated to the compiler: addresses follow from them)
+  const int n = __builtin_amdgcn_readfirstlane(min(max(p.lens[b], 0), p.S));
+  const int c =
+      __builtin_amdgcn_readfirstlane(p.counts ? min(max(p.counts[b], 0), p.T) : p.T);
   a.r0 = tile * RT;
   a.rows = min(RT, c * p.H - a.r0);
   a.p0 = n - c;
@@ -85,8 +90,21 @@ LOOM_DEV Tile tile_of(const WindowParams& p, int b, int tile, int RT) {
   a.ns = min(min(p.sinks, a.low), a.pmax + 1);
   a.nsb = (max(a.ns, 0) + kKeys - 1) / kKeys;
   a.wb0 = max(a.low / kKeys, a.nsb);
-  a.nblk = a.pmax < 0 ? 0 : a.nsb + max(0, a.pmax / kKeys - a.wb0 + 1);
+  const int end = a.pmax < 0 ? a.wb0 : max(a.wb0, a.pmax / kKeys + 1);
+  a.nblk = a.pmax < 0 ? 0 : a.nsb + end - a.wb0;
+  a.mb0 = max(a.wb0, (max(0, a.pmax - p.window + 1) + kKeys - 1) / kKeys);
+  a.mb1 = max(0, a.pmin + 1) / kKeys;
+  if (a.mb1 <= a.mb0) a.mb0 = a.mb1 = end;
+  a.nedge = a.nblk - (a.mb1 - a.mb0);
   return a;
+}
+// The block that is taken i-th: the sinks', those at the window's edges, then those that
+// all rows see.
+LOOM_DEV int tile_block(const Tile& a, int i) {
+  if (i >= a.nedge) return a.mb0 + i - a.nedge;
+  if (i < a.nsb) return i;
+  const int kb = a.wb0 + i - a.nsb;
+  return kb < a.mb0 ? kb : kb + (a.mb1 - a.mb0);
 }
 
 // W / KG waves of 16 QT rows each share 64-key stages of K and V copied by LDS DMA
@@ -161,10 +179,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
     const int x = a.r0 + lr, t = x / H;
     return (((int64_t)b * p.T + t) * p.G + gh) * H + (x - t * H);
   };
-  auto first_key = [&](int blk) {
-    const int i = i0 + blk;
-    return (i < a.nsb ? i : a.wb0 + i - a.nsb) * kKeys;
-  };
+  auto first_key = [&](int blk) { return tile_block(a, i0 + blk) * kKeys; };
 
   auto stK = [&](int s) { return (lds_char_t*)(smem + s * STAGE); };
   auto stV = [&](int s) { return (lds_char_t*)(smem + s * STAGE + K_BYTES); };
@@ -187,7 +202,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
   }
   // (tiles of few rows only: keys of larger ones are shared)
   const bool once = KG == 2 && p.once != 0;
-  auto issue = [&](int s, int blk) {
+  auto issue = [&](int s, int blk) __attribute__((always_inline)) {
     const int kv0 = first_key(blk);
     const uint32_t lk = lds_addr(stK(s)), lv = lds_addr(stV(s));
     const bool whole = kv0 + kKeys - 1 <= a.pmax && (kv0 >= a.low || kv0 + kKeys <= a.ns);
@@ -197,14 +212,14 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
         for (int i = 0; i < K_INSTR; ++i) {
           const int j = wave * K_INSTR + i;
           if (j * 8 < Dr)
-            dma_load16_s(koff[i], kg + kv0, lk + j * 1024);
+            dma_load16_s(koff[i], kg + kv0, __builtin_amdgcn_readfirstlane(lk + j * 1024));
           else
-            dma_load16(loom_zero_kb + lane * 4, lk + j * 1024);
+            dma_load16(loom_zero_kb + lane * 4, __builtin_amdgcn_readfirstlane(lk + j * 1024));
         }
       }
 #pragma unroll
       for (int i = 0; i < V_INSTR; ++i)
-        dma_load16_s(voff[i], vg + (int64_t)kv0 * Dr, lv + (wave * V_INSTR + i) * 1024);
+        dma_load16_s(voff[i], vg + (int64_t)kv0 * Dr, __builtin_amdgcn_readfirstlane(lv + (wave * V_INSTR + i) * 1024));
       return;
     }
     const int ln = KG == 2 ? lane : fresh(lane);
@@ -215,9 +230,9 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
         const int d = j * 8 + ln / 8;
         const int key = min(kv0 + ((ln % 8) ^ wk_swz(d)) * 8, S - 8);
         const uint16_t* from = kg + (int64_t)d * S + key;
-        if (j * 8 >= Dr) dma_load16(loom_zero_kb + ln * 4, lk + j * 1024);
-        else if (once) dma_once16(from, lk + j * 1024);
-        else dma_load16(from, lk + j * 1024);
+        if (j * 8 >= Dr) dma_load16(loom_zero_kb + ln * 4, __builtin_amdgcn_readfirstlane(lk + j * 1024));
+        else if (once) dma_once16(from, __builtin_amdgcn_readfirstlane(lk + j * 1024));
+        else dma_load16(from, __builtin_amdgcn_readfirstlane(lk + j * 1024));
       }
     }
 #pragma unroll
@@ -228,14 +243,14 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
       const bool seen = key <= a.pmax && (key >= a.low || key < a.ns);
       const void* from = seen ? (const void*)((const char*)(vg + (int64_t)kv0 * Dr) + voff[i])
                               : (const void*)(loom_zero_kb + ln * 4);
-      if (once) dma_once16(from, lv + j * 1024);
-      else dma_load16(from, lv + j * 1024);
+      if (once) dma_once16(from, __builtin_amdgcn_readfirstlane(lv + j * 1024));
+      else dma_load16(from, __builtin_amdgcn_readfirstlane(lv + j * 1024));
     }
   };
   // ---- KREG: K pieces of block `blk` into registers, then into stage s
   const rsrc_t krs = make_rsrc(kg, KREG ? (uint32_t)(Dr * S * 2) : 0u);
   u32x4_t kr[KREG ? K_INSTR : 1];
-  auto kload = [&](int blk) {
+  auto kload = [&](int blk) __attribute__((always_inline)) {
     const int kv0 = first_key(blk);
 #pragma unroll
     for (int i = 0; i < K_INSTR; ++i) {
@@ -245,7 +260,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
                          : u32x4_t{0u, 0u, 0u, 0u};
     }
   };
-  auto kstore = [&](int s) {
+  auto kstore = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < K_INSTR; ++i)
       *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(
@@ -313,8 +328,19 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
   // below 2^-14 (bf16 has fp32's exponents)
   constexpr float kLift = F16 ? 7.f : 0.f, kRise = kLift + 8.f;
 
-  auto compute = [&](int s, int blk) {
-    const int kv0 = first_key(blk);
+  // Whether rows of the wave see other keys of a half than other rows of the tile do.
+  // (Rows of one token see the same; and what no row sees lies there as zeros.)
+  auto mixed_half = [&](int k0) __attribute__((always_inline)) {
+    return a.pmin != a.pmax &&
+           (k0 + 31 > pw0 || (k0 <= pw1 - p.window && k0 + 31 >= a.low));
+  };
+  constexpr uint32_t kInf = F16 ? 0x7c00 : 0x7f80;
+  bool odd = false;         // such a half held an infinity or NaN
+
+  // The wave's rows against a stage's keys; EDGE: some of them are not seen by some rows.
+  // (Without the edges' branches the other blocks' products and exponentials overlap.)
+  auto compute = [&](int s, int kv0, auto any) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(any)::value;
     const lds_char_t* ks = stK(s);
     const lds_char_t* vs = stV(s);
 #pragma unroll
@@ -322,8 +348,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
       const int h = KG == 1 ? hh : kh;
       const int k0 = kv0 + 32 * h;              // this half's keys: k0 .. k0 + 31
       // a half that no row of the wave sees
-      if (k0 > pw1 || (k0 + 31 <= pw0 - p.window && k0 >= p.sinks)) continue;
-      const bool edge = k0 + 31 > pw0 || (k0 <= pw1 - p.window && k0 + 31 >= p.sinks);
+      if (EDGE && (k0 > pw1 || (k0 + 31 <= pw0 - p.window && k0 >= p.sinks))) continue;
       // ---- S^T = K^T Q^T; st[j][qt][i] = score of key k0 + 16 j + 4 g + i
       f32x4_t st[2][QT];
 #pragma unroll
@@ -357,7 +382,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             st[j][qt][i] = __builtin_fmaf(st[j][qt][i], c2, -m_run[qt]);
-        if (edge) {
+        if constexpr (EDGE) {
           // (no short circuits: a branch for every key takes longer than a comparison)
           const int ps = fresh(pos[qt]), lo = max(0, ps - p.window + 1);
           const int at0 = k0 + 4 * g - lo, n = max(0, ps + 1 - lo), sk = min(p.sinks, ps + 1) - lo;
@@ -421,15 +446,12 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
         const u32x2_t hi = lds_read_tr16(q + 16 * VROW);    // keys k0 + 16 + 4 g + 0..3
         return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
       };
-      // Keys that some rows of the tile see and the wave's do not all: a weight of zero times
-      // an infinity or NaN of theirs would reach the others.  Such values are looked
-      // for (the largest magnitude's bits, two elements at a time) and, where there
-      // are any, every row takes its own product, V's elements that it does not see
-      // as zeros.
-      // (rows of one token see the same; and what no row sees lies there as zeros)
-      const bool mixed = a.pmin != a.pmax &&
-                         (k0 + 31 > pw0 || (k0 <= pw1 - p.window && k0 + 31 >= a.low));
-      if (mixed) {
+      // Keys that some rows of the tile see and the wave's do not all: a weight of zero
+      // times an infinity or NaN of theirs would reach rows that do not see them.  Such
+      // values are looked for (the largest magnitude's bits, two elements at a time);
+      // where there are any they count as zeros here, and the rows that see them get them
+      // behind the loop.
+      if (EDGE && mixed_half(k0)) {
         typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
         u16x2_t top = u16x2_t{0, 0};
 #pragma unroll
@@ -441,34 +463,21 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
             top = __builtin_elementwise_max(top,
                                             __builtin_bit_cast(u16x2_t, w[x] & 0x7fff7fffu));
         }
-        constexpr uint16_t kInf = F16 ? 0x7c00 : 0x7f80;
         if (__builtin_amdgcn_ballot_w64(top[0] >= kInf || top[1] >= kInf) != 0) {
-          const int key0 = fresh(k0 + 4 * g);
-#pragma unroll 1
-          for (int c = 0; c < 16; ++c)
+          odd = true;
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              const int pc = __builtin_amdgcn_readlane(pos[qt], c);
-              u32x4_t keep;
+          for (int dt = 0; dt < DT; ++dt) {
+            u32x4_t vf = v_op(dt);
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                uint32_t m = 0;
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  const int key = key0 + 16 * (x >> 1) + 2 * (x & 1) + y;
-                  m |= (key <= pc) & ((key > pc - p.window) | (key < p.sinks)) ? 0xffffu << (16 * y)
-                                                                               : 0u;
-                }
-                keep[x] = m;
-              }
-#pragma unroll
-              for (int dt = 0; dt < DT; ++dt) {
-                const f32x4_t o = mfma16t<F16>(v_op(dt) & keep, pf[qt], ot[dt][qt]);
-                if (r == c) ot[dt][qt] = o;
-                // (one at a time: the registers of several would be taken from the others)
-                __builtin_amdgcn_sched_barrier(0);
-              }
+            for (int x = 0; x < 4; ++x) {
+              // (an exponent of all ones carries into the sign's place)
+              const uint32_t bad =
+                  ((vf[x] & kInf * 0x10001u) + (F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+              vf[x] &= ~((bad >> 15) * 0xffffu);
             }
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) ot[dt][qt] = mfma16t<F16>(vf, pf[qt], ot[dt][qt]);
+          }
           continue;
         }
       }
@@ -483,44 +492,77 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
 
   // ---- pipeline: NS stages (the first NS-1 issued above), waits placed by hand.  (Not
   // unrolled over the stages: their addresses would not leave registers enough.)
-  int s = 0;
-#pragma unroll 1
-  for (int it = 0; it < nblk; ++it) {
-    const int younger = min(NS - 2, nblk - 1 - it);
-    if (younger >= 1) LOOM_WAIT_VMCNT(LPW);
+  auto landed = [&](int it) __attribute__((always_inline)) {
+    if (min(NS - 2, nblk - 1 - it) >= 1) LOOM_WAIT_VMCNT(LPW);
     else LOOM_WAIT_VMCNT(0);
     // this wave's reads of the stage that is overwritten next, and KREG's stores
     LOOM_WAIT_LGKM0();
     barrier_nofence();
-    if constexpr (QDMA) {
-      if (it == 0) {
+  };
+  if constexpr (QDMA) {
+    if (nblk > 0) {
+      landed(0);
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          const int lr = rw0 + 16 * qt + r;
+      for (int qt = 0; qt < QT; ++qt) {
+        const int lr = rw0 + 16 * qt + r;
 #pragma unroll
-          for (int ds = 0; ds < DSTEPS; ++ds) {
-            const u32x4_t raw = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
-                sQ + lr * QROW + ((4 * ds + g) ^ wq_swz<D>(lr)) * 16);
-            qf[ds][qt] = ds * 32 + g * 8 < Dr ? raw : u32x4_t{0u, 0u, 0u, 0u};
-          }
+        for (int ds = 0; ds < DSTEPS; ++ds) {
+          const u32x4_t raw = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
+              sQ + lr * QROW + ((4 * ds + g) ^ wq_swz<D>(lr)) * 16);
+          qf[ds][qt] = ds * 32 + g * 8 < Dr ? raw : u32x4_t{0u, 0u, 0u, 0u};
         }
       }
     }
+  }
+  int s = 0;
+  auto step = [&](int it, auto any) __attribute__((always_inline)) {
+    landed(it);
     const int to = s == 0 ? NS - 1 : s - 1;     // the stage of block it - 1
     const bool ahead = it + NS - 1 < nblk;
     if constexpr (KREG) {
       if (ahead) kload(it + NS - 1);
     }
     if (ahead) issue(to, it + NS - 1);
-    if (active) compute(s, it);
+    if (active) compute(s, first_key(it), any);
     if constexpr (KREG) {
       if (ahead) kstore(to);
     }
     s = s == NS - 1 ? 0 : s + 1;
-  }
+  };
+  // the edges, then, by code without their branches, the rest
+  const int nedge = min(max(a.nedge - i0, 0), nblk);
+#pragma unroll 1
+  for (int it = 0; it < nedge; ++it) step(it, std::true_type{});
+#pragma unroll 1
+  for (int it = nedge; it < nblk; ++it) step(it, std::false_type{});
 
   // (without a block nothing has waited for the Q copies)
   if (nblk == 0) LOOM_WAIT_VMCNT(0);
+  // ---- infinities and NaN that counted as zeros, to the rows that see them
+  if (odd) {
+#pragma unroll 1
+    for (int it = 0; it < nblk; ++it) {
+#pragma unroll 1
+      for (int x = 0; x < kKeys; ++x) {
+        const int key = first_key(it) + x, k0 = key & ~31;
+        if ((KG == 2 && (x >> 5) != kh) || !mixed_half(k0) || key > a.pmax ||
+            (key < a.low && key >= a.ns))
+          continue;
+        const uint16_t* from = vg + (int64_t)key * Dr;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w = from[min(16 * dt + 4 * g + i, Dr - 1)];
+            if ((w & kInf) != kInf) continue;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              if ((key <= pos[qt]) & ((key > pos[qt] - p.window) | (key < p.sinks)))
+                ot[dt][qt][i] += lo16<F16>(w);
+          }
+      }
+    }
+  }
   // ---- KG 2: the pair's second wave hands its state over through the idle stages
   // (lane by lane: both hold the same rows and columns); a half that saw no key (l =
   // 0) takes no part
