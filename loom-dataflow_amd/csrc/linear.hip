@@ -8,6 +8,14 @@
 //     S_t = a S_(t-1) + k_t v_t^T,   out_t = scale S_t^T q_t,   S_(-1) = state or 0;
 //   sequence b has c = clamp(counts[b], 0, T) tokens (all T without counts), state_out
 //   is S_(c-1), and out's rows t >= c are left as they are.
+//
+// gfx950 mapping.  A prompt reads 2 (H D + D + E) and writes 2 H E bytes a token and KV
+// head for 4 H D E operations: bound by HBM where the states stay on the chip, as they do
+// here, in the accumulators of the waves that walk a head's chunks (linear_chunk_kernel).
+// Where heads are fewer than CUs the tokens are cut into segments: a first launch leaves
+// the states of their stretches, from k and v alone, a second one walks every segment
+// from the sum of those before it.  One token is a stream of the states, read and written
+// once (linear_step_kernel).
 #include "common.h"
 
 #include <cmath>
@@ -101,6 +109,15 @@ LOOM_DEV const char* uniform(const char* p) {
 // Rounding: S and P to 16 bits as operands, each once; a^(C-1-j) v_j as a sum of three
 // bf16 or two f16 numbers, so that the state keeps fp32's accuracy.  f16 operands are
 // scaled by powers of two where they leave its range.
+// What bounds it: a chunk of 128 x 128 takes a CU 1.4 us by itself (24 + 8 products of 16
+// cycles and 200 other vector instructions to each of 8 waves), its 32 KB 1.6 us at the
+// rate of a large copy.  B8 G32 of 1024 to 4096 tokens 201 us (738 MB, 3.7 TB/s: the
+// longest prompt's 128 chunks in a row, while the CUs of shorter ones idle), B1 G32 of
+// 32768 373 us (1.08 GB, and k, v once more in the first launch, 0.47 GB).  Measured:
+// chunks of 64 tokens by four waves 366 us, by eight 249 (the 64 x 64 scores cost more than
+// they save); chunks of 32 by four waves of 32 columns 251 to 257, by eight of 16 216;
+// direct reads of 16 bytes (not two of 8, which the compiler joined and took apart again
+// by moves) and one branch to a chunk's copies 201.  A fourth stage: no change.
 // ONLY_STATE: a segment's own state from zero (the first's from the initial state), which
 // later segments start from.
 template <int DK, int W, bool F16, bool ONLY_STATE>
@@ -521,7 +538,11 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
   }
 }
 
-// One token.  L lanes of four columns to a row of the state, 256 / L rows at once.
+// One token.  L lanes of four columns to a row of the state, 256 / L rows at once, 16 of
+// them in flight to a thread.  The state is stored past the caches: a program's layers
+// have more of it than these hold, so it comes from memory the next time (B64 G32 128 x 128,
+// three states in turn: 268 MB in 44.7 us, 6.0 TB/s, against 59.3 with ordinary stores; one
+// state over and over 44.5 against 40.2).
 template <bool F16>
 __global__ void __launch_bounds__(256) linear_step_kernel(LinearParams p, int L) {
   __shared__ float s_q[256], s_k[256];
@@ -593,10 +614,13 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t E, int64_t T)
   s.waves = E <= 64 ? 4 : 8;
   s.nsl = (int)cdiv64(E, 16 * s.waves);
   const int64_t wgs = B * G * H * s.nsl, chunks = cdiv64(T, kC);
-  // workgroups that run at once
+  // Segments of at least four chunks, as many workgroups as run at once (16 heads of T512:
+  // segments of 8 chunks 26.2 us, of 4 21.0, of 2 22.4; 256 heads of prompts of 1024 to 4096
+  // cut in two 292 us, whole 216: the first launch costs more than the balance gains)
   const int64_t slots = s.waves == 4 && D <= 128 ? 512 : 256;
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>({slots / wgs, chunks / 4, 64}));
-  // two stretches to a segment where its first launch would leave most of the CUs idle
+  // two stretches to a segment where its first launch would leave most of the CUs idle (the
+  // 16 heads 26.2 us against 28.8; 36 heads of 7 segments 38.4 against 35.6)
   s.sub = want > 1 && wgs * (want - 1) < 128 ? 2 : 1;
   s.cps = (int)cdiv64(chunks, want * s.sub);
   s.nseg = (int)cdiv64(chunks, s.cps * s.sub);
