@@ -16,7 +16,7 @@
 // keys that any of its rows sees: the sinks', those at the edges of the window (masked),
 // then those that all rows see, by code of its own without the masks' branches.  Taken
 // together they cost those blocks the overlap of products and exponentials (window of
-// 4096 over 8192 tokens of 64 heads 1290 us against 1087; 1.01 PFLOP/s, as attention.hip
+// 4096 over 8192 tokens of 64 heads 1290 us against 1080; 1.01 PFLOP/s, as attention.hip
 // without a window; prompts of 4096 tokens of 128 heads under 1024 + 4 keys 379 against
 // 332: a sixth of its blocks are edges).  Few rows over many keys (a step) share a tile's
 // blocks between workgroups, which a second launch joins; a step is bound by streaming
