@@ -113,11 +113,12 @@ LOOM_DEV const char* uniform(const char* p) {
 // cycles and 200 other vector instructions to each of 8 waves), its 32 KB 1.6 us at the
 // rate of a large copy.  B8 G32 of 1024 to 4096 tokens 201 us (738 MB, 3.7 TB/s: the
 // longest prompt's 128 chunks in a row, while the CUs of shorter ones idle), B1 G32 of
-// 32768 373 us (1.08 GB, and k, v once more in the first launch, 0.47 GB).  Measured:
+// 32768 376 us (1.08 GB, and k, v once more in the first launch, 0.47 GB).  Measured:
 // chunks of 64 tokens by four waves 366 us, by eight 249 (the 64 x 64 scores cost more than
 // they save); chunks of 32 by four waves of 32 columns 251 to 257, by eight of 16 216;
 // direct reads of 16 bytes (not two of 8, which the compiler joined and took apart again
-// by moves) and one branch to a chunk's copies 201.  A fourth stage: no change.
+// by moves) and one branch to a chunk's copies 201.  A fourth stage: no change.  k's
+// transposed reads without their bank conflicts, for 32 more vector instructions: 206.
 // ONLY_STATE: a segment's own state from zero (the first's from the initial state), which
 // later segments start from.
 template <int DK, int W, bool F16, bool ONLY_STATE>
