@@ -57,7 +57,12 @@ LOOM_DEV Decay split_decay(double x) {
   const float hi = (float)x;
   return Decay{hi, (float)(x - (double)hi)};
 }
-LOOM_DEV float decayed(float s, const Decay& a) { return __builtin_fmaf(s, a.hi, s * a.lo); }
+// a s + x: an infinite s stays what it is (its product with lo would be NaN, or the other
+// infinity); one more instruction, which a step's stream of states hides
+LOOM_DEV float decayed_plus(float s, const Decay& a, float x) {
+  const float f = __builtin_amdgcn_fmed3f(s, -__FLT_MAX__, __FLT_MAX__);
+  return __builtin_fmaf(s, a.hi, __builtin_fmaf(f, a.lo, x));
+}
 
 // A row's 16-byte chunks are XORed with this, so that both the 16 rows of a direct
 // read (one chunk each) and the 8 consecutive rows of a transposed read's pass (a pair
@@ -589,7 +594,7 @@ __global__ void __launch_bounds__(256) linear_step_kernel(LinearParams p, int L)
         const float k = s_k[d], q = s_q[d];
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          x[i][y] = __builtin_fmaf(x[i][y], a.hi, __builtin_fmaf(x[i][y], a.lo, k * v[y]));
+          x[i][y] = decayed_plus(x[i][y], a, k * v[y]);
           o[y] = __builtin_fmaf(q, x[i][y], o[y]);
         }
         store_stream(reinterpret_cast<f32x4_t*>(at + (int64_t)d * E), x[i]);
