@@ -527,10 +527,12 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
         }
         if constexpr (F16) o[it] *= 1.f / ps;
         // ---- o[it][e] is token 16 it + r, column col0 + 4 g4 + e
+        // (stated to lie in global memory: the counted waits at a chunk's start rely on the
+        // order of the copies and these stores, which flat ones need not keep)
         char* to = const_cast<char*>(uniform(ob)) + ooff;
         ob += ostep;
         if (16 * it + r < left && col0 + 4 * g4 < E)
-          *reinterpret_cast<u32x2_t*>(to) =
+          *(__attribute__((address_space(1))) u32x2_t*)to =
               u32x2_t{pack2<F16>(o[it][0], o[it][1]), pack2<F16>(o[it][2], o[it][3])};
       }
     }
