@@ -395,7 +395,9 @@ size_t loom_hip_linear_attention_workspace_bytes(int64_t B, int64_t G, int64_t H
  *   S_t = a S_(t-1) + k_t v_t^T,   out[b,t,g,h] = scale S_t^T q_t
  * for the first c = clamp(counts[b], 0, T) tokens (T with counts null);
  * state_out[b,g,h] = S_(c-1), and out's rows t >= c are left as they are.  What
- * tokens behind c, or later than a row, hold does not reach it.  `scale` is finite
+ * tokens behind c, or later than a row, hold does not reach it.  Infinities and NaN
+ * among q, k, v and the states give what the recurrence gives (a rounded to fp32: 0
+ * times an infinity, as of a below 2^-149, is NaN).  `scale` is finite
  * and positive, D and E multiples of 8 up to 256 (else LOOM_HIP_EUNSUP), B*G*H at
  * most 2^20, T at most 2^29.  out, state_out and the workspace overlap neither the
  * other tensors nor each other, except that state_out may be state.  Equal calls

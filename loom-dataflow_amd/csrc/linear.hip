@@ -82,6 +82,35 @@ LOOM_DEV float f16_scale(float m) {
   const int e = max(-60, (int)(__float_as_uint(m) >> 23) - 127);
   return pow2i(13 - e);
 }
+// the largest magnitude, NaN if one is NaN
+LOOM_DEV float largest(float x, float y, float z) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(y), fabsf(z)), x);
+}
+// What keeps a NaN once one of eight 16-bit numbers was infinite or NaN (bf16: or beyond
+// 2^121), two numbers at a time.  Infinite and NaN bf16 bits are NaN as f16.
+template <bool F16>
+LOOM_DEV f16x2_t odd16(f16x2_t odd, const u32x4_t& x) {
+  // (by value: a cast of an element of the vector itself reads the first one)
+  auto half2 = [](uint32_t w) { return __builtin_bit_cast(f16x2_t, w); };
+  if constexpr (F16) {
+    const f16x2_t zero = f16x2_t{0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd = __builtin_elementwise_fma(half2(x[i]), zero, odd);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+      odd = __builtin_elementwise_maximum(__builtin_elementwise_maximum(odd, half2(x[i])),
+                                          half2(x[i + 1]));
+  }
+  return odd;
+}
+// ones in the halves of w that are neither infinite nor NaN (an exponent of all ones carries
+// into the sign's place)
+template <bool F16>
+LOOM_DEV uint32_t finite16(uint32_t w) {
+  const uint32_t inf = F16 ? 0x7c007c00u : 0x7f807f80u, one = F16 ? 0x04000400u : 0x00800080u;
+  return ~(((((w & inf) + one) & 0x80008000u) >> 15) * 0xffffu);
+}
 LOOM_DEV float finite_abs(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
 
 // A value that the compiler does not know to be x: what rare paths compute from it is
@@ -124,10 +153,13 @@ LOOM_DEV const char* uniform(const char* p) {
 // direct reads of 16 bytes (not two of 8, which the compiler joined and took apart again
 // by moves) and one branch to a chunk's copies 201.  A fourth stage: no change.  k's
 // transposed reads without their bank conflicts, for 32 more vector instructions: 206.
+// Infinities and NaN: every chunk is looked over while the one before it is worked on; from
+// one that holds any on, a second loop takes the tokens one by one (by_token), which are the
+// recurrence itself.
 // ONLY_STATE: a segment's own state from zero (the first's from the initial state), which
 // later segments start from.
 template <int DK, int W, bool F16, bool ONLY_STATE>
-__global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
+__global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !F16) ? 4 : 2)
     linear_chunk_kernel(LinearParams p) {
   constexpr int SL = 16 * W;                    // columns of a workgroup
   constexpr int KROW = DK * 2, VROW = SL * 2;
@@ -144,6 +176,7 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
   __shared__ __attribute__((aligned(16))) u32x4_t s_p[ONLY_STATE ? 1 : 2 * kIT * 64];
   __shared__ float s_pow[kC + 1];
   __shared__ float s_ps[2][kIT];                // f16: what a tile of P was scaled by
+  __shared__ int s_odd[2];                      // the last chunk found to hold infinities or NaN
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -249,11 +282,20 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
 
   const float lg = p.g[gh];
   if (tid <= kC) s_pow[tid] = (float)decay_pow(lg, tid);
+  if (tid < 2) s_odd[tid] = -1;
+  Decay one = split_decay(decay_pow(lg, 1));
+  one.hi = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(one.hi)));
+  one.lo = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(one.lo)));
+  // Powers that fp32 holds as zero are its smallest number where the decay is not zero, so
+  // that an infinite state stays infinite; a finite one is then 2^-149 of itself, not zero.
+  const float least = __uint_as_float(one.hi > 0.f ? 1u : 0u);
   // over a whole chunk, and over the last one.  A rounded factor near 1, applied over and
   // over, would be off by its rounding times the chunks that a head remembers: what the
   // factors so far are off by (relatively) is kept, and each makes up for it.
-  const Decay full = split_decay(decay_pow(lg, kC));
-  const Decay last = split_decay(decay_pow(lg, tokens - (nch - 1) * kC));
+  Decay full = split_decay(decay_pow(lg, kC));
+  Decay last = split_decay(decay_pow(lg, tokens - (nch - 1) * kC));
+  full.hi = fmaxf(full.hi, least);
+  last.hi = fmaxf(last.hi, least);
   const float inv_full = full.hi > 1e-30f ? 1.f / full.hi : 0.f;
   float owed = 0.f;
 
@@ -295,8 +337,9 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
     const int to = seg * p.sub;
 #pragma unroll 1
     for (int u = seg == 0 ? 0 : 1; u <= to; ++u) {
-      const float w = (float)exp((double)(to - u) * (double)sublen *
-                                 (double)(lg < -1e30f ? -1e30f : lg));
+      const float w = fmaxf((float)exp((double)(to - u) * (double)sublen *
+                                       (double)(lg < -1e30f ? -1e30f : lg)),
+                            least);
       f32x4_t x[DT];
       read_state(p.ws + (bgh * slots + u) * sz, x);
 #pragma unroll
@@ -312,7 +355,7 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
 #pragma unroll
   for (int x = 0; x < 8; ++x) w[x] = s_pow[kC - 1 - token(x)];
 #pragma unroll
-  for (int it = 0; it < kIT; ++it) rise[it] = p.scale * s_pow[16 * it + r + 1];
+  for (int it = 0; it < kIT; ++it) rise[it] = fmaxf(p.scale * s_pow[16 * it + r + 1], least);
   // A wave's part of P^T: of a tile of queries, the half of 16 tokens, in f16 both (which
   // share what they are scaled by).  Of 8 waves (in f16 4) they take turns.
   const int pit = F16 ? wave & 1 : (wave >> 1) & 1, pt = F16 ? 0 : wave & 1;
@@ -349,8 +392,9 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
     const u32x2_t hi = lds_read_tr16(at + 16 * (N * 2));    // (the same swizzle)
     return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
   };
-  // P^T of the chunk in a stage, as the operands that every wave reads, into s_p[to]
-  auto build_p = [&](const lds_char_t* st, int to) {
+  // P^T of chunk ci in a stage, as the operands that every wave reads, into s_p[ci & 1]
+  auto build_p = [&](const lds_char_t* st, int ci) {
+    const int to = ci & 1;
     f32x4_t x[PT] = {};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -358,6 +402,11 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
 #pragma unroll
       for (int t = 0; t < PT; ++t) x[t] = mfma16t<F16>(row_op(st + Q_BYTES, pt + t, ks), q, x[t]);
     }
+    // an infinity or NaN of q or k makes all its scores so, those of tokens not seen too
+    float big = 0.f;
+#pragma unroll
+    for (int t = 0; t < PT; ++t) big = largest(largest(big, x[t][0], x[t][1]), x[t][2], x[t][3]);
+    if (__builtin_amdgcn_ballot_w64(!(big < INFINITY)) != 0 && lane == 0) s_odd[to] = ci;
 #pragma unroll
     for (int t = 0; t < PT; ++t)
 #pragma unroll
@@ -381,29 +430,162 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
       reinterpret_cast<u32x2_t*>(&s_p[(to * kIT + pit) * 64 + lane])[pt + t] =
           u32x2_t{pack2<F16>(x[t][0], x[t][1]), pack2<F16>(x[t][2], x[t][3])};
   };
-  if constexpr (!ONLY_STATE) {
-    if (nch > 0) {
-      LOOM_WAIT_VMCNT(0);
+  // Whether chunk ci in a stage holds infinities or NaN: of k and v (without scores; the
+  // parts that this wave copied), or of v, by the waves whose turn at P^T comes next.  A
+  // chunk ahead, so that its work has no branch in its midst, which took 8% (the checks
+  // take 1 to 2).
+  auto look = [&](const lds_char_t* st, int ci) {
+    f16x2_t odd = f16x2_t{0, 0};
+    auto piece = [&](int at) {
+      const u32x4_t x = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
+          st + Q_BYTES + at * 1024 + lane * 16);
+      odd = odd16<F16>(odd, x);
+    };
+    if constexpr (ONLY_STATE) {
+#pragma unroll
+      for (int i = 0; i < QK_INSTR; ++i)
+        if (QK_ALL % W == 0 || wave + W * i < QK_ALL) piece(wave + W * i);
+      piece(QK_ALL + wave);
+    } else {
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) piece(QK_ALL + (wave - turn * (W / TURNS)) * TURNS + i);
+    }
+    if (__builtin_amdgcn_ballot_w64(odd[0] != odd[0] || odd[1] != odd[1]) != 0 && lane == 0)
+      s_odd[ci & 1] = ci;
+  };
+  if (nch > 0) {
+    LOOM_WAIT_VMCNT(0);
+    if constexpr (ONLY_STATE) {
+      look((lds_char_t*)smem, 0);
+    } else {
       barrier_nofence();
       if (turn == 0) build_p((lds_char_t*)smem, 0);
+      if (turn == TURNS - 1) look((lds_char_t*)smem, 0);
     }
   }
+  // A chunk that holds an infinity or NaN, token by token as the recurrence has it, in
+  // fp32: products with zeros and with the numbers that v is split into would make NaN of
+  // infinities, and reach rows ahead of theirs.  Returns which of this lane's outputs are
+  // not finite, two bits each: 1 inf, 2 -inf, 3 NaN.
+  auto by_token = [&](const lds_char_t* st, int n) __attribute__((always_inline)) {
+    uint32_t bad = 0;
+    const int ln = fresh(lane), r = ln & 15, g4 = ln >> 4;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const lds_char_t* const kr = st + Q_BYTES + j * KROW;
+      const lds_char_t* const vr = st + Q_BYTES + K_BYTES + j * VROW;
+      const float v = lo16<F16>(*reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(
+          vr + ((wave * 2 + (r >> 3)) ^ row_swz<SL>(j)) * 16 + (r & 7) * 2));
+      float o = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const int at = ((4 * (dt >> 1) + g4) ^ row_swz<DK>(j)) * 16 + 8 * (dt & 1);
+        const u32x2_t k = *reinterpret_cast<const __attribute__((address_space(3))) u32x2_t*>(kr + at);
+        u32x2_t q = u32x2_t{0u, 0u};
+        if constexpr (!ONLY_STATE)
+          q = *reinterpret_cast<const __attribute__((address_space(3))) u32x2_t*>(st + j * KROW + at);
+        lds_order();      // (one tile's reads at a time: registers)
+        if (32 * (dt >> 1) + 8 * g4 >= D) continue;     // (rows past D stay zeros)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float ki = i & 1 ? hi16<F16>(k[i >> 1]) : lo16<F16>(k[i >> 1]);
+          s[dt][i] = decayed_plus(s[dt][i], one, ki * v);
+          if constexpr (!ONLY_STATE)
+            o = __builtin_fmaf(s[dt][i], i & 1 ? hi16<F16>(q[i >> 1]) : lo16<F16>(q[i >> 1]), o);
+        }
+      }
+      if constexpr (!ONLY_STATE) {
+        o += __shfl_xor(o, 16);
+        o += __shfl_xor(o, 32);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {                   // column 4 g4 + e of token j
+          const float x = __shfl(o, 4 * g4 + e);
+          const uint32_t is = x == INFINITY ? 1u : x == -INFINITY ? 2u : x != x ? 3u : 0u;
+          if (r == (j & 15)) bad |= is << (2 * (4 * (j >> 4) + e));
+        }
+      }
+    }
+    return bad;
+  };
   int stage = 0;
-  for (int ci = 0; ci < nch; ++ci) {
-    char* const st = smem + stage * STAGE;
-    lds_char_t* const lq = (lds_char_t*)st;
-    lds_char_t* const lk = (lds_char_t*)(st + Q_BYTES);
-    lds_char_t* const lv = (lds_char_t*)(st + Q_BYTES + K_BYTES);
+  f32x4_t o[kIT];
+  u32x4_t vf;               // v as an operand
+  // ---- S^T Q^T of the state before a chunk, times scale a^(i+1), into o.  Products that
+  // wait for each other are kept apart; between: what is worked out among them, in fours
+  auto ahead_of = [&](const lds_char_t* lq, auto between) __attribute__((always_inline)) {
+    float sc = 1.f;
+    if constexpr (F16) {
+      float mx = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, finite_abs(s[dt][i]));
+      sc = f16_scale(mx);
+    }
+    const float back = F16 ? 1.f / sc : 1.f;
+#pragma unroll
+    for (int it = 0; it < kIT; ++it) o[it] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      f32x4_t x = s[2 * ks], y = s[2 * ks + 1];
+      if constexpr (F16) {
+        x *= sc;
+        y *= sc;
+      }
+      const u32x4_t sp = u32x4_t{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]),
+                                 pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3])};
+#pragma unroll
+      for (int it = 0; it < kIT; ++it) o[it] = mfma16t<F16>(sp, row_op(lq, it, ks), o[it]);
+#pragma unroll
+      for (int y4 = 4 * ks / KS; y4 < 4 * (ks + 1) / KS; ++y4) between(y4);
+    }
+#pragma unroll
+    for (int it = 0; it < kIT; ++it)
+      o[it] *= F16 ? fmaxf(rise[it] * back, least) : rise[it];
+  };
+  // ---- V^T P^T of the chunk's own tokens, and its outputs
+  auto finish = [&](int ci, auto is_odd, uint32_t bad) __attribute__((always_inline)) {
     const int left = tokens - ci * kC;
+#pragma unroll
+    for (int it = 0; it < kIT; ++it) {
+      const u32x4_t pf = s_p[((ci & 1) * kIT + it) * 64 + lane];
+      const float ps = F16 ? s_ps[ci & 1][it] : 1.f;
+      if constexpr (F16) o[it] *= ps;
+      o[it] = mfma16t<F16>(vf, pf, o[it]);
+      if constexpr (F16) o[it] *= 1.f / ps;
+      if constexpr (decltype(is_odd)::value) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t is = bad >> (2 * (4 * it + e)) & 3u;
+          o[it][e] = is == 0 ? o[it][e] : is == 1 ? INFINITY : is == 2 ? -INFINITY : NAN;
+        }
+      }
+      // ---- o[it][e] is token 16 it + r, column col0 + 4 g4 + e
+      char* to = const_cast<char*>(uniform(ob)) + ooff;
+      ob += ostep;
+      if (16 * it + r < left && col0 + 4 * g4 < E)
+        *(__attribute__((address_space(1))) u32x2_t*)to =
+            u32x2_t{pack2<F16>(o[it][0], o[it][1]), pack2<F16>(o[it][2], o[it][3])};
+    }
+  };
+  // The start of chunk ci: its copies have landed, those of chunk ci + 2 set out, and chunk
+  // ci + 1's scores are built.  Returns whether it holds infinities or NaN (the same in
+  // every wave).
+  lds_char_t* lq = nullptr;         // where the chunk lies
+  float a = 0.f;                    // its decay
+  auto begin = [&](int ci) __attribute__((always_inline)) {
+    const int left = tokens - ci * kC;
+    lq = (lds_char_t*)(smem + stage * STAGE);
     lds_order();
     // the copies of the next chunk; the stores of the one before are younger
     if (stores && ci > 0) LOOM_WAIT_VMCNT(STORES);
     else LOOM_WAIT_VMCNT(0);
     LOOM_WAIT_LGKM0();
     barrier_nofence();
+    const int flag = s_odd[ci & 1];
     if (ci + NS - 1 < nch) issue(stage == 0 ? NS - 1 : stage - 1);
     stage = stage == NS - 1 ? 0 : stage + 1;
-    float a = __builtin_fmaf(full.hi, owed, full.hi);
+    a = __builtin_fmaf(full.hi, owed, full.hi);
     owed = __builtin_fmaf((full.hi - a) + full.lo, inv_full, owed);
     if (left < kC) {          // the last, partial chunk
       a = __builtin_fmaf(last.hi, owed, last.hi);
@@ -411,13 +593,23 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
 #pragma unroll
       for (int x = 0; x < 8; ++x) w[x] = s_pow[max(0, left - 1 - (16 * (x >> 2) + j0 + (x & 3)))];
     }
-    if constexpr (!ONLY_STATE) {
-      if (ci + 1 < nch && turn == (ci + 1) % TURNS)
-        build_p((lds_char_t*)(smem + stage * STAGE), ~ci & 1);
+    if (ci + 1 < nch) {
+      const lds_char_t* const next = (lds_char_t*)(smem + stage * STAGE);
+      if constexpr (!ONLY_STATE)
+        if (turn == (ci + 1) % TURNS) build_p(next, ci + 1);
+      if (ONLY_STATE || turn == (ci + 2) % TURNS) look(next, ci + 1);
     }
+    return __builtin_amdgcn_readfirstlane(flag) == ci;
+  };
+  // (One way out of the loop, at its end: with another the state would be copied in it.)
+  int ci = 0;
+  bool go = nch > 0 && !begin(0);
+#pragma unroll 1
+  while (go) {
+    const lds_char_t *const lk = lq + Q_BYTES, *const lv = lk + K_BYTES;
 
     // ---- v as an operand, and a^(C-1-j) v as a sum of 16-bit numbers
-    const u32x4_t vf = col_op(lv, VC{}, wave * 2 + (c4 >> 1), c4 & 1);
+    vf = col_op(lv, VC{}, wave * 2 + (c4 >> 1), c4 & 1);
     u32x4_t vt[TERMS];
     // f16: the second number 2^11 times larger, in sums of its own, so that it keeps
     // its bits
@@ -435,38 +627,8 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
       }
     };
 
-    // ---- S^T Q^T of the state before the chunk, times scale a^(i+1).  Products that wait
-    // for each other are kept apart, and v's factors are worked out between them.
-    f32x4_t o[kIT];
     if constexpr (!ONLY_STATE) {
-      float sc = 1.f;
-      if constexpr (F16) {
-        float mx = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, finite_abs(s[dt][i]));
-        sc = f16_scale(mx);
-      }
-      const float back = F16 ? 1.f / sc : 1.f;
-#pragma unroll
-      for (int it = 0; it < kIT; ++it) o[it] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        f32x4_t x = s[2 * ks], y = s[2 * ks + 1];
-        if constexpr (F16) {
-          x *= sc;
-          y *= sc;
-        }
-        const u32x4_t sp = u32x4_t{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]),
-                                   pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3])};
-#pragma unroll
-        for (int it = 0; it < kIT; ++it) o[it] = mfma16t<F16>(sp, row_op(lq, it, ks), o[it]);
-#pragma unroll
-        for (int y4 = 4 * ks / KS; y4 < 4 * (ks + 1) / KS; ++y4) weigh(y4);
-      }
-#pragma unroll
-      for (int it = 0; it < kIT; ++it) o[it] *= rise[it] * back;
+      ahead_of(lq, weigh);
     } else {
 #pragma unroll
       for (int x = 0; x < 4; ++x) weigh(x);
@@ -496,48 +658,35 @@ __global__ void __launch_bounds__(64 * W, ONLY_STATE && DK < 256 ? 4 : 2)
           const float z = F16 ? __builtin_fmaf(y[u][i], 1.f / kLow, x[u][i]) : x[u][i];
           s[d4 + u][i] = __builtin_fmaf(s[d4 + u][i], a, z);
         }
-    }
-
-    if constexpr (!ONLY_STATE) {
-      // ---- V^T P^T of the chunk's own tokens
-      // A token whose v is not finite makes its columns of the state so: then every
-      // query takes its own product, tokens behind it as zeros, since a weight of zero
-      // times an infinity would reach the queries ahead of them.
-      const bool alone = __builtin_amdgcn_ballot_w64(!(fabsf(s[0][0]) < INFINITY)) != 0;
+      // (stated where the compiler would otherwise put these sums off to the next chunk, and
+      // keep their operands in registers that it does not have: D 256 spilled, and took
+      // 297 us where it takes 196 at B4 G32 T2048)
+      if constexpr (DK == 256 && !ONLY_STATE)
 #pragma unroll
-      for (int it = 0; it < kIT; ++it) {
-        const u32x4_t pf = s_p[((ci & 1) * kIT + it) * 64 + lane];
-        const float ps = F16 ? s_ps[ci & 1][it] : 1.f;
-        if constexpr (F16) o[it] *= ps;
-        if (!alone) {
-          o[it] = mfma16t<F16>(vf, pf, o[it]);
-        } else {
-          const int j0 = fresh(4 * g4);
-#pragma unroll 1
-          for (int x = 0; x < 16; ++x) {
-            u32x4_t keep;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const int j = 16 * (y >> 1) + j0 + 2 * (y & 1), i = 16 * it + x;
-              keep[y] = (j <= i ? 0xffffu : 0u) | (j + 1 <= i ? 0xffff0000u : 0u);
-            }
-            const f32x4_t z = mfma16t<F16>(vf & keep, pf, o[it]);
-            if (r == x) o[it] = z;
-          }
-        }
-        if constexpr (F16) o[it] *= 1.f / ps;
-        // ---- o[it][e] is token 16 it + r, column col0 + 4 g4 + e
-        // (stated to lie in global memory: the counted waits at a chunk's start rely on the
-        // order of the copies and these stores, which flat ones need not keep)
-        char* to = const_cast<char*>(uniform(ob)) + ooff;
-        ob += ostep;
-        if (16 * it + r < left && col0 + 4 * g4 < E)
-          *(__attribute__((address_space(1))) u32x2_t*)to =
-              u32x2_t{pack2<F16>(o[it][0], o[it][1]), pack2<F16>(o[it][2], o[it][3])};
-      }
+        for (int u = 0; u < 4; ++u) asm volatile("" : "+v"(s[d4 + u]));
     }
+    if constexpr (ONLY_STATE && F16)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) asm volatile("" : "+v"(s[dt]));
+    if constexpr (!ONLY_STATE) finish(ci, std::false_type{}, 0);
+    go = ++ci < nch;
+    if (go) go = !begin(ci);
   }
-
+  // From a chunk with infinities or NaN on, by another loop: one that took such chunks
+  // beside the others would keep the state in registers of its own for them.
+  while (ci < nch) {
+    if constexpr (ONLY_STATE) {
+      by_token(lq, min(tokens - ci * kC, kC));
+    } else {
+      ahead_of(lq, [](int) {});
+      const uint32_t bad = by_token(lq, min(tokens - ci * kC, kC));
+      vf = col_op(lq + Q_BYTES + K_BYTES, VC{}, wave * 2 + (c4 >> 1), c4 & 1);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) vf[x] &= finite16<F16>(vf[x]);
+      finish(ci, std::true_type{}, bad);
+    }
+    if (++ci < nch) begin(ci);
+  }
   if constexpr (ONLY_STATE) {
     if (!wanted) return;
     write_state(p.ws + (bgh * slots + seg + 1) * sz);

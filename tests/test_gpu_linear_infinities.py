@@ -88,3 +88,87 @@ def test_step(lh, decay, e):  # noqa: F811
         o = lh.linear_attention_step(d["q"], d["k"], d["v"], d["log_decay"], d["state"])
         alike(d["state"], end, etol, f"infinite step {decay} {e} state")
         alike(o, want[:, 0], tol[:, 0], f"infinite step {decay} {e} out")
+
+
+# B, G, H, D, E, T, counts: every key dim's kernel on 64 and 128 columns, prompts in one
+# piece (more heads than run at once) and in segments
+PROMPTS = [
+    (2, 2, 2, 64, 64, 100, [100, 77]), (2, 1, 3, 40, 72, 130, None), (1, 2, 1, 128, 128, 97, None),
+    (2, 1, 2, 128, 48, 70, [70, 33]), (1, 1, 2, 256, 64, 66, None), (2, 1, 1, 136, 136, 95, [95, 64]),
+    (2, 1, 1, 64, 64, 700, [700, 515]), (1, 2, 1, 128, 128, 650, None), (1, 1, 1, 200, 40, 600, None),
+    (1, 1, 1, 256, 256, 520, None), (1, 1, 2, 72, 64, 640, None), (1, 1, 1, 16, 160, 610, None),
+]
+
+
+def spoiled(shape, e, decay, seed):
+    """Inputs with infinities and NaN of q, k, v and the states, in columns, rows and tokens
+    of their own (early, at a chunk's ends, late) beside untouched ones."""
+    B, G, H, D, E, T, counts = shape
+    t = make(B, G, H, D, E, T, counts, e, True, seed)
+    t["log_decay"][:] = decay
+    t["q"][..., 0, :] = t["q"][..., 0, :].abs() + 0.25        # (heads 0: infinities keep their sign)
+    k, v, q, s = t["k"], t["v"], t["q"], t["state"]
+    k[:, :, 0, 1:3] = k[:, :, 0, 1:3].abs() + 0.1
+    k[0, 20, 0] = k[0, 20, 0].abs() + 0.1                      # (one that makes a column all +inf)
+    v[0, 20, 0, 3], v[0, 31, 0, 4], v[0, 32, 0, 6] = INF, -INF, INF
+    v[0, 40, 0, 7], v[0, T - 3, 0, E - 1] = NAN, INF
+    v[0, 20, 0, 9], v[0, 50, 0, 9] = INF, -INF
+    v[0, 45, 0, 10], k[0, 45, 0, 5] = INF, 0.0
+    s[0, 0, 0, 3, 12], s[0, 0, H - 1, 4, 13], s[0, 0, 0, 2, 14] = INF, -INF, NAN
+    if B > 1:                                                  # a sequence with an infinite key
+        k[1, 12, 0, 1] = INF
+        k[1, 39, 0, 2], v[1, 39, 0, 8] = -INF, INF
+    if G > 1:                                                  # heads with infinite queries only
+        q[0, 35, 1, 0, 3], q[0, 64, 1, H - 1, 2], q[0, 5, 1, 0, 1] = INF, -INF, NAN
+    return t
+
+
+def run(lh, t, counts):  # noqa: F811
+    d = on_gpu(t)
+    B, T, G, H, _ = t["q"].shape
+    out = torch.full((B, T, G, H, t["v"].shape[-1]), 7.0, dtype=t["q"].dtype, device="cuda")
+    return lh.linear_attention(d["q"], d["k"], d["v"], d["log_decay"], d["state"], out,
+                               counts=ints(counts))
+
+
+@pytest.mark.parametrize("e", TYPES)
+@pytest.mark.parametrize("shape", PROMPTS, ids=["x".join(map(str, s[:6])) for s in PROMPTS])
+def test_prompt(lh, shape, e):  # noqa: F811
+    for decay in (0.0, -0.05, -30.0, -200.0):
+        print("prompt", shape, decay, e, flush=True)
+        t = spoiled(shape, TYPES[e], decay, shape[3])
+        want, tol, end, etol = recurrence(t, shape[6])
+        o, s = run(lh, t, shape[6])
+        alike(s, end, etol, f"infinite prompt {shape[3:6]} {decay} {e} state")
+        alike(o, want, tol, f"infinite prompt {shape[3:6]} {decay} {e} out")
+
+
+@pytest.mark.parametrize("e", TYPES)
+@pytest.mark.parametrize("decay", [-0.5, -INF])
+def test_decays_of_many_heads(lh, decay, e):  # noqa: F811
+    """More heads than run at once: prompts in one piece."""
+    shape = (4, 33, 2, 64, 72, 90, [90, 0, 31, 64])
+    assert not lh.linear_attention_workspace_bytes(*shape[:6])
+    t = spoiled((4, 33, 2, 64, 72, 90, None), TYPES[e], decay, 5)
+    for b, c in enumerate(shape[6]):
+        for x in "qkv":
+            t[x][b, c:] = NAN
+    want, tol, end, etol = recurrence(t, shape[6])
+    o, s = run(lh, t, shape[6])
+    alike(s, end, etol, f"infinite prompt, many heads {decay} {e} state")
+    alike(o, want, tol, f"infinite prompt, many heads {decay} {e} out")
+
+
+@pytest.mark.parametrize("e", TYPES)
+@pytest.mark.parametrize("x", "vkq")
+def test_earlier_rows_keep_their_bits(lh, x, e):  # noqa: F811
+    """Rows ahead of an infinity, in its chunk and before, are what they are without it."""
+    for B, G, H, D, E, T, at in ((1, 2, 1, 64, 64, 100, 50), (1, 1, 2, 128, 128, 640, 333),
+                                 (1, 1, 1, 40, 72, 70, 69)):
+        t = make(B, G, H, D, E, T, None, TYPES[e], True, 3)
+        a, _ = run(lh, t, None)
+        t[x][0, at, 0, ..., 5] = INF
+        b, _ = run(lh, t, None)
+        assert torch.equal(a[:, :at], b[:, :at])
+        assert not torch.isfinite(b[0, at, 0]).all()
+        assert torch.equal(a[:, :, 1:], b[:, :, 1:])          # other heads' rows
