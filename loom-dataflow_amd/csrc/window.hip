@@ -579,6 +579,17 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
       }
     }
   }
+  // ---- a row without a key of finite score is zero, whatever its keys' v held
+  bool none = false;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) none |= lacc[qt][0] == 0.f;
+  if (__builtin_amdgcn_ballot_w64(none) != 0) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+      if (lacc[qt][0] == 0.f)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) ot[dt][qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
   // ---- KG 2: the pair's second wave hands its state over through the idle stages
   // (lane by lane: both hold the same rows and columns); a half that saw no key (l =
   // 0) takes no part
