@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
       u32x2_t{pack2<F16>(acc[0] * inv, acc[1] * inv), pack2<F16>(acc[2] * inv, acc[3] * inv)};
 }
 
-// The launch's shape, from the extents alone.
+// The launch's shape, from the extents alone.  (launch_window has the kernels that it gives.)
 struct Shape {
   int tile;         // rows of a tile: 32, 64, 128 or 256
   int64_t ntiles;   // per (b, g)
@@ -767,6 +767,13 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t T, int64_t S,
   const int64_t slots = D > 128 ? 256 : 512;
   const int64_t want = std::min<int64_t>(slots / (BG * s.ntiles), blocks / 2);
   s.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
+  // Tiles past 32 rows are 256 at least, a round of workgroups.  Exactly 256 are cut in two
+  // where two of their workgroups fit a CU, by LDS and registers, and a tile's blocks are
+  // worth the join (tiles of 64 rows, G8 H4 T512: D 64 window 2048 24.5 us whole, 29.9 cut,
+  // 4096 41.4 and 42.9, 8192 72.7 and 65.1; D 96 29.7 and 37.3, 50.2 and 52.3, 89.2 and 79.7;
+  // 256 rows of D 128, T2048 window 1024: 42.9 and 66.3).
+  const bool two = s.tile <= (D > 96 ? 32 : D > 64 ? 64 : 128);
+  if (s.tile > 32 && !(two && blocks >= 72)) s.nsplit = 1;
   return s;
 }
 
@@ -776,32 +783,36 @@ template <bool F16, bool KREG, bool SPLIT>
 void launch_window(const WindowParams& p, const Shape& s, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)p.B * p.G * s.ntiles * s.nsplit)), b4(256), b8(512);
   auto launch = [&](auto kern, dim3 block) { hipLaunchKernelGGL(kern, grid, block, 0, st, p); };
+  // a tile that is never split
+  auto whole = [&](auto kern, dim3 block) {
+    if constexpr (!SPLIT) launch(kern, block);
+  };
   // the kernel built for 64, 128 or 256 (the next one up) runs any narrower head
   if (p.D > 128) {
     switch (s.tile) {
       case 32: launch(window_tile_kernel<256, 1, 4, F16, KREG, SPLIT, 2, 2, 1, 256>, b4); break;
-      default: launch(window_tile_kernel<256, 1, 8, F16, KREG, SPLIT, 1, 2, 1, 256>, b8); break;
+      default: whole(window_tile_kernel<256, 1, 8, F16, KREG, false, 1, 2, 1, 256>, b8); break;
     }
   } else if (p.D > 96) {
     switch (s.tile) {
       case 32: launch(window_tile_kernel<128, 1, 4, F16, KREG, SPLIT, 2, 2, 2, 128>, b4); break;
-      case 64: launch(window_tile_kernel<128, 1, 8, F16, KREG, SPLIT, 2, 2, 2, 128>, b8); break;
-      case 128: launch(window_tile_kernel<128, 1, 8, F16, KREG, SPLIT, 1, 3, 1, 128>, b8); break;
-      default: launch(window_tile_kernel<128, 2, 8, F16, KREG, SPLIT, 1, 3, 1, 128>, b8); break;
+      case 64: whole(window_tile_kernel<128, 1, 8, F16, KREG, false, 2, 2, 2, 128>, b8); break;
+      case 128: whole(window_tile_kernel<128, 1, 8, F16, KREG, false, 1, 3, 1, 128>, b8); break;
+      default: whole(window_tile_kernel<128, 2, 8, F16, KREG, false, 1, 3, 1, 128>, b8); break;
     }
   } else if (p.D > 64) {
     switch (s.tile) {
       case 32: launch(window_tile_kernel<128, 1, 4, F16, KREG, SPLIT, 2, 2, 2, 96>, b4); break;
       case 64: launch(window_tile_kernel<128, 1, 8, F16, KREG, SPLIT, 2, 2, 2, 96>, b8); break;
-      case 128: launch(window_tile_kernel<128, 1, 8, F16, KREG, SPLIT, 1, 3, 1, 96>, b8); break;
-      default: launch(window_tile_kernel<128, 2, 8, F16, KREG, SPLIT, 1, 3, 1, 96>, b8); break;
+      case 128: whole(window_tile_kernel<128, 1, 8, F16, KREG, false, 1, 3, 1, 96>, b8); break;
+      default: whole(window_tile_kernel<128, 2, 8, F16, KREG, false, 1, 3, 1, 96>, b8); break;
     }
   } else {
     switch (s.tile) {
       case 32: launch(window_tile_kernel<64, 1, 4, F16, KREG, SPLIT, 2, 2, 2, 64>, b4); break;
       case 64: launch(window_tile_kernel<64, 1, 8, F16, KREG, SPLIT, 2, 2, 2, 64>, b8); break;
       case 128: launch(window_tile_kernel<64, 1, 8, F16, KREG, SPLIT, 1, 3, 1, 64>, b8); break;
-      default: launch(window_tile_kernel<64, 2, 8, F16, KREG, SPLIT, 1, 3, 1, 64>, b8); break;
+      default: whole(window_tile_kernel<64, 2, 8, F16, KREG, false, 1, 3, 1, 64>, b8); break;
     }
   }
 }
