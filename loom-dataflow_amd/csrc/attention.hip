@@ -56,31 +56,8 @@ struct AttnParams {
 // lazy: a row's running max only moves (and O, l are rescaled) when a block
 // raises it by more than 8 in the log2 domain, which keeps P <= 2^8 and the
 // result exact (numerator and denominator share the stale base).
-// Ks rows (128 B) and Vs rows (2 D bytes) XOR their 16-byte chunk index with
-// k_swz / v_swz so that the 32 lanes of each pass of a transposed read touch
-// distinct banks.  The banks repeat every 256 bytes (measured: rows 256 bytes
-// apart conflict, SQ_LDS_BANK_CONFLICT), so a 32-byte row piece has eight
-// positions per window.
+// Ks, Vs and Q / O staging rows lie under k_swz, v_swz and q_swz.
 // ---------------------------------------------------------------------------
-// One pass of a K^T read covers Ks rows d..d+3 and d+8..d+11, 32 bytes each;
-// 128-byte rows put the even rows on one half of the window and the odd rows
-// on the other, so rows d, d^2, d^8, d^10 must take distinct chunk pairs:
-// row bits 1 and 3 pick them (bit 0 only repeats the half's pattern).
-LOOM_DEV int k_swz(int d) { return (2 * (d & 3)) ^ (2 * ((d >> 3) & 1)); }
-// One pass of a V^T read covers 8 consecutive Vs rows, 32 bytes each.  D 128
-// and 256 (rows of a multiple of 256 bytes): all eight share a window
-// position, row bits 0-2 pick the pair.  D 64 (128-byte rows): rows r, r^2,
-// r^4, r^6 share one, bits 1-2.
-template <int D>
-LOOM_DEV int v_swz(int k) { return D >= 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3); }
-// Q / O staging rows (2 D bytes): chunk c of row lr sits at position
-// c ^ q_swz(lr), so the 16 rows of a 32-lane pass (16-byte reads of chunks
-// c and c + 1, or 8-byte halves of one chunk) land on distinct banks: rows
-// 256 bytes apart at D 128, 128 bytes apart at D 64 (there bits 0-2 of the
-// row XOR bit 3, which tells rows 8 apart apart).
-template <int D>
-LOOM_DEV int q_swz(int lr) { return D >= 128 ? (lr & 15) : ((lr ^ (lr >> 3)) & 7); }
-
 // KREG (Skv not a multiple of 8): K rows [d][0..Skv) do not start on
 // 16-byte boundaries, so K cannot be copied by 16-byte LDS DMA.  Each lane
 // then loads its 16-byte pieces of a K block into registers (row_piece8: one

@@ -75,27 +75,13 @@ LOOM_DEV int seq_len(const StepParams& p, int b) { return min(max(p.lens[b], 0),
 // ---------------------------------------------------------------------------
 // One part: up to RT query rows against the keys [s0, s1) of one K, V.
 // ---------------------------------------------------------------------------
-// dma_load16 of data that is read once: non-temporal, so the stream displaces
-// nothing that is read again.  Taken for the own keys of caches larger than the
-// 256 MB last-level cache (B48 G8 S4096 under a prefix 124 -> 113 us a step, B8 G8
+// Own keys of caches larger than the 256 MB last-level cache are copied by
+// dma_once16, so that the stream displaces nothing that is read again (B48 G8 S4096 under a prefix 124 -> 113 us a step, B8 G8
 // S8192 43.5 -> 38.7); smaller ones may still lie there from the last step (B16
 // G8 S2048 29.3 against 31.6), and a prefix is read by many sequences.  The rule
 // knows the capacity, not the lengths: large caches that hold little pay up to 5%
 // (B48 G8 H8 S8192 holding 1024 to 1536 keys each 55.6 against 53.1 us, 100 to 400
-// keys 20.6 against 20.0)
-LOOM_DEV void dma_once16(const void* g, uint32_t lds) {
-  asm volatile(
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %0, off nt"
-      :
-      : "v"(g), "s"(lds)
-      : "memory", "m0");
-}
-LOOM_DEV int ck_swz(int d) { return (2 * (d & 3)) ^ (2 * ((d >> 3) & 1)); }
-template <int D>
-LOOM_DEV int cv_swz(int k) { return D >= 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3); }
-
+// keys 20.6 against 20.0).
 struct Part {
   const uint16_t* k;    // [D][ld]
   const uint16_t* v;    // [ld][D]
@@ -176,7 +162,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
       for (int i = 0; i < K_INSTR; ++i) {
         const int j = wave * K_INSTR + i;
         const int d = j * 8 + lane / 8;
-        const int key = min(kv0 + ((lane % 8) ^ ck_swz(d)) * 8, ld - 8);
+        const int key = min(kv0 + ((lane % 8) ^ k_swz(d)) * 8, ld - 8);
         if (j * 8 < Dr)                                 // wave-uniform
           copy(kg + (int64_t)d * ld + key, lk + j * 1024);
         else
@@ -187,7 +173,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
     for (int i = 0; i < V_INSTR; ++i) {
       const int j = wave * V_INSTR + i;
       const int kr = j * V_ROWS_PER_I + lane / (D / 8);
-      const int c = min((lane % (D / 8)) ^ cv_swz<D>(kr), Dr / 8 - 1);
+      const int c = min((lane % (D / 8)) ^ v_swz<D>(kr), Dr / 8 - 1);
       const int key = kv0 + kr;
       const void* const from = key < s1 ? (const void*)(vg + (int64_t)key * Dr + c * 8)
                                         : (const void*)(loom_zero_kb + lane * 4);
@@ -207,7 +193,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
     for (int i = 0; i < K_INSTR; ++i) {
       const int j = wave * K_INSTR + i;
       const int d = j * 8 + lane / 8;
-      kr[i] = j * 8 < Dr ? row_piece8(krs, ld, d, kv0 + ((lane % 8) ^ ck_swz(d)) * 8)
+      kr[i] = j * 8 < Dr ? row_piece8(krs, ld, d, kv0 + ((lane % 8) ^ k_swz(d)) * 8)
                          : u32x4_t{0u, 0u, 0u, 0u};
     }
   };
@@ -265,7 +251,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
     // for the LDS
     auto k_op = [&](int jt, int ds) {
       const int d = ds * 32 + g * 8 + a4;
-      const int ch = (2 * jt + (c4 >> 1)) ^ ck_swz(d);
+      const int ch = (2 * jt + (c4 >> 1)) ^ k_swz(d);
       const lds_char_t* q = ks + d * (kKeys * 2) + ch * 16 + (c4 & 1) * 8;
       const u32x2_t lo = lds_read_tr16(q);
       const u32x2_t hi = lds_read_tr16(q + 4 * (kKeys * 2));
@@ -273,7 +259,7 @@ LOOM_DEV void run_part(const StepParams& p, const Part& a, char* smem) {
     };
     auto v_op = [&](int hv, int dt) {
       const int k0r = 32 * hv + 4 * g + a4;
-      const int ch = (2 * dt + (c4 >> 1)) ^ cv_swz<D>(k0r);
+      const int ch = (2 * dt + (c4 >> 1)) ^ v_swz<D>(k0r);
       const lds_char_t* q = vs + k0r * VROW + ch * 16 + (c4 & 1) * 8;
       const u32x2_t lo = lds_read_tr16(q);
       const u32x2_t hi = lds_read_tr16(q + 16 * VROW);

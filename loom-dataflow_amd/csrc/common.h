@@ -130,6 +130,14 @@ LOOM_DEV void transpose8x8(const u32x4_t (&in)[8], u32x4_t (&out)[8]) {
   }
 }
 
+// A value that the compiler does not know to be x: what rare paths compute from it is
+// worked out there, not ahead of a loop in registers that it needs.  (A spilled register
+// costs more than its load there: that load's wait is one for every copy on its way.)
+LOOM_DEV int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 LOOM_DEV float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Map a linear workgroup id so that each of the 8 XCDs (which receive ids
@@ -353,6 +361,17 @@ LOOM_DEV void dma_load16(const void* g, uint32_t lds) {
       : "memory", "m0");
 }
 
+// dma_load16 of keys that no other workgroup reads: non-temporal
+LOOM_DEV void dma_once16(const void* g, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, off nt"
+      :
+      : "v"(g), "s"(lds)
+      : "memory", "m0");
+}
+
 // 1 KB of zeros in device memory: the source of the LDS-DMA copies of
 // padding rows (an operand narrower than the tile built for it), so those
 // rows hold zeros and every wave still issues the same copies per stage.
@@ -375,6 +394,30 @@ LOOM_DEV int tr_swz(int k, int rb) {
   const int pr = g >= 32 ? g / 32 : 1;                 // rows of a pass sharing an offset
   return 2 * ((k >> (8 - __builtin_ctz(g))) & (pr - 1));   // (k / (256 / g)) % pr
 }
+
+// The stages of 64 keys of the attention kernels, Ks [d][key] (128-byte rows) and Vs
+// [key][d] (rows of 2 D bytes): rows XOR their 16-byte chunk index with k_swz / v_swz so
+// that the 32 lanes of each pass of a transposed read touch distinct banks.  The banks
+// repeat every 256 bytes (measured: rows 256 bytes apart conflict, SQ_LDS_BANK_CONFLICT),
+// so a 32-byte row piece has eight positions per window.
+// One pass of a K^T read covers Ks rows d..d+3 and d+8..d+11, 32 bytes each;
+// 128-byte rows put the even rows on one half of the window and the odd rows
+// on the other, so rows d, d^2, d^8, d^10 must take distinct chunk pairs:
+// row bits 1 and 3 pick them (bit 0 only repeats the half's pattern).
+LOOM_DEV int k_swz(int d) { return (2 * (d & 3)) ^ (2 * ((d >> 3) & 1)); }
+// One pass of a V^T read covers 8 consecutive Vs rows, 32 bytes each.  D 128
+// and 256 (rows of a multiple of 256 bytes): all eight share a window
+// position, row bits 0-2 pick the pair.  D 64 (128-byte rows): rows r, r^2,
+// r^4, r^6 share one, bits 1-2.
+template <int D>
+LOOM_DEV int v_swz(int k) { return D >= 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3); }
+// Q / O staging rows (2 D bytes): chunk c of row lr sits at position
+// c ^ q_swz(lr), so the 16 rows of a 32-lane pass (16-byte reads of chunks
+// c and c + 1, or 8-byte halves of one chunk) land on distinct banks: rows
+// 256 bytes apart at D 128, 128 bytes apart at D 64 (there bits 0-2 of the
+// row XOR bit 3, which tells rows 8 apart apart).
+template <int D>
+LOOM_DEV int q_swz(int lr) { return D >= 128 ? (lr & 15) : ((lr ^ (lr >> 3)) & 7); }
 
 // ds_read_b64_tr_b16: in each 16-lane group, lanes 4a..4a+3 address the four
 // 8-byte pieces of row a of a 4x16 matrix of 16-bit values; lane j receives

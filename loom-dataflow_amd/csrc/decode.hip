@@ -189,15 +189,6 @@ __global__ void __launch_bounds__(256) decode_combine_row_kernel(DecodeParams p)
 // Blocks start at the split's first key rounded down to a multiple of 8;
 // keys outside [s0, s1) are masked to -inf, reads past S are clamped.
 // ---------------------------------------------------------------------------
-// 16-byte chunk swizzles of the Ks and Vs rows, as in attention.hip: the
-// banks repeat every 256 bytes, and each 32-lane pass of a transposed read
-// must touch distinct ones.  Ks (128-byte rows): rows d, d^2, d^8, d^10 share
-// a window position.  Vs: D 128 (256-byte rows) all eight rows of a pass, D 64
-// rows r, r^2, r^4, r^6.
-LOOM_DEV int dk_swz(int d) { return (2 * (d & 3)) ^ (2 * ((d >> 3) & 1)); }
-template <int D>
-LOOM_DEV int dv_swz(int k) { return D >= 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3); }
-
 // KREG (S not a multiple of 8): K rows [d][0..S) do not start on 16-byte
 // boundaries, so K cannot be copied by 16-byte LDS DMA.  Each lane then
 // loads its 16-byte pieces of a K block into registers (row_piece8), issued
@@ -258,7 +249,7 @@ __global__ void __launch_bounds__(64 * W) decode_dma_kernel(DecodeParams p) {
       for (int i = 0; i < K_INSTR; ++i) {
         const int j = wave * K_INSTR + i;
         const int d = j * 8 + lane / 8;                 // Ks row
-        const int c = (lane % 8) ^ dk_swz(d);
+        const int c = (lane % 8) ^ k_swz(d);
         const int key = min(kv0 + c * 8, S - 8);
         if (j * 8 < Dr)                                 // wave-uniform
           dma_load16(kg + (int64_t)d * S + key, lk + j * 1024);
@@ -270,7 +261,7 @@ __global__ void __launch_bounds__(64 * W) decode_dma_kernel(DecodeParams p) {
     for (int i = 0; i < V_INSTR; ++i) {
       const int j = wave * V_INSTR + i;
       const int kr = j * V_ROWS_PER_I + lane / (D / 8); // Vs row (key)
-      const int c = min((lane % (D / 8)) ^ dv_swz<D>(kr), Dr / 8 - 1);
+      const int c = min((lane % (D / 8)) ^ v_swz<D>(kr), Dr / 8 - 1);
       const int key = min(kv0 + kr, S - 1);
       dma_load16(vg + (int64_t)key * Dr + c * 8, lv + j * 1024);
     }
@@ -286,7 +277,7 @@ __global__ void __launch_bounds__(64 * W) decode_dma_kernel(DecodeParams p) {
     for (int i = 0; i < K_INSTR; ++i) {
       const int j = wave * K_INSTR + i;
       const int d = j * 8 + lane / 8;
-      const int c = (lane % 8) ^ dk_swz(d);
+      const int c = (lane % 8) ^ k_swz(d);
       kr[i] = j * 8 < Dr ? row_piece8(krs, S, d, kv0 + c * 8)   // padding rows: zeros
                          : u32x4_t{0u, 0u, 0u, 0u};
     }
@@ -347,7 +338,7 @@ __global__ void __launch_bounds__(64 * W) decode_dma_kernel(DecodeParams p) {
       for (int j = 0; j < 2; ++j) {
         const int jt = 2 * kh + j;
         const int d = ds * 32 + g * 8 + a4;
-        const int ch = (2 * jt + (c4 >> 1)) ^ dk_swz(d);
+        const int ch = (2 * jt + (c4 >> 1)) ^ k_swz(d);
         const lds_char_t* q = ks + d * (KB * 2) + ch * 16 + (c4 & 1) * 8;
         const u32x2_t lo = lds_read_tr16(q);
         const u32x2_t hi = lds_read_tr16(q + 4 * (KB * 2));
@@ -407,7 +398,7 @@ __global__ void __launch_bounds__(64 * W) decode_dma_kernel(DecodeParams p) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const int k0r = 32 * kh + 4 * g + a4;
-      const int ch = (2 * dt + (c4 >> 1)) ^ dv_swz<D>(k0r);
+      const int ch = (2 * dt + (c4 >> 1)) ^ v_swz<D>(k0r);
       const lds_char_t* q = vs + k0r * VROW + ch * 16 + (c4 & 1) * 8;
       const u32x2_t lo = lds_read_tr16(q);                // keys 4 g + 0..3
       const u32x2_t hi = lds_read_tr16(q + 16 * VROW);    // keys 16 + 4 g + 0..3

@@ -113,13 +113,6 @@ LOOM_DEV uint32_t finite16(uint32_t w) {
 }
 LOOM_DEV float finite_abs(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
 
-// A value that the compiler does not know to be x: what rare paths compute from it is
-// worked out there, not ahead of a loop in registers that it needs
-LOOM_DEV int fresh(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
 // The same address in every lane, stated to the compiler
 LOOM_DEV const char* uniform(const char* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);

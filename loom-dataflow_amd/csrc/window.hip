@@ -51,34 +51,6 @@ struct WindowParams {
   float c2;         // scale * log2(e)
 };
 
-// K [d][key] and V [key][d] rows lie in LDS with their 16-byte chunks XORed so that
-// the 32 lanes of each pass of a transposed read touch distinct banks (see
-// attention.hip, whose stages these are)
-LOOM_DEV int wk_swz(int d) { return (2 * (d & 3)) ^ (2 * ((d >> 3) & 1)); }
-template <int D>
-LOOM_DEV int wv_swz(int k) { return D >= 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3); }
-template <int D>
-LOOM_DEV int wq_swz(int lr) { return D >= 128 ? (lr & 15) : ((lr ^ (lr >> 3)) & 7); }
-
-// A value that the compiler does not know to be x: what rare paths compute from it is
-// worked out there, not ahead of a loop in registers that it needs.  (A spilled register
-// costs more than its load there: that load's wait is one for every copy on its way.)
-LOOM_DEV int fresh(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
-// dma_load16 of keys that no other workgroup reads: non-temporal
-LOOM_DEV void dma_once16(const void* g, uint32_t lds) {
-  asm volatile(
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %0, off nt"
-      :
-      : "v"(g), "s"(lds)
-      : "memory", "m0");
-}
-
 // What a tile of rows reads: sequence b's rows (t, h), t-major, r0 .. r0 + rows - 1
 // of c H, and the blocks of 64 keys that any of them sees: nsb blocks of sinks, then
 // those from wb0 on.
@@ -209,12 +181,12 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
   for (int i = 0; i < K_INSTR; ++i) {
     const int j = wave * K_INSTR + i, d = j * 8 + lane / 8;
     // unsigned: it wraps (and goes unused, koff32 == 0) when D * S * 2 >= 2^32
-    koff[i] = ((uint32_t)d * (uint32_t)S + (uint32_t)(((lane % 8) ^ wk_swz(d)) * 8)) * 2u;
+    koff[i] = ((uint32_t)d * (uint32_t)S + (uint32_t)(((lane % 8) ^ k_swz(d)) * 8)) * 2u;
   }
 #pragma unroll
   for (int i = 0; i < V_INSTR; ++i) {
     const int j = wave * V_INSTR + i, kr = j * V_ROWS_PER_I + lane / (D / 8);
-    voff[i] = (uint32_t)(kr * Dr + min((lane % (D / 8)) ^ wv_swz<D>(kr), Dr / 8 - 1) * 8) * 2;
+    voff[i] = (uint32_t)(kr * Dr + min((lane % (D / 8)) ^ v_swz<D>(kr), Dr / 8 - 1) * 8) * 2;
   }
   // (tiles of few rows only: keys of larger ones are shared)
   const bool once = KG == 2 && p.once != 0;
@@ -244,7 +216,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
       for (int i = 0; i < K_INSTR; ++i) {
         const int j = wave * K_INSTR + i;
         const int d = j * 8 + ln / 8;
-        const int key = min(kv0 + ((ln % 8) ^ wk_swz(d)) * 8, S - 8);
+        const int key = min(kv0 + ((ln % 8) ^ k_swz(d)) * 8, S - 8);
         const uint16_t* from = kg + (int64_t)d * S + key;
         if (j * 8 >= Dr) dma_load16(loom_zero_kb + ln * 4, __builtin_amdgcn_readfirstlane(lk + j * 1024));
         else if (once) dma_once16(from, __builtin_amdgcn_readfirstlane(lk + j * 1024));
@@ -272,7 +244,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
     for (int i = 0; i < K_INSTR; ++i) {
       const int j = wave * K_INSTR + i;
       const int d = j * 8 + lane / 8;
-      kr[i] = j * 8 < Dr ? row_piece8(krs, S, d, kv0 + ((lane % 8) ^ wk_swz(d)) * 8)
+      kr[i] = j * 8 < Dr ? row_piece8(krs, S, d, kv0 + ((lane % 8) ^ k_swz(d)) * 8)
                          : u32x4_t{0u, 0u, 0u, 0u};
     }
   };
@@ -292,7 +264,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
       const int j = wave * Q_INSTR + i;
       const int e = j * 1024 + lane * 16;
       const int lr = e / QROW, cp = (e % QROW) / 16;
-      const int c = min(cp ^ wq_swz<D>(lr), Dr / 8 - 1);
+      const int c = min(cp ^ q_swz<D>(lr), Dr / 8 - 1);
       dma_load16(p.q + row_of(min(lr, a.rows - 1)) * Dr + c * 8, lq + j * 1024);
     }
   }
@@ -377,7 +349,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
         for (int j = 0; j < 2; ++j) {
           const int jt = 2 * h + j;
           const int d = ds * 32 + g * 8 + a4;               // & 3 == a4
-          const int ch = (2 * jt + (c4 >> 1)) ^ wk_swz(d);
+          const int ch = (2 * jt + (c4 >> 1)) ^ k_swz(d);
           const lds_char_t* q = ks + d * (kKeys * 2) + ch * 16 + (c4 & 1) * 8;
           const u32x2_t lo = lds_read_tr16(q);
           const u32x2_t hi = lds_read_tr16(q + 4 * (kKeys * 2));
@@ -456,7 +428,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
       }
       auto v_op = [&](int dt) {
         const int k0r = 32 * h + 4 * g + a4;
-        const int ch = (2 * dt + (c4 >> 1)) ^ wv_swz<D>(k0r);
+        const int ch = (2 * dt + (c4 >> 1)) ^ v_swz<D>(k0r);
         const lds_char_t* q = vs + k0r * VROW + ch * 16 + (c4 & 1) * 8;
         const u32x2_t lo = lds_read_tr16(q);                // keys k0 + 4 g + 0..3
         const u32x2_t hi = lds_read_tr16(q + 16 * VROW);    // keys k0 + 16 + 4 g + 0..3
@@ -524,7 +496,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
 #pragma unroll
         for (int ds = 0; ds < DSTEPS; ++ds) {
           const u32x4_t raw = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
-              sQ + lr * QROW + ((4 * ds + g) ^ wq_swz<D>(lr)) * 16);
+              sQ + lr * QROW + ((4 * ds + g) ^ q_swz<D>(lr)) * 16);
           qf[ds][qt] = ds * 32 + g * 8 < Dr ? raw : u32x4_t{0u, 0u, 0u, 0u};
         }
       }
@@ -654,7 +626,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const f32x4_t o = ot[dt][qt];
-          const int at = (2 * dt + (g >> 1)) ^ wq_swz<D>(lr);
+          const int at = (2 * dt + (g >> 1)) ^ q_swz<D>(lr);
           *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(
               sQ + lr * QROW + at * 16 + (g & 1) * 8) =
               u32x2_t{pack2<F16>(o[0] * inv, o[1] * inv), pack2<F16>(o[2] * inv, o[3] * inv)};
@@ -669,7 +641,7 @@ __global__ void __launch_bounds__(64 * W, WPE) window_tile_kernel(WindowParams p
         const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
             sQ + lr * QROW + cp * 16);
         if (lr < a.rows)
-          *reinterpret_cast<u32x4_t*>(p.out + row_of(lr) * Dr + (cp ^ wq_swz<D>(lr)) * 8) = v;
+          *reinterpret_cast<u32x4_t*>(p.out + row_of(lr) * Dr + (cp ^ q_swz<D>(lr)) * 8) = v;
       }
       return;
     }
