@@ -13,7 +13,7 @@
 // head for 4 H D E operations: bound by HBM where the states stay on the chip, as they do
 // here, in the accumulators of the waves that walk a head's chunks (linear_chunk_kernel).
 // Where heads are fewer than CUs the tokens are cut into segments: a first launch leaves
-// the states of their stretches, from k and v alone, a second one walks every segment
+// the segments' states, from k and v alone, a second one walks every segment
 // from the sum of those before it.  One token is a stream of the states, read and written
 // once (linear_step_kernel).
 #include "common.h"
@@ -35,11 +35,11 @@ struct LinearParams {
   const int* counts;
   uint16_t* out;
   float* state_out;
-  float* ws;             // [B G H, (nseg - 1) sub + 1, D, E]: the states of stretches
+  float* ws;             // [B G H, nseg, D, E]: the initial states and those of segments
   int B, G, H, D, E, T;
   int nsl;               // slices of E
   int nseg;              // segments of a prompt
-  int sub, cps;          // stretches of a segment, chunks to one
+  int cps;               // chunks of a segment
   float scale;
 };
 
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
   const int a4 = r >> 2, c4 = r & 3;
   // (b, g) outermost, then segments, heads, slices: those that share k and v side by side
   const int nsl = p.nsl, H = p.H, D = p.D, E = p.E, GH = p.G * H;
-  const int nseg = ONLY_STATE ? (p.nseg - 1) * p.sub : p.nseg;
+  const int nseg = ONLY_STATE ? p.nseg - 1 : p.nseg;
   int id = xcd_remap(blockIdx.x, gridDim.x);
   const int sl = id % nsl;
   id /= nsl;
@@ -187,14 +187,12 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
   const int b = bg / p.G, g = bg - b * p.G, gh = g * H + h;
   const int c =
       __builtin_amdgcn_readfirstlane(p.counts ? min(max(p.counts[b], 0), p.T) : p.T);
-  // tokens of a segment, and of the stretches whose states the first launch leaves
-  const int64_t sublen = (int64_t)p.cps * kC, seglen = sublen * p.sub;
-  const int64_t mylen = ONLY_STATE ? sublen : seglen;
-  const int t0 = (int)(seg * mylen);            // (T < 2^29 and a segment within T)
-  // the state of a stretch is asked for by the segments behind it only
-  const bool wanted = !ONLY_STATE || (seg / p.sub + 1) * seglen < c;
+  const int64_t seglen = (int64_t)p.cps * kC;
+  const int t0 = (int)(seg * seglen);           // (T < 2^29 and a segment within T)
+  // a segment's state is asked for by those behind it only
+  const bool wanted = !ONLY_STATE || (seg + 1) * seglen < c;
   if (seg > 0 && (!wanted || t0 >= c)) return;
-  const int tokens = wanted ? (int)min((int64_t)(c - t0), mylen) : 0;
+  const int tokens = wanted ? (int)min((int64_t)(c - t0), seglen) : 0;
   const int nch = (tokens + kC - 1) / kC;
 
   // ---- copies of chunk ci into a stage: rows past the sequence and chunks past D or E
@@ -321,16 +319,15 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) s[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   // the first launch's states: slot 0 the initial one (state_out may be state: the first
-  // segment reads this copy), slot u + 1 that of stretch u
-  const int64_t slots = (int64_t)(p.nseg - 1) * p.sub + 1;
+  // segment reads this copy), slot u + 1 that of segment u
+  const int64_t slots = p.nseg;
   if (p.nseg == 1 || (ONLY_STATE && seg == 0)) {
     if (p.state) read_state(p.state + bgh * sz, s);
     if constexpr (ONLY_STATE) write_state(p.ws + bgh * slots * sz);
   } else if constexpr (!ONLY_STATE) {
-    const int to = seg * p.sub;
 #pragma unroll 1
-    for (int u = seg == 0 ? 0 : 1; u <= to; ++u) {
-      const float w = fmaxf((float)exp((double)(to - u) * (double)sublen *
+    for (int u = seg == 0 ? 0 : 1; u <= seg; ++u) {
+      const float w = fmaxf((float)exp((double)(seg - u) * (double)seglen *
                                        (double)(lg < -1e30f ? -1e30f : lg)),
                             least);
       f32x4_t x[DT];
@@ -756,7 +753,7 @@ __global__ void __launch_bounds__(256) linear_step_kernel(LinearParams p, int L)
 
 // The launch's shape, from the extents alone.
 struct Shape {
-  int waves, nsl, nseg, sub, cps;
+  int waves, nsl, nseg, cps;
 };
 Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t E, int64_t T) {
   Shape s{};
@@ -764,23 +761,24 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t E, int64_t T)
   s.waves = E <= 64 ? 4 : 8;
   s.nsl = (int)cdiv64(E, 16 * s.waves);
   const int64_t wgs = B * G * H * s.nsl, chunks = cdiv64(T, kC);
-  // Segments of at least four chunks, as many workgroups as run at once (16 heads of T512:
-  // segments of 8 chunks 26.2 us, of 4 21.0, of 2 22.4; 256 heads of prompts of 1024 to 4096
-  // cut in two 292 us, whole 216: the first launch costs more than the balance gains)
+  // Segments of at least four chunks (T512 of 16 heads 20.0 us, of eight chunks 28.2, of two
+  // 18.5; T2048 of 8 heads 26.9, 31.4, 37.9), as many workgroups as run at once.  More of
+  // them cost more in the first launch than they balance (256 heads of prompts of 1024 to
+  // 4096 cut in two 285 us, whole 197; 160 of T4096 in three 237, whole 193), and so did two
+  // stretches to a segment for the first launch, whose states a segment's start adds up one
+  // by one (T8192 of one head 110 us, 65 without; T512 of 16 20.4).
+  // (Of eight waves two workgroups run on a CU too up to D 64 in bf16: not counted.)
   const int64_t slots = s.waves == 4 && D <= 128 ? 512 : 256;
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>({slots / wgs, chunks / 4, 64}));
-  // two stretches to a segment where its first launch would leave most of the CUs idle (the
-  // 16 heads 26.2 us against 28.8; 36 heads of 7 segments 38.4 against 35.6)
-  s.sub = want > 1 && wgs * (want - 1) < 128 ? 2 : 1;
-  s.cps = (int)cdiv64(chunks, want * s.sub);
-  s.nseg = (int)cdiv64(chunks, s.cps * s.sub);
+  s.cps = (int)cdiv64(chunks, want);
+  s.nseg = (int)cdiv64(chunks, s.cps);
   return s;
 }
 
 template <bool F16, bool ONLY_STATE>
 void launch_chunks(const LinearParams& p, const Shape& s, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)p.B * p.G * p.H * s.nsl *
-                             (ONLY_STATE ? (s.nseg - 1) * s.sub : s.nseg))),
+                             (ONLY_STATE ? s.nseg - 1 : s.nseg))),
       block(64 * s.waves);
   auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, st, p); };
   // the kernel built for 64, 128 or 256 (the next one up) runs any narrower key dim
@@ -868,7 +866,6 @@ int linear_impl(const void* q, const void* k, const void* v,
   p.ws = static_cast<float*>(workspace);
   p.nsl = s.nsl;
   p.nseg = s.nseg;
-  p.sub = s.sub;
   p.cps = s.cps;
   if (s.nseg > 1) {
     launch_chunks<F16, true>(p, s, st);
@@ -889,7 +886,7 @@ size_t loom_hip_linear_attention_workspace_bytes(int64_t B, int64_t G, int64_t H
   // what does not fit is reported as no size at all fits
   if (T > (1 << 29) || D > 256 || E > 256 || !loom_prod_le({B, G, H}, 1 << 20)) return SIZE_MAX;
   const Shape s = shape_of(B, G, H, D, E, T);
-  return s.nseg == 1 ? 0 : (size_t)(B * G * H * ((s.nseg - 1) * s.sub + 1)) * D * E * 4;
+  return s.nseg == 1 ? 0 : (size_t)(B * G * H * s.nseg) * D * E * 4;
 }
 
 int loom_hip_linear_attention(const void* q, const void* k, const void* v, const void* log_decay,

@@ -25,3 +25,11 @@ def test_few_rows_and_small_tiles_are_split():
     assert lh.window_attention_workspace_bytes(1, 8, 4, 96, 512, 8192, 8192, 4)
     assert not lh.window_attention_workspace_bytes(1, 8, 4, 64, 1024, 2048, 1024, 4)
     assert not lh.window_attention_workspace_bytes(1, 8, 4, 96, 512, 2048, 1024, 4)
+
+
+@pytest.mark.parametrize("G,T,segments", [(1, 8192, 64), (2, 2048, 16), (16, 512, 4), (4, 4096, 32),
+                                          (32, 32768, 8), (256, 4096, 0)])
+def test_a_prompt_s_segments_leave_one_state_each(G, T, segments):
+    """The workspace holds a state to each segment: none is cut any further for the first
+    launch, whose states every segment's start adds up."""
+    assert lh.linear_attention_workspace_bytes(1, G, 1, 128, 128, T) == G * segments * 128 * 128 * 4
