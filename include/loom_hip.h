@@ -367,7 +367,10 @@ size_t loom_hip_window_attention_workspace_bytes(int64_t B, int64_t G, int64_t H
  *   out = sum over j <= p, j > p - window or j < sinks, of softmax_j(scale q.k_j) v_j.
  * A row that sees no key (p < 0), or whose scores are all -inf, gives zeros; rows
  * t >= c are left as they are.  What a key that a row does not see holds (NaN,
- * infinities) does not reach the row.  T = 1 is a decoding step.  `scale` is finite
+ * infinities) does not reach the row.  Scores, their maxima and sums are fp32; every
+ * weight is rounded to the 16-bit type for its product with v, and out, divided by the
+ * sum of the rounded weights, once more.  So an infinite v that a row sees makes it
+ * infinite, or NaN where the key's weight rounds to zero.  T = 1 is a decoding step.  `scale` is finite
  * and positive, window at least 1 (from S on: every key up to p), sinks at least 0,
  * D a multiple of 8 up to 256 (else LOOM_HIP_EUNSUP), B*G <= 65535, S and T*H at
  * most 2^29, B*G*ceil(T*H/32) at most 2^23; S not a multiple of 8 needs D*S < 2^30.
@@ -397,7 +400,9 @@ size_t loom_hip_linear_attention_workspace_bytes(int64_t B, int64_t G, int64_t H
  * state_out[b,g,h] = S_(c-1), and out's rows t >= c are left as they are.  What
  * tokens behind c, or later than a row, hold does not reach it.  Infinities and NaN
  * among q, k, v and the states give what the recurrence gives (a rounded to fp32: 0
- * times an infinity, as of a below 2^-149, is NaN).  `scale` is finite
+ * times an infinity, as of a below 2^-149, is NaN).  States are held to fp32's
+ * accuracy; of an output, the state that meets q and each q.k a^(t-j) that meets v are
+ * rounded to the 16-bit type, and out once more.  `scale` is finite
  * and positive, D and E multiples of 8 up to 256 (else LOOM_HIP_EUNSUP), B*G*H at
  * most 2^20, T at most 2^29.  out, state_out and the workspace overlap neither the
  * other tensors nor each other, except that state_out may be state.  Equal calls
@@ -416,7 +421,7 @@ int loom_hip_linear_attention_f16(const void* q, const void* k, const void* v,
 
 /* The same for one token, its state updated in place: q, out [B,G,H,D], [B,G,H,E],
  * k [B,G,D], v [B,G,E].  A sequence with counts[b] <= 0 has none: its state and its
- * rows of out are left as they are. */
+ * rows of out are left as they are.  All of it is fp32; out alone is rounded. */
 int loom_hip_linear_attention_step(const void* q, const void* k, const void* v,
                                    const void* log_decay, void* state, const void* counts,
                                    void* out, int64_t B, int64_t G, int64_t H, int64_t D,

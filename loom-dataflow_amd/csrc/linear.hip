@@ -64,9 +64,12 @@ LOOM_DEV float decayed_plus(float s, const Decay& a, float x) {
   return __builtin_fmaf(s, a.hi, __builtin_fmaf(f, a.lo, x));
 }
 
-// A row's 16-byte chunks are XORed with this, so that both the 16 rows of a direct
-// read (one chunk each) and the 8 consecutive rows of a transposed read's pass (a pair
-// of chunks each) lie on distinct banks: rows of 128 bytes and of multiples of 256.
+// A row's 16-byte chunks are XORed with this, so that both the 16 rows of a direct read
+// of q or k (one chunk each) and the 8 consecutive rows of a pass of v's transposed reads
+// (a pair of chunks each) lie on distinct banks: rows of 128 bytes and of multiples of 256.
+// k's transposed reads take four chunks of a row, two of which share banks (40 to 47% of
+// the kernel's LDS cycles): reads without these conflicts took 32 more vector instructions
+// a chunk, and longer (32768 tokens 395 us against 375 in the version they were tried in).
 template <int N>
 LOOM_DEV int row_swz(int row) {
   return (N >= 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3)) ^ ((row >> 3) & 1);
@@ -134,18 +137,20 @@ LOOM_DEV const char* uniform(const char* p) {
 // 16 bytes of q that it reads.  P^T is built from the accumulators of K Q^T, one chunk
 // ahead, by four waves (in f16 two), and shared through LDS: one barrier to a chunk.
 // Rounding: S and P to 16 bits as operands, each once; a^(C-1-j) v_j as a sum of three
-// bf16 or two f16 numbers, so that the state keeps fp32's accuracy.  f16 operands are
-// scaled by powers of two where they leave its range.
+// bf16 or two f16 numbers, so that the state keeps fp32's accuracy (f16: to 2^-36 of k
+// where v is below 2^-14).  f16 operands are scaled by powers of two where they leave its
+// range.
 // What bounds it: a chunk of 128 x 128 takes a CU 1.4 us by itself (24 + 8 products of 16
 // cycles and 200 other vector instructions to each of 8 waves), its 32 KB 1.6 us at the
-// rate of a large copy.  B8 G32 of 1024 to 4096 tokens 201 us (738 MB, 3.7 TB/s: the
+// rate of a large copy.  B8 G32 of 1024 to 4096 tokens 197 to 206 us (738 MB, 3.7 TB/s: the
 // longest prompt's 128 chunks in a row, while the CUs of shorter ones idle), B1 G32 of
-// 32768 376 us (1.08 GB, and k, v once more in the first launch, 0.47 GB).  Measured:
-// chunks of 64 tokens by four waves 366 us, by eight 249 (the 64 x 64 scores cost more than
-// they save); chunks of 32 by four waves of 32 columns 251 to 257, by eight of 16 216;
-// direct reads of 16 bytes (not two of 8, which the compiler joined and took apart again
-// by moves) and one branch to a chunk's copies 201.  A fourth stage: no change.  k's
-// transposed reads without their bank conflicts, for 32 more vector instructions: 206.
+// 32768 370 to 395 us (1.08 GB, and k, v once more in the first launch, 0.47 GB); key dims
+// of 256: B4 G32 256 x 256 T2048 189 us, in f16 489 (28 spilled registers).  Measured while
+// it was built, at B8 G32: chunks of 64 tokens by four waves 366 us, by eight 249 (the 64 x
+// 64 scores cost more than they save); of 32 by four waves of 32 columns 251 to 257, by
+// eight of 16 216; then direct reads of 16 bytes (not two of 8, which the compiler joined
+// and took apart again by moves) and one branch to a chunk's copies 201, and k's transposed
+// reads without their bank conflicts 206.  A fourth stage: no change.
 // Infinities and NaN: every chunk is looked over while the one before it is worked on; from
 // one that holds any on, a second loop takes the tokens one by one (by_token), which are the
 // recurrence itself.
@@ -420,37 +425,36 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
       reinterpret_cast<u32x2_t*>(&s_p[(to * kIT + pit) * 64 + lane])[pt + t] =
           u32x2_t{pack2<F16>(x[t][0], x[t][1]), pack2<F16>(x[t][2], x[t][3])};
   };
-  // Whether chunk ci in a stage holds infinities or NaN: of k and v (without scores; the
-  // parts that this wave copied), or of v, by the waves whose turn at P^T comes next.  A
-  // chunk ahead, so that its work has no branch in its midst, which took 8% (the checks
-  // take 1 to 2).
-  auto look = [&](const lds_char_t* st, int ci) {
-    f16x2_t odd = f16x2_t{0, 0};
-    auto piece = [&](int at) {
-      const u32x4_t x = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
+  // Whether chunk ci in a stage holds infinities or NaN: of k and v (without scores; a piece
+  // of each to a wave), or of v, by the waves whose turn at P^T comes next.  A chunk ahead,
+  // so that its work has no branch in its midst, which took 8% (the checks take 1 to 2).
+  constexpr int PIECES = ONLY_STATE ? QK_INSTR + 1 : TURNS;
+  u32x4_t held[PIECES];
+  auto peek = [&](const lds_char_t* st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      int at = QK_ALL + (ONLY_STATE ? wave : (wave - turn * (W / TURNS)) * TURNS + i);
+      if (ONLY_STATE && i < QK_INSTR) at = min(wave + W * i, QK_ALL - 1);
+      held[i] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
           st + Q_BYTES + at * 1024 + lane * 16);
-      odd = odd16<F16>(odd, x);
-    };
-    if constexpr (ONLY_STATE) {
-#pragma unroll
-      for (int i = 0; i < QK_INSTR; ++i)
-        if (QK_ALL % W == 0 || wave + W * i < QK_ALL) piece(wave + W * i);
-      piece(QK_ALL + wave);
-    } else {
-#pragma unroll
-      for (int i = 0; i < TURNS; ++i) piece(QK_ALL + (wave - turn * (W / TURNS)) * TURNS + i);
     }
+  };
+  auto judge = [&](int ci) __attribute__((always_inline)) {
+    f16x2_t odd = f16x2_t{0, 0};
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) odd = odd16<F16>(odd, held[i]);
     if (__builtin_amdgcn_ballot_w64(odd[0] != odd[0] || odd[1] != odd[1]) != 0 && lane == 0)
       s_odd[ci & 1] = ci;
   };
   if (nch > 0) {
     LOOM_WAIT_VMCNT(0);
-    if constexpr (ONLY_STATE) {
-      look((lds_char_t*)smem, 0);
-    } else {
-      barrier_nofence();
-      if (turn == 0) build_p((lds_char_t*)smem, 0);
-      if (turn == TURNS - 1) look((lds_char_t*)smem, 0);
+    barrier_nofence();
+    const lds_char_t* const st = (lds_char_t*)smem;
+    if constexpr (!ONLY_STATE)
+      if (turn == 0) build_p(st, 0);
+    if (ONLY_STATE || turn == TURNS - 1) {
+      peek(st);
+      judge(0);
     }
   }
   // A chunk that holds an infinity or NaN, token by token as the recurrence has it, in
@@ -573,6 +577,8 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
     LOOM_WAIT_LGKM0();
     barrier_nofence();
     const int flag = s_odd[ci & 1];
+    const lds_char_t* const next = (lds_char_t*)(smem + (stage == NS - 1 ? 0 : stage + 1) * STAGE);
+    if constexpr (ONLY_STATE) peek(next);         // (judged below: behind the copies' start)
     if (ci + NS - 1 < nch) issue(stage == 0 ? NS - 1 : stage - 1);
     stage = stage == NS - 1 ? 0 : stage + 1;
     a = __builtin_fmaf(full.hi, owed, full.hi);
@@ -584,10 +590,15 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
       for (int x = 0; x < 8; ++x) w[x] = s_pow[max(0, left - 1 - (16 * (x >> 2) + j0 + (x & 3)))];
     }
     if (ci + 1 < nch) {
-      const lds_char_t* const next = (lds_char_t*)(smem + stage * STAGE);
-      if constexpr (!ONLY_STATE)
+      if constexpr (!ONLY_STATE) {
         if (turn == (ci + 1) % TURNS) build_p(next, ci + 1);
-      if (ONLY_STATE || turn == (ci + 2) % TURNS) look(next, ci + 1);
+        if (turn == (ci + 2) % TURNS) {
+          peek(next);
+          judge(ci + 1);
+        }
+      } else {
+        judge(ci + 1);
+      }
     }
     return __builtin_amdgcn_readfirstlane(flag) == ci;
   };

@@ -1112,7 +1112,11 @@ def window_attention(k, v, q, lens, window, out=None, workspace=None, *, sinks=0
     default) are the new tokens', whose token t, at position p = lens[b] -
     counts[b] + t, sees the keys j <= p with j > p - ``window`` or j < ``sinks``.
     Rows behind a sequence's tokens are left as they are (unset where ``out`` is not
-    given).  ``scale`` defaults to 1/sqrt(D)."""
+    given).  ``scale`` defaults to 1/sqrt(D).
+
+    Scores and sums are fp32; each weight is rounded to the 16-bit type for its product
+    with v (an infinite v gives infinities, NaN where its weight rounds to zero), and the
+    output, divided by the sum of the rounded weights, once more."""
     return _window("window_attention", k, v, q, lens, window, out, workspace, sinks, counts, scale)
 
 
@@ -1138,7 +1142,11 @@ def linear_attention(q, k, v, log_decay, state=None, out=None, state_out=None, w
     (zero by default) on; state_out is the last S, and may be ``state``.  Sequence b
     has ``counts[b]`` tokens (int32; all T by default); rows of out behind them are left as
     they are (unset where ``out`` is not given).  ``scale`` defaults to
-    1/sqrt(D)."""
+    1/sqrt(D).
+
+    States are held to fp32's accuracy; of an output, the state that meets q and each
+    q.k exp(log_decay)^(t-j) that meets v are rounded to the 16-bit type, and the output
+    once more.  Infinities and NaN give what the recurrence gives."""
     plan, dev, ptrs = _cache_enter("linear_attention",
                                    (q, k, v, log_decay, state, counts, out, state_out), (),
                                    _bounded_plan)
@@ -1161,7 +1169,8 @@ def linear_attention_step(q, k, v, log_decay, state, out=None, *, counts=None, s
 
     q [B,G,H,D], k [B,G,D], v [B,G,E], log_decay [G,H] fp32, state [B,G,H,D,E] fp32 ->
     out [B,G,H,E].  A sequence whose ``counts[b]`` (int32) is 0 has no token: its state
-    and its rows of out are left as they are."""
+    and its rows of out are left as they are.  All of it is fp32; the output alone is
+    rounded."""
     plan, dev, ptrs = _cache_enter("linear_attention_step",
                                    (q, k, v, log_decay, state, counts, out), (), _bounded_plan)
     dims = plan[2]
