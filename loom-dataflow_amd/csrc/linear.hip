@@ -151,9 +151,9 @@ LOOM_DEV const char* uniform(const char* p) {
 // eight of 16 216; then direct reads of 16 bytes (not two of 8, which the compiler joined
 // and took apart again by moves) and one branch to a chunk's copies 201, and k's transposed
 // reads without their bank conflicts 206.  A fourth stage: no change.
-// Infinities and NaN: every chunk is looked over while the one before it is worked on; from
-// one that holds any on, a second loop takes the tokens one by one (by_token), which are the
-// recurrence itself.
+// Infinities and NaN: every chunk is looked over while the one before it is worked on; one
+// that holds any, other than for states lost to NaN already, is taken token by token
+// (by_token), by the recurrence itself, for about 14 us.
 // ONLY_STATE: a segment's own state from zero (the first's from the initial state), which
 // later segments start from.
 template <int DK, int W, bool F16, bool ONLY_STATE>
@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
   __shared__ __attribute__((aligned(16))) u32x4_t s_p[ONLY_STATE ? 1 : 2 * kIT * 64];
   __shared__ float s_pow[kC + 1];
   __shared__ float s_ps[2][kIT];                // f16: what a tile of P was scaled by
-  __shared__ int s_odd[2];                      // the last chunk found to hold infinities or NaN
+  // the last chunks found to hold infinities or NaN, and to hold them in q or k
+  __shared__ int s_odd[2], s_keys[2];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
 
   const float lg = p.g[gh];
   if (tid <= kC) s_pow[tid] = (float)decay_pow(lg, tid);
-  if (tid < 2) s_odd[tid] = -1;
+  if (tid < 2) s_odd[tid] = s_keys[tid] = -1;
   Decay one = split_decay(decay_pow(lg, 1));
   one.hi = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(one.hi)));
   one.lo = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(one.lo)));
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
     float big = 0.f;
 #pragma unroll
     for (int t = 0; t < PT; ++t) big = largest(largest(big, x[t][0], x[t][1]), x[t][2], x[t][3]);
-    if (__builtin_amdgcn_ballot_w64(!(big < INFINITY)) != 0 && lane == 0) s_odd[to] = ci;
+    if (__builtin_amdgcn_ballot_w64(!(big < INFINITY)) != 0 && lane == 0) s_odd[to] = s_keys[to] = ci;
 #pragma unroll
     for (int t = 0; t < PT; ++t)
 #pragma unroll
@@ -440,11 +441,20 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
     }
   };
   auto judge = [&](int ci) __attribute__((always_inline)) {
-    f16x2_t odd = f16x2_t{0, 0};
+    auto any = [&](int from, int to) {
+      f16x2_t odd = f16x2_t{0, 0};
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) odd = odd16<F16>(odd, held[i]);
-    if (__builtin_amdgcn_ballot_w64(odd[0] != odd[0] || odd[1] != odd[1]) != 0 && lane == 0)
-      s_odd[ci & 1] = ci;
+      for (int i = 0; i < PIECES; ++i)
+        if (i >= from && i < to) odd = odd16<F16>(odd, held[i]);
+      return __builtin_amdgcn_ballot_w64(odd[0] != odd[0] || odd[1] != odd[1]) != 0;
+    };
+    if (any(0, PIECES)) {
+      const bool keys = ONLY_STATE && any(0, PIECES - 1);
+      if (lane == 0) {
+        s_odd[ci & 1] = ci;
+        if (keys) s_keys[ci & 1] = ci;
+      }
+    }
   };
   if (nch > 0) {
     LOOM_WAIT_VMCNT(0);
@@ -460,7 +470,7 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
   // A chunk that holds an infinity or NaN, token by token as the recurrence has it, in
   // fp32: products with zeros and with the numbers that v is split into would make NaN of
   // infinities, and reach rows ahead of theirs.  Returns which of this lane's outputs are
-  // not finite, two bits each: 1 inf, 2 -inf, 3 NaN.
+  // infinite or NaN: a bit each, 8 for inf, 8 for -inf, 8 for NaN.
   auto by_token = [&](const lds_char_t* st, int n) __attribute__((always_inline)) {
     uint32_t bad = 0;
     const int ln = fresh(lane), r = ln & 15, g4 = ln >> 4;
@@ -489,14 +499,16 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
         }
       }
       if constexpr (!ONLY_STATE) {
-        o += __shfl_xor(o, 16);
-        o += __shfl_xor(o, 32);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {                   // column 4 g4 + e of token j
-          const float x = __shfl(o, 4 * g4 + e);
-          const uint32_t is = x == INFINITY ? 1u : x == -INFINITY ? 2u : x != x ? 3u : 0u;
-          if (r == (j & 15)) bad |= is << (2 * (4 * (j >> 4) + e));
-        }
+        // (which part of a sum over d was infinite or NaN tells what it is)
+        auto columns = [](bool is) {
+          const uint64_t m = __builtin_amdgcn_ballot_w64(is), x = m | m >> 32;
+          return (uint32_t)(x | x >> 16) & 0xffffu;
+        };
+        const uint32_t pos = columns(o == INFINITY), neg = columns(o == -INFINITY);
+        const uint32_t nan = columns(o != o) | (pos & neg);
+        if (r == (j & 15))                              // columns 4 g4 .. + 3 of token j
+          bad |= ((pos >> 4 * g4 & 15u) | (neg >> 4 * g4 & 15u) << 8 | (nan >> 4 * g4 & 15u) << 16)
+                 << 4 * (j >> 4);
       }
     }
     return bad;
@@ -550,8 +562,8 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
       if constexpr (decltype(is_odd)::value) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t is = bad >> (2 * (4 * it + e)) & 3u;
-          o[it][e] = is == 0 ? o[it][e] : is == 1 ? INFINITY : is == 2 ? -INFINITY : NAN;
+          const uint32_t is = bad >> (4 * it + e);
+          o[it][e] = is & 0x10000u ? NAN : is & 1u ? INFINITY : is & 0x100u ? -INFINITY : o[it][e];
         }
       }
       // ---- o[it][e] is token 16 it + r, column col0 + 4 g4 + e
@@ -562,9 +574,29 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
             u32x2_t{pack2<F16>(o[it][0], o[it][1]), pack2<F16>(o[it][2], o[it][3])};
     }
   };
+  // Whether by_token has to take the chunk, which holds infinities or NaN of q or k (keys)
+  // or of v: not where these only meet columns whose states are all NaN already, and stay so
+  // (else whatever follows a NaN would take as long).
+  auto matters = [&](const lds_char_t* lv, bool keys) __attribute__((always_inline)) {
+    const int g4 = fresh(lane) >> 4;
+    bool lost = true;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lost &= s[dt][i] != s[dt][i] || 32 * (dt >> 1) + 8 * g4 >= D;
+    const f16x2_t x =
+        odd16<F16>(f16x2_t{0, 0}, col_op(lv, VC{}, wave * 2 + (c4 >> 1), c4 & 1));
+    // a bit to each of the wave's columns, all of whose four lanes, or one of them
+    auto fold = [](uint64_t m) {
+      m |= m >> 32;
+      return (uint32_t)(m | m >> 16) & 0xffffu;
+    };
+    const uint32_t live = fold(__builtin_amdgcn_ballot_w64(!lost && ec < E)),
+                   odd = fold(__builtin_amdgcn_ballot_w64(x[0] != x[0] || x[1] != x[1]));
+    return (live & (keys ? 0xffffu : odd)) != 0;
+  };
   // The start of chunk ci: its copies have landed, those of chunk ci + 2 set out, and chunk
-  // ci + 1's scores are built.  Returns whether it holds infinities or NaN (the same in
-  // every wave).
+  // ci + 1's scores are built.  Returns whether by_token has to take it.
   lds_char_t* lq = nullptr;         // where the chunk lies
   float a = 0.f;                    // its decay
   auto begin = [&](int ci) __attribute__((always_inline)) {
@@ -600,11 +632,16 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
         judge(ci + 1);
       }
     }
-    return __builtin_amdgcn_readfirstlane(flag) == ci;
+    if (__builtin_amdgcn_readfirstlane(flag) != ci) return false;
+    return matters(lq + Q_BYTES + K_BYTES,
+                   __builtin_amdgcn_readfirstlane(s_keys[ci & 1]) == ci);
   };
-  // (One way out of the loop, at its end: with another the state would be copied in it.)
+  // By_token's chunks in a loop around the others'.  (Beside them in one, or with another way
+  // out of theirs than at its end, the state would be copied in it.)
   int ci = 0;
   bool go = nch > 0 && !begin(0);
+#pragma unroll 1
+  while (ci < nch) {
 #pragma unroll 1
   while (go) {
     const lds_char_t *const lk = lq + Q_BYTES, *const lv = lk + K_BYTES;
@@ -666,27 +703,26 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
 #pragma unroll
         for (int u = 0; u < 4; ++u) asm volatile("" : "+v"(s[d4 + u]));
     }
-    if constexpr (ONLY_STATE && F16)
+    if constexpr (ONLY_STATE)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) asm volatile("" : "+v"(s[dt]));
     if constexpr (!ONLY_STATE) finish(ci, std::false_type{}, 0);
     go = ++ci < nch;
     if (go) go = !begin(ci);
   }
-  // From a chunk with infinities or NaN on, by another loop: one that took such chunks
-  // beside the others would keep the state in registers of its own for them.
-  while (ci < nch) {
-    if constexpr (ONLY_STATE) {
-      by_token(lq, min(tokens - ci * kC, kC));
-    } else {
-      ahead_of(lq, [](int) {});
-      const uint32_t bad = by_token(lq, min(tokens - ci * kC, kC));
-      vf = col_op(lq + Q_BYTES + K_BYTES, VC{}, wave * 2 + (c4 >> 1), c4 & 1);
+  if (ci >= nch) break;
+  if constexpr (ONLY_STATE) {
+    by_token(lq, min(tokens - ci * kC, kC));
+  } else {
+    ahead_of(lq, [](int) {});
+    const uint32_t bad = by_token(lq, min(tokens - ci * kC, kC));
+    vf = col_op(lq + Q_BYTES + K_BYTES, VC{}, wave * 2 + (c4 >> 1), c4 & 1);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) vf[x] &= finite16<F16>(vf[x]);
-      finish(ci, std::true_type{}, bad);
-    }
-    if (++ci < nch) begin(ci);
+    for (int x = 0; x < 4; ++x) vf[x] &= finite16<F16>(vf[x]);
+    finish(ci, std::true_type{}, bad);
+  }
+  go = ++ci < nch;
+  if (go) go = !begin(ci);
   }
   if constexpr (ONLY_STATE) {
     if (!wanted) return;

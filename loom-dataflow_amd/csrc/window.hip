@@ -15,12 +15,14 @@
 // tokens and reads window + 64 keys, not window + 256.  A tile walks the blocks of 64
 // keys that any of its rows sees: the sinks', those at the edges of the window (masked),
 // then those that all rows see, by code of its own without the masks' branches.  Taken
-// together they cost those blocks the overlap of products and exponentials (window of
-// 4096 over 8192 tokens of 64 heads 1290 us against 1080; 1.01 PFLOP/s, as attention.hip
-// without a window; prompts of 4096 tokens of 128 heads under 1024 + 4 keys 379 against
-// 332: a sixth of its blocks are edges).  Few rows over many keys (a step) share a tile's
-// blocks between workgroups, which a second launch joins; a step is bound by streaming
-// the window (B32 G8 H4 f16 window 4096: 490 MB in 81 us, 6.0 TB/s).
+// together they cost those blocks the overlap of products and exponentials (when it was
+// built, a window of 4096 over 8192 tokens of 64 heads 1290 us against 1087, and prompts of
+// 4096 tokens of 128 heads under 1024 + 4 keys 379 against 332: a sixth of the blocks are
+// edges.  Now 1040 to 1110 us, 1.0 PFLOP/s as attention.hip without a window, and 309 to
+// 335).  Few rows over many keys (a step) share a tile's blocks between workgroups, which a
+// second launch joins; a step is bound by streaming the window (B32 G8 H4 f16 window 4096:
+// 490 MB in 82 us, 6.0 TB/s; of D 256, whose tiles of 32 rows take every vector register, 980
+// MB in 158 us).
 // Rounding: scores, bases and sums are fp32 (scale log2 e multiplies the fp32 score: q
 // times it, rounded, would cost a steep row two digits); p is rounded to 16 bits for its
 // product with v, and out divided by the sum of the rounded p.  f16, which loses bits
@@ -723,8 +725,9 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t T, int64_t S,
                int64_t sinks) {
   Shape s{};
   const int64_t rows = T * H, BG = B * G;
-  // The largest tile that leaves a workgroup to every CU (f16 B3 G2 H5 D80 T1001: 64 rows
-  // 27.6 us, 128 31.9, 32 29.4; B4 G8 H4 T4096 window 1024: 256 rows 380 us, 128 508).  Past
+  // The largest tile that leaves a workgroup to every CU (B4 G8 H4 T4096 window 1024: 256
+  // rows 310 us, 128 426; f16 B3 G2 H5 D80 T1001: 64 rows 19.9, 32 27.5, and 128, with 237
+  // workgroups, 18.1).  Past
   // D 128 two waves of 16 rows each would not hold a pair's 64 rows without spills.
   const int64_t most = D > 128 ? 128 : 256;
   s.tile = 32;
@@ -735,7 +738,7 @@ Shape shape_of(int64_t B, int64_t G, int64_t H, int64_t D, int64_t T, int64_t S,
   const int64_t span = std::min(S, std::min(window, S) + cdiv64(s.tile, H));
   const int64_t blocks = cdiv64(span, kKeys) + 1 + cdiv64(std::min(sinks, S), kKeys);
   // Splits of at least two blocks, as many as run at once (B1 H32 window 512: 5 splits and
-  // their join 10.9 us a call, one workgroup 12.6)
+  // their join 10.4 us a call, one workgroup 11.0)
   const int64_t slots = D > 128 ? 256 : 512;
   const int64_t want = std::min<int64_t>(slots / (BG * s.ntiles), blocks / 2);
   s.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));

@@ -172,3 +172,29 @@ def test_earlier_rows_keep_their_bits(lh, x, e):  # noqa: F811
         assert torch.equal(a[:, :at], b[:, :at])
         assert not torch.isfinite(b[0, at, 0]).all()
         assert torch.equal(a[:, :, 1:], b[:, :, 1:])          # other heads' rows
+
+
+@pytest.mark.parametrize("e", TYPES)
+@pytest.mark.parametrize("T", [220, 700])
+@pytest.mark.parametrize("D,E", [(64, 64), (128, 136), (40, 72)])
+def test_what_follows_lost_columns(lh, D, E, T, e):  # noqa: F811
+    """Infinities and NaN that meet columns of NaN, beside live ones, in chunks apart from
+    each other with ordinary ones between (T220: one piece, 700: segments)."""
+    for decay in (-0.01, -20.0):
+        print("lost columns", D, E, T, decay, e, flush=True)
+        t = make(3, 1, 2, D, E, T, None, TYPES[e], True, D + T)
+        t["log_decay"][:] = decay
+        t["q"][..., 0, :] = t["q"][..., 0, :].abs() + 0.25
+        k, v = t["k"], t["v"]
+        v[0, 40:, 0, :] = NAN                  # a sequence lost from token 40 on, in all columns
+        k[0, 100, 0, 3], v[0, 130, 0, 5] = INF, INF
+        v[1, 10:, 0, :16] = NAN                # a wave's columns, then infinities there and beside
+        v[1, 70, 0, 3], v[1, 100, 0, 20], v[1, 101, 0, 20], v[1, T - 1, 0, 30] = INF, INF, -INF, INF
+        k[1, 165, 0], v[1, 165, 0, E - 1] = 0.5, -INF
+        v[2, 33, 0, 1:E:2] = NAN               # every other column; then an infinite key
+        t["q"][2, 150, 0, 1, 2] = -INF
+        k[2, 190, 0, 4] = -INF
+        want, tol, end, etol = recurrence(t, None)
+        o, s = run(lh, t, None)
+        alike(s, end, etol, f"lost columns D{D} E{E} T{T} {decay} {e} state")
+        alike(o, want, tol, f"lost columns D{D} E{E} T{T} {decay} {e} out")
