@@ -145,7 +145,7 @@ LOOM_DEV const char* uniform(const char* p) {
 // rate of a large copy.  B8 G32 of 1024 to 4096 tokens 197 to 206 us (738 MB, 3.7 TB/s: the
 // longest prompt's 128 chunks in a row, while the CUs of shorter ones idle), B1 G32 of
 // 32768 370 to 395 us (1.08 GB, and k, v once more in the first launch, 0.47 GB); key dims
-// of 256: B4 G32 256 x 256 T2048 189 us, in f16 489 (28 spilled registers).  Measured while
+// of 256: B4 G32 256 x 256 T2048 189 us, in f16 493 (37 spilled registers).  Measured while
 // it was built, at B8 G32: chunks of 64 tokens by four waves 366 us, by eight 249 (the 64 x
 // 64 scores cost more than they save); of 32 by four waves of 32 columns 251 to 257, by
 // eight of 16 216; then direct reads of 16 bytes (not two of 8, which the compiler joined
