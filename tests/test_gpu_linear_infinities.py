@@ -198,3 +198,17 @@ def test_what_follows_lost_columns(lh, D, E, T, e):  # noqa: F811
         o, s = run(lh, t, None)
         alike(s, end, etol, f"lost columns D{D} E{E} T{T} {decay} {e} state")
         alike(o, want, tol, f"lost columns D{D} E{E} T{T} {decay} {e} out")
+
+
+def test_finite_values_that_look_like_infinities(lh):  # noqa: F811
+    """bf16 values past 2^121 have the bits of f16's infinities and NaN: finite all the same."""
+    for T in (70, 700):
+        t = make(2, 1, 2, 64, 64, T, None, torch.bfloat16, True, T)
+        t["v"][0, 20, 0, 5], t["v"][1, T - 2, 0, 6] = 2.0 ** 121, -2.0 ** 123
+        t["k"][0, 33, 0, 7] = 2.0 ** 121
+        t["v"][0, 33, 0] = 2.0 ** -8
+        want, tol, end, etol = recurrence(t, None)
+        assert torch.isfinite(want).all() and float(want.abs().max()) < 2.0 ** 127
+        o, s = run(lh, t, None)
+        alike(s, end, etol, f"huge T{T} state")
+        alike(o, want, tol, f"huge T{T} out")
