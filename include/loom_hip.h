@@ -370,10 +370,11 @@ size_t loom_hip_window_attention_workspace_bytes(int64_t B, int64_t G, int64_t H
  * infinities) does not reach the row.  Scores, their maxima and sums are fp32; every
  * weight is rounded to the 16-bit type for its product with v, and out, divided by the
  * sum of the rounded weights, once more.  So an infinite v that a row sees makes it
- * infinite, or NaN where the key's weight rounds to zero.  T = 1 is a decoding step.  `scale` is finite
- * and positive, window at least 1 (from S on: every key up to p), sinks at least 0,
- * D a multiple of 8 up to 256 (else LOOM_HIP_EUNSUP), B*G <= 65535, S and T*H at
- * most 2^29, B*G*ceil(T*H/32) at most 2^23; S not a multiple of 8 needs D*S < 2^30.
+ * infinite, or NaN where the key's weight rounds to zero.  T = 1 is a decoding step.
+ * `scale` is finite and positive, window at least 1 (from S on: every key up to p),
+ * sinks at least 0, D a multiple of 8 up to 256 (else LOOM_HIP_EUNSUP), B*G <= 65535,
+ * S and T*H at most 2^29, B*G*ceil(T*H/32) at most 2^23; S not a multiple of 8 needs
+ * D*S < 2^30.
  * out and the workspace overlap neither the other tensors nor each other, except
  * that out may be q.  Equal calls give equal bits. */
 int loom_hip_window_attention(const void* k, const void* v, const void* q, const void* lens,

@@ -145,7 +145,7 @@ LOOM_DEV const char* uniform(const char* p) {
 // rate of a large copy.  B8 G32 of 1024 to 4096 tokens 197 to 206 us (738 MB, 3.7 TB/s: the
 // longest prompt's 128 chunks in a row, while the CUs of shorter ones idle), B1 G32 of
 // 32768 370 to 395 us (1.08 GB, and k, v once more in the first launch, 0.47 GB); key dims
-// of 256: B4 G32 256 x 256 T2048 189 us, in f16 493 (37 spilled registers).  Measured while
+// of 256: B4 G32 256 x 256 T2048 189 us, in f16 274.  Measured while
 // it was built, at B8 G32: chunks of 64 tokens by four waves 366 us, by eight 249 (the 64 x
 // 64 scores cost more than they save); of 32 by four waves of 32 columns 251 to 257, by
 // eight of 16 216; then direct reads of 16 bytes (not two of 8, which the compiler joined
@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
     float big = 0.f;
 #pragma unroll
     for (int t = 0; t < PT; ++t) big = largest(largest(big, x[t][0], x[t][1]), x[t][2], x[t][3]);
-    if (__builtin_amdgcn_ballot_w64(!(big < INFINITY)) != 0 && lane == 0) s_odd[to] = s_keys[to] = ci;
+    if (__builtin_amdgcn_ballot_w64(!(big < INFINITY)) != 0 && lane == 0)
+      s_odd[to] = s_keys[to] = ci;
 #pragma unroll
     for (int t = 0; t < PT; ++t)
 #pragma unroll
@@ -478,16 +479,18 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
     for (int j = 0; j < n; ++j) {
       const lds_char_t* const kr = st + Q_BYTES + j * KROW;
       const lds_char_t* const vr = st + Q_BYTES + K_BYTES + j * VROW;
-      const float v = lo16<F16>(*reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(
+      typedef const __attribute__((address_space(3))) uint16_t* at16_t;
+      typedef const __attribute__((address_space(3))) u32x2_t* at64_t;
+      const float v = lo16<F16>(*reinterpret_cast<at16_t>(
           vr + ((wave * 2 + (r >> 3)) ^ row_swz<SL>(j)) * 16 + (r & 7) * 2));
       float o = 0.f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const int at = ((4 * (dt >> 1) + g4) ^ row_swz<DK>(j)) * 16 + 8 * (dt & 1);
-        const u32x2_t k = *reinterpret_cast<const __attribute__((address_space(3))) u32x2_t*>(kr + at);
+        const u32x2_t k = *reinterpret_cast<at64_t>(kr + at);
         u32x2_t q = u32x2_t{0u, 0u};
         if constexpr (!ONLY_STATE)
-          q = *reinterpret_cast<const __attribute__((address_space(3))) u32x2_t*>(st + j * KROW + at);
+          q = *reinterpret_cast<at64_t>(st + j * KROW + at);
         lds_order();      // (one tile's reads at a time: registers)
         if (32 * (dt >> 1) + 8 * g4 >= D) continue;     // (rows past D stay zeros)
 #pragma unroll
@@ -514,6 +517,7 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
     return bad;
   };
   int stage = 0;
+  // (one of each for both kinds of chunks: as their own, the kernels of D 256 spill)
   f32x4_t o[kIT];
   u32x4_t vf;               // v as an operand
   // ---- S^T Q^T of the state before a chunk, times scale a^(i+1), into o.  Products that
@@ -636,14 +640,8 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
     return matters(lq + Q_BYTES + K_BYTES,
                    __builtin_amdgcn_readfirstlane(s_keys[ci & 1]) == ci);
   };
-  // By_token's chunks in a loop around the others'.  (Beside them in one, or with another way
-  // out of theirs than at its end, the state would be copied in it.)
-  int ci = 0;
-  bool go = nch > 0 && !begin(0);
-#pragma unroll 1
-  while (ci < nch) {
-#pragma unroll 1
-  while (go) {
+  // A chunk without infinities or NaN that matter
+  auto usual = [&](int ci) __attribute__((always_inline)) {
     const lds_char_t *const lk = lq + Q_BYTES, *const lv = lk + K_BYTES;
 
     // ---- v as an operand, and a^(C-1-j) v as a sum of 16-bit numbers
@@ -707,22 +705,34 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) asm volatile("" : "+v"(s[dt]));
     if constexpr (!ONLY_STATE) finish(ci, std::false_type{}, 0);
+  };
+  // One with some
+  auto spoiled = [&](int ci) __attribute__((always_inline)) {
+    if constexpr (!ONLY_STATE) ahead_of(lq, [](int) {});
+    const uint32_t bad = by_token(lq, min(tokens - ci * kC, kC));
+    if constexpr (!ONLY_STATE) {
+      vf = col_op(lq + Q_BYTES + K_BYTES, VC{}, wave * 2 + (c4 >> 1), c4 & 1);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) vf[x] &= finite16<F16>(vf[x]);
+      finish(ci, std::true_type{}, bad);
+    }
+  };
+  // The latter in a loop around the others.  (Beside them in one, or with another way out
+  // of theirs than at its end, the state would be copied in it.)
+  int ci = 0;
+  bool go = nch > 0 && !begin(0);
+#pragma unroll 1
+  while (ci < nch) {
+#pragma unroll 1
+    while (go) {
+      usual(ci);
+      go = ++ci < nch;
+      if (go) go = !begin(ci);
+    }
+    if (ci >= nch) break;
+    spoiled(ci);
     go = ++ci < nch;
     if (go) go = !begin(ci);
-  }
-  if (ci >= nch) break;
-  if constexpr (ONLY_STATE) {
-    by_token(lq, min(tokens - ci * kC, kC));
-  } else {
-    ahead_of(lq, [](int) {});
-    const uint32_t bad = by_token(lq, min(tokens - ci * kC, kC));
-    vf = col_op(lq + Q_BYTES + K_BYTES, VC{}, wave * 2 + (c4 >> 1), c4 & 1);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) vf[x] &= finite16<F16>(vf[x]);
-    finish(ci, std::true_type{}, bad);
-  }
-  go = ++ci < nch;
-  if (go) go = !begin(ci);
   }
   if constexpr (ONLY_STATE) {
     if (!wanted) return;
@@ -735,8 +745,8 @@ __global__ void __launch_bounds__(64 * W, (ONLY_STATE ? DK < 256 : DK == 64 && !
 // One token.  L lanes of four columns to a row of the state, 256 / L rows at once, 16 of
 // them in flight to a thread.  The state is stored past the caches: a program's layers
 // have more of it than these hold, so it comes from memory the next time (B64 G32 128 x 128,
-// three states in turn: 268 MB in 44.7 us, 6.0 TB/s, against 59.3 with ordinary stores; one
-// state over and over 44.5 against 40.2).
+// three states in turn: 268 MB in 44.9 us, 6.0 TB/s, against 59.4 with ordinary stores; one
+// state over and over 44.7 against 40.5).
 template <bool F16>
 __global__ void __launch_bounds__(256) linear_step_kernel(LinearParams p, int L) {
   __shared__ float s_q[256], s_k[256];
