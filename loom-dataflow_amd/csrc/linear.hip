@@ -142,7 +142,7 @@ LOOM_DEV const char* uniform(const char* p) {
 // range.
 // What bounds it: a chunk of 128 x 128 takes a CU 1.4 us by itself (24 + 8 products of 16
 // cycles and 200 other vector instructions to each of 8 waves), its 32 KB 1.6 us at the
-// rate of a large copy.  B8 G32 of 1024 to 4096 tokens 197 to 206 us (738 MB, 3.7 TB/s: the
+// rate of a large copy.  B8 G32 of 1024 to 4096 tokens 195 to 206 us (738 MB, 3.7 TB/s: the
 // longest prompt's 128 chunks in a row, while the CUs of shorter ones idle), B1 G32 of
 // 32768 370 to 395 us (1.08 GB, and k, v once more in the first launch, 0.47 GB); key dims
 // of 256: B4 G32 256 x 256 T2048 189 us, in f16 274.  Measured while
